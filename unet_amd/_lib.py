@@ -135,6 +135,11 @@ PROTOTYPES = {
                                         C.POINTER(MiTensor), C.POINTER(MiTensor), C.c_float, C.c_uint64, C.c_uint32, _P]),
     "mi_instnorm_prelu_bwd": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int, C.POINTER(MiTensor), C.POINTER(MiTensor),
                                         _P, _P, _P, _P, C.POINTER(MiTensor), C.c_float, C.c_uint64, C.c_uint32, _P]),
+    "mi_groupnorm_act_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int]),
+    "mi_groupnorm_act_fwd": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, C.POINTER(MiTensor), _P, _P, C.c_int, _P,
+                                       C.POINTER(MiTensor), C.POINTER(MiTensor), C.c_float, _P, _P, _P]),
+    "mi_groupnorm_act_bwd": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, C.POINTER(MiTensor), C.POINTER(MiTensor),
+                                       _P, _P, _P, C.c_int, _P, C.POINTER(MiTensor), _P, _P, _P, _P, _P]),
 }
 
 
@@ -181,6 +186,24 @@ def current_stream(device) -> int:
     import torch
 
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device):
+    """Context in which launches go to ``device``: a kernel goes to the process's current device, whatever the stream."""
+    import torch
+
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 LABEL_DTYPES = None

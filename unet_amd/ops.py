@@ -1,5 +1,5 @@
 """Operator-level Python bindings (channels-last tensors) over the C ABI: convolution forward / data
-gradient / weight gradient and instance-norm + PReLU.  Used by the operator parity tests and by
+gradient / weight gradient, instance-norm + PReLU and group norm + activation.  Used by the operator parity tests and by
 callers that want to assemble other networks from the same kernels.
 
 Tensors are ``[N, (D,) H, W, C]`` contiguous, dtype ``torch.bfloat16`` or ``torch.float32``.
@@ -189,3 +189,122 @@ def instnorm_prelu_bwd(dy, raw, stats, alpha, dropout=0.0, seed=0, layer=0):
                                          float(dropout), C.c_uint64(seed), layer, _lib.current_stream(raw.device)),
                "mi_instnorm_prelu_bwd")
     return dx, dalpha
+
+
+_ACT = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "prelu": 4}
+
+
+def _pixels(t, name, like=None):
+    """``t`` [N, .., C] as (tensor, pitch): pixels at one common distance, channels side by side.  A slice of the channels
+    of a wider tensor is taken as it lies; any other order of the memory is copied into a dense tensor."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if like is not None:
+        if t.shape != like.shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
+        if t.dtype != like.dtype or t.device != like.device:
+            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    c, pitch, span = t.shape[-1], None, 1
+    dense = t.stride(-1) == 1 or c == 1
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if pitch is None:
+            pitch = stride
+        dense = dense and stride == pitch * span
+        span *= size
+    if pitch is None:
+        pitch = c
+    if not dense or pitch < c or pitch > 0x7FFFFFFF:
+        return t.contiguous(), c
+    return t, pitch
+
+
+def _view(t, pitch):
+    m = _lib.MiTensor()
+    m.ptr, m.pitch = t.data_ptr(), pitch
+    return m
+
+
+def _channel_param(t, n, x, name):
+    if t is None:
+        return None
+    if t.numel() != n or t.dim() != 1:
+        raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
+    if t.device != x.device:
+        raise ValueError(f"{name} is on {t.device}, expected {x.device}")
+    return t.detach().contiguous().float()
+
+
+def _groupnorm_args(x, groups, weight, bias, act, alpha):
+    if not isinstance(x, torch.Tensor) or x.dim() < 2:
+        raise ValueError("x must be a channels-last tensor [N, .., C]")
+    if not x.is_cuda:
+        raise RuntimeError("unet_amd.ops run on an AMD GPU only (no CPU or eager fallback)")
+    if x.dtype not in _DT:
+        raise ValueError(f"x must be torch.float32 or torch.bfloat16, got {x.dtype}")
+    if act not in _ACT:
+        raise ValueError(f"act must be one of {sorted(_ACT)}, got {act!r}")
+    if (alpha is None) == (act == "prelu"):
+        raise ValueError("alpha (one slope) belongs to act='prelu' and to no other")
+    nb, c = x.shape[0], x.shape[-1]
+    groups = int(groups)
+    if c < 1 or groups < 1 or c % groups:
+        raise ValueError(f"{groups} groups do not divide {c} channels")
+    npix = 1
+    for v in x.shape[1:-1]:
+        npix *= v
+    if npix == 0:
+        raise ValueError("an image without pixels has no mean")
+    return (nb, npix, c, groups, _channel_param(weight, c, x, "weight"), _channel_param(bias, c, x, "bias"),
+            _channel_param(alpha, 1, x, "alpha"))
+
+
+def groupnorm_act_fwd(x, groups, weight=None, bias=None, act="silu", alpha=None, res=None, eps=1e-5):
+    """``act(F.group_norm(x, groups, weight, bias, eps)) (+ res)`` of a channels-last ``x`` [N, .., C]; ``act`` is one of
+    "none", "relu", "silu", "gelu" (erf) and "prelu" (with its one slope ``alpha`` [1]).  ``weight`` and ``bias`` [C] and
+    ``alpha`` are read as fp32.  Returns (y, stats [N, groups, 2] fp32: mean and 1 / sqrt(variance + eps), for the backward call)."""
+    nb, npix, c, groups, weight, bias, alpha = _groupnorm_args(x, groups, weight, bias, act, alpha)
+    x, xp = _pixels(x, "x")
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(nb, groups, 2, dtype=torch.float32, device=x.device)
+    if res is not None:
+        res, rp = _pixels(res, "res", x)
+    if nb == 0:
+        return out, stats
+    lib, dt = _lib.load(), _DT[x.dtype]
+    with _lib.on_device(x.device):
+        ws = torch.empty(lib.mi_groupnorm_act_workspace_bytes(dt, nb, npix, c, groups, 0), dtype=torch.uint8, device=x.device)
+        tx, to, tr = _view(x, xp), _view(out, c), _view(res, rp) if res is not None else None
+        _lib.check(lib.mi_groupnorm_act_fwd(dt, nb, npix, c, groups, C.byref(tx), _lib.ptr(weight), _lib.ptr(bias), _ACT[act],
+                                            _lib.ptr(alpha), C.byref(tr) if tr is not None else None, C.byref(to), float(eps),
+                                            stats.data_ptr(), ws.data_ptr(), _lib.current_stream(x.device)), "mi_groupnorm_act_fwd")
+    return out, stats
+
+
+def groupnorm_act_bwd(dy, x, stats, groups, weight=None, bias=None, act="silu", alpha=None):
+    """Gradients of ``groupnorm_act_fwd`` from its input and its ``stats``: (dx, dweight, dbias, dalpha), fp32 for the
+    parameters and None for those that were not given.  The gradient with respect to ``res`` is ``dy`` itself."""
+    nb, npix, c, groups, weight, bias, alpha = _groupnorm_args(x, groups, weight, bias, act, alpha)
+    dy, dp = _pixels(dy, "dy", x)
+    x, xp = _pixels(x, "x")
+    if tuple(stats.shape) != (nb, groups, 2) or stats.dtype != torch.float32 or stats.device != x.device:
+        raise ValueError(f"stats must be the fp32 tensor [{nb}, {groups}, 2] of the forward call")
+    stats = stats.contiguous()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    new = torch.zeros if nb == 0 else torch.empty
+    dw = new(c, dtype=torch.float32, device=x.device) if weight is not None else None
+    db = new(c, dtype=torch.float32, device=x.device) if bias is not None else None
+    da = new(1, dtype=torch.float32, device=x.device) if alpha is not None else None
+    if nb == 0:
+        return dx, dw, db, da
+    lib, dt = _lib.load(), _DT[x.dtype]
+    with _lib.on_device(x.device):
+        ws = torch.empty(lib.mi_groupnorm_act_workspace_bytes(dt, nb, npix, c, groups, 1), dtype=torch.uint8, device=x.device)
+        tdy, tx, tdx = _view(dy, dp), _view(x, xp), _view(dx, c)
+        _lib.check(lib.mi_groupnorm_act_bwd(dt, nb, npix, c, groups, C.byref(tdy), C.byref(tx), stats.data_ptr(), _lib.ptr(weight),
+                                            _lib.ptr(bias), _ACT[act], _lib.ptr(alpha), C.byref(tdx), _lib.ptr(dw), _lib.ptr(db),
+                                            _lib.ptr(da), ws.data_ptr(), _lib.current_stream(x.device)), "mi_groupnorm_act_bwd")
+    return dx, dw, db, da
