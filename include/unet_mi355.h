@@ -320,6 +320,31 @@ int mi_groupnorm_act_bwd(int dtype, int nb, int64_t npix, int c, int groups, con
                          const float* stats, const float* weight, const float* bias, int act, const float* alpha,
                          const mi_tensor* dx, float* dweight, float* dbias, float* dalpha, void* workspace, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Student training on a teacher's top logits.  No counterpart in the reference, whose teacher's predictions become hard
+ * labels on disk; these keep what the teacher knew about the other classes.  Rows: the pixels of a channels-last tensor of
+ * class logits, [rows][pitch] with v <= pitch classes used.
+ * ------------------------------------------------------------------------------------------ */
+/* values[r][j], index[r][j]: the k largest logits of row r, largest first, equal ones by ascending class (-0 equals 0, NaN counts
+ * as the largest).  values has the type of the logits.  1 <= k <= 256, k <= v <= 2^28. */
+int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, void* values, int32_t* index,
+                  void* stream);
+/* Row loss T^2 * KL(q || p): q = softmax(teacher / T) over the used slots of the row's list, p = softmax(logits / T) over all v
+ * classes.  A slot is unused when its index lies outside [0, v) or its teacher logit is -inf; a class may be listed
+ * more than once (its weights add).  Rows without a used slot have loss 0 and gradient 0, whatever their logits are.
+ * teacher [rows][k] (teacher_dtype 0 fp32 | 1 bf16), index [rows][k] (index_dtype 2 int64 | 3 int32), 1 <= k <= 256.
+ * reduction: 0 none (loss [rows]), 1 mean over the rows with a used slot (0 if there are none), 2 sum (loss [1]).
+ * `saved` (mi_distill_loss_saved_bytes, 8-byte aligned; 0: bad sizes) is written by the forward call and read by the backward call of the same
+ * arguments.  grad_out: [rows] or [1], on the device; dlogits [rows][dpitch], type of the logits, v classes written.
+ * Results do not depend on the order in which workgroups run. */
+size_t mi_distill_loss_saved_bytes(int dtype, int64_t rows, int v, int k);
+int mi_distill_loss_fwd(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
+                        const void* teacher, int index_dtype, const void* index, float temperature, int reduction, float* loss,
+                        void* saved, void* stream);
+int mi_distill_loss_bwd(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
+                        const void* teacher, int index_dtype, const void* index, float temperature, int reduction,
+                        const float* grad_out, const void* saved, int64_t dpitch, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,7 +3,7 @@ kernels behind a C ABI, with the reference's Python surface (MONAI-style ``UNet`
 ``DiceMetric``, ``sliding_window_inference``) on top.  GPU only: no CPU or eager fallback.
 """
 from .nets import UNet  # noqa: F401
-from .losses import DiceCELoss, DiceLoss  # noqa: F401
+from .losses import DiceCELoss, DiceLoss, TopLogitDistillationLoss  # noqa: F401
 from .metrics import DiceMetric, calculate_dice_score, confusion_counts  # noqa: F401
 from .inferers import sliding_window_inference, window_starts, shard_range  # noqa: F401
 from .transforms import Activations, AsDiscrete, Compose, decollate_batch  # noqa: F401

@@ -140,6 +140,12 @@ PROTOTYPES = {
                                        C.POINTER(MiTensor), C.POINTER(MiTensor), C.c_float, _P, _P, _P]),
     "mi_groupnorm_act_bwd": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, C.POINTER(MiTensor), C.POINTER(MiTensor),
                                        _P, _P, _P, C.c_int, _P, C.POINTER(MiTensor), _P, _P, _P, _P, _P]),
+    "mi_top_logits": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, _P, _P, _P]),
+    "mi_distill_loss_saved_bytes": (C.c_size_t, [C.c_int, C.c_int64, C.c_int, C.c_int]),
+    "mi_distill_loss_fwd": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, C.c_int, _P, C.c_int, _P, C.c_float,
+                                      C.c_int, _P, _P, _P]),
+    "mi_distill_loss_bwd": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, C.c_int, _P, C.c_int, _P, C.c_float,
+                                      C.c_int, _P, _P, C.c_int64, _P, _P]),
 }
 
 

@@ -17,7 +17,7 @@ CSRC = HERE / "csrc"
 LIBDIR = HERE / "lib"
 OBJDIR = HERE / "lib" / "obj"
 LIBNAME = "libunet_mi355.so"
-SOURCES = ["igemm.hip", "igemm_dma.hip", "conv2d.hip", "wgrad2.hip", "wgrad3.hip", "norm.hip", "small.hip", "loss.hip", "pipeline.hip", "ops.hip", "engine.hip", "comm.hip", "groupnorm.hip"]
+SOURCES = ["igemm.hip", "igemm_dma.hip", "conv2d.hip", "wgrad2.hip", "wgrad3.hip", "norm.hip", "small.hip", "loss.hip", "pipeline.hip", "ops.hip", "engine.hip", "comm.hip", "groupnorm.hip", "distill.hip", "toplogits.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-munsafe-fp-atomics",
          # no packed fp32 instructions: some of their forms have given wrong results on this part now and then
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

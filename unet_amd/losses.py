@@ -1,6 +1,7 @@
 """``DiceLoss`` / ``DiceCELoss`` with MONAI's call surface (reference/train.py:88,116,142), computed by
 single-pass HIP reductions: per-sample sums of sigmoid(z)*t, sigmoid(z), t and the BCE-with-logits
-terms in one kernel, the gradient w.r.t. the logits in another.
+terms in one kernel, the gradient w.r.t. the logits in another.  ``TopLogitDistillationLoss`` trains a student on
+the top logits of a teacher.
 """
 from __future__ import annotations
 
@@ -8,6 +9,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .ops import _DT, _pixels
 
 
 class _DiceCEFunction(torch.autograd.Function):
@@ -107,3 +109,91 @@ class DiceLoss(DiceCELoss):
                          softmax=softmax, other_act=other_act, squared_pred=squared_pred, jaccard=jaccard,
                          reduction=reduction, smooth_nr=smooth_nr, smooth_dr=smooth_dr, batch=batch,
                          lambda_dice=1.0, lambda_ce=0.0, fold_label_two=fold_label_two)
+
+
+_REDUCTION = {"none": 0, "mean": 1, "sum": 2}
+_INDEX = {torch.int64: 2, torch.int32: 3}
+
+
+class _DistillFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher, index, temperature, red):
+        lib, dev = _lib.load(), logits.device
+        z, pitch = _pixels(logits, "input")
+        v, k = z.shape[-1], index.shape[-1]
+        rows = index.numel() // k
+        loss = torch.empty(index.shape[:-1] if red == 0 else (), dtype=torch.float32, device=dev)
+        args = (_DT[z.dtype], rows, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(), _INDEX[index.dtype],
+                index.data_ptr(), temperature, red)
+        with _lib.on_device(dev):
+            saved = torch.empty(lib.mi_distill_loss_saved_bytes(args[0], rows, v, k), dtype=torch.uint8, device=dev)
+            _lib.check(lib.mi_distill_loss_fwd(*args, loss.data_ptr(), saved.data_ptr(), _lib.current_stream(dev)), "mi_distill_loss_fwd")
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, teacher, index, saved)
+            ctx.cfg = (temperature, red)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        logits, teacher, index, saved = ctx.saved_tensors
+        temperature, red = ctx.cfg
+        lib, dev = _lib.load(), logits.device
+        z, pitch = _pixels(logits, "input")
+        v, k = z.shape[-1], index.shape[-1]
+        dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
+        g = gout.contiguous().float()
+        with _lib.on_device(dev):
+            _lib.check(lib.mi_distill_loss_bwd(_DT[z.dtype], index.numel() // k, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(),
+                                               _INDEX[index.dtype], index.data_ptr(), temperature, red, g.data_ptr(), saved.data_ptr(),
+                                               v, dz.data_ptr(), _lib.current_stream(dev)), "mi_distill_loss_bwd")
+        return dz, None, None, None, None
+
+
+class TopLogitDistillationLoss(nn.Module):
+    """Trains a student on the top logits of a teacher (``ops.top_logits``):
+    ``temperature**2 * KL(q || softmax(input / temperature))`` per pixel, where ``q`` is the softmax of the pixel's listed
+    teacher logits over ``temperature``.
+
+    ``forward(input, teacher_logits, teacher_index)``: ``input`` [.., V] class logits of the student, channels last, fp32 or
+    bf16 (other types are read as fp32); ``teacher_logits`` [.., k] (fp32, bf16; others are read as fp32) and ``teacher_index``
+    [.., k] (int32 or int64), k at most 256.  A slot whose index lies outside [0, V), or whose logit is -inf, is unused: -1
+    fills up short lists and leaves out pixels.  The weights of a class listed twice add.  ``reduction``: "mean" over the pixels with a used slot (0 if
+    there are none), "sum", or "none" (one loss per pixel, 0 where no slot is used).  The gradient flows to ``input`` alone.
+    """
+
+    def __init__(self, temperature=1.0, reduction="mean"):
+        super().__init__()
+        temperature = float(temperature)
+        if not 0.0 < temperature < float("inf"):
+            raise ValueError(f"temperature must be positive and finite, got {temperature}")
+        if reduction not in _REDUCTION:
+            raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, input: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor) -> torch.Tensor:
+        x = input.as_subclass(torch.Tensor) if type(input) is not torch.Tensor else input
+        t, i = teacher_logits, teacher_index
+        if x.dim() < 1 or t.shape != i.shape or t.shape[:-1] != x.shape[:-1] or t.dim() != x.dim():
+            raise ValueError(f"input [.., V] and the teacher's lists [.., k] must agree in front of the last dimension, got {tuple(x.shape)}, "
+                             f"{tuple(t.shape)} and {tuple(i.shape)}")
+        if x.shape[-1] < 1 or not 1 <= i.shape[-1] <= 256:
+            raise ValueError(f"the lists must have 1 .. 256 slots and the input at least one class, got {i.shape[-1]} and {x.shape[-1]}")
+        if i.dtype not in _INDEX:
+            raise ValueError(f"teacher_index must be torch.int32 or torch.int64, got {i.dtype}")
+        if not x.is_floating_point() or not t.is_floating_point():
+            raise ValueError(f"input and teacher_logits must be floating point, got {x.dtype} and {t.dtype}")
+        if not x.is_cuda:
+            raise RuntimeError("unet_amd losses run on an AMD GPU only (no CPU or eager fallback)")
+        if t.device != x.device or i.device != x.device:
+            raise ValueError(f"the teacher's lists are on {t.device} and {i.device}, expected {x.device}")
+        if x.dtype not in _DT:
+            x = x.float()
+        t = t.detach()
+        if t.dtype not in _DT:
+            t = t.float()
+        red = _REDUCTION[self.reduction]
+        if i.numel() == 0:
+            total = x.float().sum(-1)                              # nothing to learn from: zeros that know the input
+            return total if red == 0 else total.sum()
+        return _DistillFunction.apply(x, t.contiguous(), i.contiguous(), self.temperature, red)

@@ -1,5 +1,5 @@
 """Operator-level Python bindings (channels-last tensors) over the C ABI: convolution forward / data
-gradient / weight gradient, instance-norm + PReLU and group norm + activation.  Used by the operator parity tests and by
+gradient / weight gradient, instance-norm + PReLU, group norm + activation and the top logits of a teacher.  Used by the operator parity tests and by
 callers that want to assemble other networks from the same kernels.
 
 Tensors are ``[N, (D,) H, W, C]`` contiguous, dtype ``torch.bfloat16`` or ``torch.float32``.
@@ -308,3 +308,28 @@ def groupnorm_act_bwd(dy, x, stats, groups, weight=None, bias=None, act="silu", 
                                             _lib.ptr(bias), _ACT[act], _lib.ptr(alpha), C.byref(tdx), _lib.ptr(dw), _lib.ptr(db),
                                             _lib.ptr(da), ws.data_ptr(), _lib.current_stream(x.device)), "mi_groupnorm_act_bwd")
     return dx, dw, db, da
+
+
+def top_logits(logits, k):
+    """The ``k`` (at most 256) largest of the class logits [.., V] of every pixel, largest first, equal ones by ascending class:
+    (values [.., k] of the logits' type, index [.., k] int32), the lists that ``TopLogitDistillationLoss`` reads.
+    NaN counts as the largest value."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
+        raise ValueError("logits must be a tensor [.., V]")
+    if not logits.is_cuda:
+        raise RuntimeError("unet_amd.ops run on an AMD GPU only (no CPU or eager fallback)")
+    if logits.dtype not in _DT:
+        raise ValueError(f"logits must be torch.float32 or torch.bfloat16, got {logits.dtype}")
+    v, k = logits.shape[-1], int(k)
+    if not 1 <= k <= min(v, 256):
+        raise ValueError(f"k must be in 1 .. {min(v, 256)} for {v} classes, got {k}")
+    x, pitch = _pixels(logits, "logits")
+    shape = logits.shape[:-1] + (k,)
+    values = torch.empty(shape, dtype=x.dtype, device=x.device)
+    index = torch.empty(shape, dtype=torch.int32, device=x.device)
+    rows = index.numel() // k
+    if rows:
+        with _lib.on_device(x.device):
+            _lib.check(_lib.load().mi_top_logits(_DT[x.dtype], rows, v, pitch, x.data_ptr(), k, values.data_ptr(), index.data_ptr(),
+                                                 _lib.current_stream(x.device)), "mi_top_logits")
+    return values, index
