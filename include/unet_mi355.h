@@ -308,7 +308,7 @@ int mi_instnorm_prelu_bwd(int dtype, int nb, int64_t npix, int c, const mi_tenso
  * xh = (x - mean) * rstd over the pixels and the c / groups channels of a group (biased variance, eps under the root).
  * act: 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 prelu (one slope, alpha[0]; NULL for the others).  weight and bias: [c] fp32,
  * each may be NULL (1 and 0).  stats: [nb][groups][2] fp32 {mean, rstd}, written by the forward call and read by the
- * backward call.  workspace: mi_groupnorm_act_workspace_bytes (0: bad arguments).  1 <= c <= 8192, groups <= 2048, any
+ * backward call.  workspace: mi_groupnorm_act_workspace_bytes (0: bad arguments), 16-byte aligned, stats 8-byte.  1 <= c <= 8192, groups <= 2048, any
  * pixel count and pitch; tensors may not overlap.  Backward: dx, and where not NULL dweight [c], dbias [c] and dalpha [1],
  * all written (not accumulated); the gradient with respect to res is dy itself.  Results do not depend on the order in which
  * workgroups run. */

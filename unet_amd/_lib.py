@@ -10,6 +10,8 @@ import ctypes as C
 import os
 from pathlib import Path
 
+import torch
+
 _LIB_PATH = Path(__file__).resolve().parent / "lib" / "libunet_mi355.so"
 _lib = None
 
@@ -189,9 +191,13 @@ def ptr(t) -> int:
 
 
 def current_stream(device) -> int:
-    import torch
-
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def stream_of(device) -> int:
+    """The current stream of a tensor's device (one with an index), without building a ``torch.cuda.Stream`` object:
+    1 us less host time per call."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class _Here:
@@ -207,8 +213,6 @@ _HERE = _Here()
 
 def on_device(device):
     """Context in which launches go to ``device``: a kernel goes to the process's current device, whatever the stream."""
-    import torch
-
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
@@ -216,8 +220,6 @@ LABEL_DTYPES = None
 
 
 def label_dtype_code(t) -> int:
-    import torch
-
     global LABEL_DTYPES
     if LABEL_DTYPES is None:
         LABEL_DTYPES = {torch.float32: 0, torch.uint8: 1, torch.int64: 2, torch.int32: 3}

@@ -451,6 +451,7 @@ int mi_distill_loss_fwd(int dtype, int64_t rows, int v, int64_t pitch, const voi
                         void* saved, void* stream) {
     if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, reduction)) return r;
     MI_CHECK(loss && saved, "null argument");
+    MI_CHECK((uintptr_t)saved % 8 == 0 && (uintptr_t)loss % 4 == 0, "saved or loss is not aligned");
     const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);
     DistParams p;
     fill(p, q, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, reduction, saved);
@@ -475,6 +476,7 @@ int mi_distill_loss_bwd(int dtype, int64_t rows, int v, int64_t pitch, const voi
                         const float* grad_out, const void* saved, int64_t dpitch, void* dlogits, void* stream) {
     if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, reduction)) return r;
     MI_CHECK(grad_out && saved && dlogits, "null argument");
+    MI_CHECK((uintptr_t)saved % 8 == 0 && (uintptr_t)grad_out % 4 == 0, "saved or grad_out is not aligned");
     MI_CHECK(dpitch >= v, "pitch of the gradient must cover the classes");
     MI_CHECK((uintptr_t)dlogits % (dtype ? 2 : 4) == 0, "address is not a multiple of the element size");
     const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);

@@ -16,6 +16,7 @@
 // Sums: a thread adds fp32 differences from its own first value (at most CHUNK of them), so that a mean far from zero
 // does not cancel; from there on everything is fp64 plain sums, joined in a fixed order (no atomics).
 #include <string.h>
+#include <type_traits>
 
 #include "common.h"
 #include "../../include/unet_mi355.h"
@@ -24,6 +25,7 @@ namespace {
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_PRELU = 4 };
 constexpr int TPB = 256;
+constexpr int U = 4, UB = 2;         // vectors in flight per thread and tensor: forward, backward
 constexpr int CHUNK = 256;           // pixels a thread adds in fp32 before the sums move to fp64
 constexpr int MAX_C = 8192, MAX_G = 2048;
 
@@ -134,7 +136,22 @@ __device__ __forceinline__ float act_grad(int act, float alpha, const float* u, 
     return da;
 }
 
-// Sums of `rows` threads that share a vector column, per channel, in a fixed order: NV doubles per thread in LDS as
+// Raw vectors: what a load leaves in registers, unpacked when it is used
+template <int BYTES> struct RawOf;
+template <> struct RawOf<16> { typedef uint4 T; };
+template <> struct RawOf<8> { typedef uint2 T; };
+template <> struct RawOf<4> { typedef unsigned T; };
+template <> struct RawOf<2> { typedef unsigned short T; };
+template <class TR, int VEC> using Raw = typename RawOf<VEC * TR::ESZ>::T;
+template <class TR, int VEC>
+__device__ __forceinline__ Raw<TR, VEC> ldr(const char* p) { return *reinterpret_cast<const Raw<TR, VEC>*>(p); }
+template <class TR, int VEC>
+__device__ __forceinline__ void unraw(const Raw<TR, VEC>& r, float* v) {
+    Raw<TR, VEC> t = r;
+    ldv<TR, VEC>(reinterpret_cast<const char*>(&t), v);
+}
+
+// Sums of the `rows` threads that share a vector column, in a fixed order: NV doubles per thread in LDS as
 // [NV][TPB] (consecutive lanes, consecutive addresses), halved until row 0 holds the totals.
 template <int NV>
 __device__ __forceinline__ void row_tree(double* sm, int tid, int row, int rows, int cols) {
@@ -151,12 +168,83 @@ __device__ __forceinline__ void row_tree(double* sm, int tid, int row, int rows,
 }
 
 struct Lane { int cols, rows, col, row; };
-__device__ __forceinline__ Lane lane_of(int cv, int col0) {
+__device__ __forceinline__ Lane lane_of(int cols) {
     Lane l;
-    l.cols = min(cv - col0, TPB);
-    l.rows = TPB / l.cols;
-    l.col = threadIdx.x % l.cols; l.row = threadIdx.x / l.cols;
+    l.cols = cols;
+    l.rows = TPB / cols;
+    l.col = threadIdx.x % cols; l.row = threadIdx.x / cols;
     return l;
+}
+
+// Channel sums (two doubles per channel of the thread's column) of `rows` threads -> sums of the groups g0 .. added to
+// gs[2 g].  Where a vector lies inside a group its channels are added in registers and the tree carries two values, else 2 * VEC.
+// `sm`: 2 * VEC * TPB doubles.  c0: first channel of column 0.
+template <int VEC>
+__device__ __forceinline__ void add_groups(double* sm, double* gs, const double* d1, const double* d2, const Lane& l, int c0, int cg) {
+    const int tid = threadIdx.x, c1 = c0 + l.cols * VEC, g0 = c0 / cg, g1 = (c1 - 1) / cg;
+    __syncthreads();
+    if (cg % VEC == 0) {
+        double a = 0.0, b = 0.0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { a += d1[j]; b += d2[j]; }
+        sm[tid] = a; sm[TPB + tid] = b;
+        row_tree<2>(sm, tid, l.row, l.rows, l.cols);
+        for (int g = g0 + tid; g <= g1; g += TPB) {
+            double a = 0.0, b = 0.0;
+            for (int k = max(0, (g * cg - c0) / VEC); k < min(l.cols, ((g + 1) * cg - c0) / VEC); ++k) { a += sm[k]; b += sm[TPB + k]; }
+            gs[2 * g] += a; gs[2 * g + 1] += b;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { sm[j * TPB + tid] = d1[j]; sm[(VEC + j) * TPB + tid] = d2[j]; }
+        row_tree<2 * VEC>(sm, tid, l.row, l.rows, l.cols);
+        for (int g = g0 + tid; g <= g1; g += TPB) {
+            double a = 0.0, b = 0.0;
+            for (int ch = max(c0, g * cg); ch < min(c1, (g + 1) * cg); ++ch) {
+                a += sm[((ch - c0) % VEC) * TPB + (ch - c0) / VEC];
+                b += sm[(VEC + (ch - c0) % VEC) * TPB + (ch - c0) / VEC];
+            }
+            gs[2 * g] += a; gs[2 * g + 1] += b;
+        }
+    }
+    __syncthreads();
+}
+
+// The pairs part[s][g], s < S, of an image added up by the whole workgroup: f(g, sum a, sum b) for every group.  Threads
+// side by side take neighbouring pairs; the sub-sums of a group are joined in a fixed order.
+template <class F>
+__device__ __forceinline__ void join_groups(const double* part, int S, int groups, double* sm, F f) {
+    const int tid = threadIdx.x;
+    const double2* q = reinterpret_cast<const double2*>(part);
+    for (int g0 = 0; g0 < groups; g0 += TPB) {
+        const Lane l = lane_of(min(groups - g0, TPB));
+        double a = 0.0, b = 0.0;
+        if (l.row < l.rows) {
+#pragma unroll 4
+            for (int s = l.row; s < S; s += l.rows) {
+                const double2 v = q[(int64_t)s * groups + g0 + l.col];
+                a += v.x; b += v.y;
+            }
+        }
+        __syncthreads();
+        sm[tid] = a; sm[TPB + tid] = b;
+        row_tree<2>(sm, tid, l.row, l.rows, l.cols);
+        if (tid < l.cols) f(g0 + tid, sm[tid], sm[TPB + tid]);
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ float2 moments(double a, double b, double cnt, double eps) {
+    const double m = a / cnt;
+    double var = b / cnt - m * m;
+    var = var < 0.0 ? 0.0 : var;                                    // a NaN stays
+    return make_float2((float)m, (float)(1.0 / sqrt(var + eps)));
+}
+
+// sum and sum of squares of cnt values k + d, from sums of d and d^2
+__device__ __forceinline__ void about_zero(double cnt, double k, double s1, double s2, double& d1, double& d2) {
+    d1 += cnt * k + s1;
+    d2 += cnt * k * k + 2.0 * k * s1 + s2;
 }
 
 // ---- forward, pass 1: sum and sum of squares per (image, split, group) -------------------------------------------
@@ -171,53 +259,43 @@ __global__ __launch_bounds__(TPB) void gn_stats_kernel(GnParams p) {
     for (int g = tid; g < 2 * p.groups; g += TPB) gs[g] = 0.0;
     const int cv = p.c / VEC;
     for (int col0 = 0; col0 < cv; col0 += TPB) {
-        const Lane l = lane_of(cv, col0);
-        const char* xc = x + (int64_t)(col0 + l.col) * (VEC * TR::ESZ);
+        const Lane l = lane_of(min(cv - col0, TPB));
+        const int64_t step = l.rows * p.x.pitch;
+        const char* xc = x + (int64_t)(col0 + l.col) * (VEC * TR::ESZ) + (p0 + l.row) * p.x.pitch;
         double d1[VEC], d2[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) d1[j] = d2[j] = 0.0;
-        int64_t q = l.row < l.rows ? p0 + l.row : p1;
-        while (q < p1) {
-            const int64_t left = (p1 - q + l.rows - 1) / l.rows;
+        int64_t left = l.row < l.rows && p0 + l.row < p1 ? (p1 - p0 - l.row + l.rows - 1) / l.rows : 0;
+        while (left > 0) {
             const int cnt = (int)min((int64_t)CHUNK, left);
             float k[VEC], s1[VEC], s2[VEC];
-            ldv<TR, VEC>(xc + q * p.x.pitch, k);
+            ldv<TR, VEC>(xc, k);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) s1[j] = s2[j] = 0.0f;
-#pragma unroll 4
-            for (int i = 1; i < cnt; ++i) {
+            auto take = [&](const Raw<TR, VEC>& r) {
                 float v[VEC];
-                ldv<TR, VEC>(xc + (q + (int64_t)i * l.rows) * p.x.pitch, v);
+                unraw<TR, VEC>(r, v);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     const float d = v[j] - k[j];
                     s1[j] += d; s2[j] = fmaf(d, d, s2[j]);
                 }
-            }
-            // sum (k + d) = cnt k + s1 ; sum (k + d)^2 = cnt k^2 + 2 k s1 + s2
+            };
+            int i = 0;
+            for (; i + U <= cnt; i += U) {
+                Raw<TR, VEC> r[U];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const double kk = k[j], a = s1[j];
-                d1[j] += cnt * kk + a;
-                d2[j] += cnt * kk * kk + 2.0 * kk * a + s2[j];
-            }
-            q += (int64_t)cnt * l.rows;
-        }
-        __syncthreads();
+                for (int u = 0; u < U; ++u) r[u] = ldr<TR, VEC>(xc + u * step);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) { sm[j * TPB + tid] = d1[j]; sm[(VEC + j) * TPB + tid] = d2[j]; }
-        row_tree<2 * VEC>(sm, tid, l.row, l.rows, l.cols);
-        // channels of this slab -> their groups, one thread per group, ascending
-        const int c0 = col0 * VEC, c1 = c0 + l.cols * VEC;
-        for (int g = c0 / p.cg + tid; g <= (c1 - 1) / p.cg; g += TPB) {
-            double a = 0.0, b = 0.0;
-            for (int ch = max(c0, g * p.cg); ch < min(c1, (g + 1) * p.cg); ++ch) {
-                a += sm[((ch - c0) % VEC) * TPB + (ch - c0) / VEC];
-                b += sm[(VEC + (ch - c0) % VEC) * TPB + (ch - c0) / VEC];
+                for (int u = 0; u < U; ++u) take(r[u]);
+                xc += U * step;
             }
-            gs[2 * g] += a; gs[2 * g + 1] += b;
+            for (; i < cnt; ++i) { take(ldr<TR, VEC>(xc)); xc += step; }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) about_zero(cnt, k[j], s1[j], s2[j], d1[j], d2[j]);
+            left -= cnt;
         }
-        __syncthreads();
+        add_groups<VEC>(sm, gs, d1, d2, l, col0 * VEC, p.cg);
     }
     double* out = p.part + (int64_t)blockIdx.x * p.groups * 2;
     for (int g = tid; g < 2 * p.groups; g += TPB) out[g] = gs[g];
@@ -225,53 +303,77 @@ __global__ __launch_bounds__(TPB) void gn_stats_kernel(GnParams p) {
 
 // ---- forward, pass 2 ----------------------------------------------------------------------------------------------
 template <class TR, int VEC>
-__global__ __launch_bounds__(TPB) void gn_apply_kernel(GnParams p) {
-    extern __shared__ float mr[];                                   // [groups][2] mean, rstd
-    const int n = blockIdx.x / p.B, bi = blockIdx.x % p.B, tid = threadIdx.x;
-    const double cnt = (double)p.npix * p.cg;
-    for (int g = tid; g < p.groups; g += TPB) {
-        double a = 0.0, b = 0.0;
-        const double* q = p.part + ((int64_t)n * p.S * p.groups + g) * 2;
-        for (int s = 0; s < p.S; ++s) { a += q[(int64_t)s * p.groups * 2]; b += q[(int64_t)s * p.groups * 2 + 1]; }
-        const double m = a / cnt;
-        double var = b / cnt - m * m;
-        var = var < 0.0 ? 0.0 : var;                                // a NaN stays
-        mr[2 * g] = (float)m; mr[2 * g + 1] = (float)(1.0 / sqrt(var + p.eps));
-        if (bi == 0) { float* o = p.stats + ((int64_t)n * p.groups + g) * 2; o[0] = mr[2 * g]; o[1] = mr[2 * g + 1]; }
+struct FwdConst {
+    float mean[VEC], a[VEC], b[VEC];
+    __device__ __forceinline__ void load(const GnParams& p, const float2* mr, int g0, int ch0) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float2 m = mr[(ch0 + j) / p.cg - g0];
+            mean[j] = m.x;
+            a[j] = m.y * (p.w ? p.w[ch0 + j] : 1.0f);
+            b[j] = p.b ? p.b[ch0 + j] : 0.0f;
+        }
     }
-    __syncthreads();
+    __device__ __forceinline__ void apply(int act, float alpha, float* v) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = fmaf(v[j] - mean[j], a[j], b[j]);
+        act_apply<VEC>(act, alpha, v);
+    }
+};
+
+template <class TR, int VEC>
+__global__ __launch_bounds__(TPB) void gn_apply_kernel(GnParams p) {
+    extern __shared__ float2 mr[];                                  // [groups] mean, rstd
+    __shared__ double sm[2 * TPB];
+    const int n = blockIdx.x / p.B, bi = blockIdx.x % p.B;
+    const double cnt = (double)p.npix * p.cg;
+    join_groups(p.part + (int64_t)n * p.S * p.groups * 2, p.S, p.groups, sm, [&](int g, double a, double b) {
+        mr[g] = moments(a, b, cnt, p.eps);
+        if (bi == 0) reinterpret_cast<float2*>(p.stats)[(int64_t)n * p.groups + g] = mr[g];
+    });
     const float alpha = p.alpha ? p.alpha[0] : 0.0f;
     const int64_t per = (p.npix + p.B - 1) / p.B;
     const int64_t p0 = bi * per, p1 = min(p.npix, p0 + per);
     const int cv = p.c / VEC;
     for (int col0 = 0; col0 < cv; col0 += TPB) {
-        const Lane l = lane_of(cv, col0);
+        const Lane l = lane_of(min(cv - col0, TPB));
         if (l.row >= l.rows) continue;
         const int ch0 = (col0 + l.col) * VEC;
-        float mean[VEC], a[VEC], b[VEC];
+        FwdConst<TR, VEC> k;
+        k.load(p, mr, 0, ch0);
+        const int64_t at = (int64_t)n * p.npix + p0 + l.row, off = (int64_t)ch0 * TR::ESZ;
+        const char* x = p.x.p + at * p.x.pitch + off;
+        const char* r = p.res.p ? p.res.p + at * p.res.pitch + off : nullptr;
+        char* o = p.out.p + at * p.out.pitch + off;
+        const int64_t xs = l.rows * p.x.pitch, rs = l.rows * p.res.pitch, os = l.rows * p.out.pitch;
+        int64_t left = p0 + l.row < p1 ? (p1 - p0 - l.row + l.rows - 1) / l.rows : 0;
+        auto batch = [&](auto nu) {
+            constexpr int N = decltype(nu)::value;
+            Raw<TR, VEC> xv[N], rv[N];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const int g = (ch0 + j) / p.cg;
-            mean[j] = mr[2 * g];
-            a[j] = mr[2 * g + 1] * (p.w ? p.w[ch0 + j] : 1.0f);
-            b[j] = p.b ? p.b[ch0 + j] : 0.0f;
-        }
-        const int64_t base = (int64_t)n * p.npix, off = (int64_t)ch0 * TR::ESZ;
-#pragma unroll 4
-        for (int64_t q = p0 + l.row; q < p1; q += l.rows) {
-            float v[VEC];
-            ldv<TR, VEC>(p.x.p + (base + q) * p.x.pitch + off, v);
+            for (int u = 0; u < N; ++u) xv[u] = ldr<TR, VEC>(x + u * xs);
+            if (r) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = fmaf(v[j] - mean[j], a[j], b[j]);
-            act_apply<VEC>(p.act, alpha, v);
-            if (p.res.p) {
-                float r[VEC];
-                ldv<TR, VEC>(p.res.p + (base + q) * p.res.pitch + off, r);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] += r[j];
+                for (int u = 0; u < N; ++u) rv[u] = ldr<TR, VEC>(r + u * rs);
+                r += N * rs;
             }
-            stv<TR, VEC>(p.out.p + (base + q) * p.out.pitch + off, v);
-        }
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                float v[VEC];
+                unraw<TR, VEC>(xv[u], v);
+                k.apply(p.act, alpha, v);
+                if (r) {
+                    float q[VEC];
+                    unraw<TR, VEC>(rv[u], q);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[j] += q[j];
+                }
+                stv<TR, VEC>(o + u * os, v);
+            }
+            x += N * xs; o += N * os;
+        };
+        for (; left >= U; left -= U) batch(std::integral_constant<int, U>{});
+        for (; left > 0; --left) batch(std::integral_constant<int, 1>{});
     }
 }
 
@@ -282,13 +384,43 @@ struct BwdConst {
     __device__ __forceinline__ void load(const GnParams& p, int n, int ch0) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            const float* st = p.stats + ((int64_t)n * p.groups + (ch0 + j) / p.cg) * 2;
-            mean[j] = st[0]; rstd[j] = st[1];
+            const float2 st = reinterpret_cast<const float2*>(p.stats)[(int64_t)n * p.groups + (ch0 + j) / p.cg];
+            mean[j] = st.x; rstd[j] = st.y;
             w[j] = p.w ? p.w[ch0 + j] : 1.0f;
             b[j] = p.b ? p.b[ch0 + j] : 0.0f;
         }
     }
+    // v: x -> xh; g: gradient in front of the activation; returns the slope's sum
+    __device__ __forceinline__ float grad(int act, float alpha, float* v, const float* dy, float* g) const {
+        float u[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { v[j] = (v[j] - mean[j]) * rstd[j]; u[j] = fmaf(v[j], w[j], b[j]); }
+        return act_grad<VEC>(act, alpha, u, dy, g);
+    }
+    // dx from xh and g
+    __device__ __forceinline__ void dx(const float* v, const float* g, const float* m0, const float* m1, float* o) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = rstd[j] * (fmaf(w[j], g[j], -m0[j]) - v[j] * m1[j]);
+    }
 };
+
+// Channel sums of a workgroup (LDS, [2 * VEC][TPB], row 0 holds the totals): written to pc[channel], and weighted into the
+// groups' sums gs.
+template <int VEC>
+__device__ __forceinline__ void spread_channels(const GnParams& p, const double* sm, const Lane& l, int c0, double* pc, double* gs, int g00) {
+    const int tid = threadIdx.x, c1 = c0 + l.cols * VEC;
+    for (int ch = tid; ch < c1 - c0; ch += TPB)
+        reinterpret_cast<double2*>(pc)[ch] = make_double2(sm[(ch % VEC) * TPB + ch / VEC], sm[(VEC + ch % VEC) * TPB + ch / VEC]);
+    for (int g = c0 / p.cg + tid; g <= (c1 - 1) / p.cg; g += TPB) {
+        double a = 0.0, b = 0.0;
+        for (int ch = max(c0, g * p.cg); ch < min(c1, (g + 1) * p.cg); ++ch) {
+            const double w = p.w ? p.w[ch] : 1.0f;
+            a += w * sm[((ch - c0) % VEC) * TPB + (ch - c0) / VEC];
+            b += w * sm[(VEC + (ch - c0) % VEC) * TPB + (ch - c0) / VEC];
+        }
+        gs[2 * (g - g00)] += a; gs[2 * (g - g00) + 1] += b;
+    }
+}
 
 // ---- backward, pass 1: per (image, split) the channel sums of g and g xh, the group sums of w g and w g xh ----------
 template <class TR, int VEC>
@@ -303,59 +435,50 @@ __global__ __launch_bounds__(TPB) void gn_bwd_reduce_kernel(GnParams p) {
     const int cv = p.c / VEC;
     double da = 0.0;
     for (int col0 = 0; col0 < cv; col0 += TPB) {
-        const Lane l = lane_of(cv, col0);
+        const Lane l = lane_of(min(cv - col0, TPB));
         const int ch0 = (col0 + l.col) * VEC;
-        double d1[VEC], d2[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) d1[j] = d2[j] = 0.0;
+        for (int j = 0; j < 2 * VEC; ++j) sm[j * TPB + tid] = 0.0;  // the thread's own sums
         if (l.row < l.rows) {
             BwdConst<VEC> k;
             k.load(p, n, ch0);
-            const int64_t base = (int64_t)n * p.npix, off = (int64_t)ch0 * TR::ESZ;
-            int64_t q = p0 + l.row;
-            while (q < p1) {
-                const int64_t left = (p1 - q + l.rows - 1) / l.rows;
+            const int64_t at = (int64_t)n * p.npix + p0 + l.row, off = (int64_t)ch0 * TR::ESZ;
+            const char* x = p.x.p + at * p.x.pitch + off;
+            const char* d = p.dy.p + at * p.dy.pitch + off;
+            const int64_t xs = l.rows * p.x.pitch, ds = l.rows * p.dy.pitch;
+            int64_t left = p0 + l.row < p1 ? (p1 - p0 - l.row + l.rows - 1) / l.rows : 0;
+            while (left > 0) {
                 const int cnt = (int)min((int64_t)CHUNK, left);
                 float s1[VEC], s2[VEC], sa = 0.0f;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) s1[j] = s2[j] = 0.0f;
-#pragma unroll 2
-                for (int i = 0; i < cnt; ++i) {
-                    const int64_t at = base + q + (int64_t)i * l.rows;
-                    float v[VEC], d[VEC], u[VEC], g[VEC];
-                    ldv<TR, VEC>(p.x.p + at * p.x.pitch + off, v);
-                    ldv<TR, VEC>(p.dy.p + at * p.dy.pitch + off, d);
+                auto batch = [&](auto nu) {
+                    constexpr int N = decltype(nu)::value;
+                    Raw<TR, VEC> xv[N], dv[N];
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) { v[j] = (v[j] - k.mean[j]) * k.rstd[j]; u[j] = fmaf(v[j], k.w[j], k.b[j]); }
-                    sa += act_grad<VEC>(p.act, alpha, u, d, g);
+                    for (int u = 0; u < N; ++u) { xv[u] = ldr<TR, VEC>(x + u * xs); dv[u] = ldr<TR, VEC>(d + u * ds); }
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) { s1[j] += g[j]; s2[j] = fmaf(g[j], v[j], s2[j]); }
-                }
+                    for (int u = 0; u < N; ++u) {
+                        float v[VEC], dy[VEC], g[VEC];
+                        unraw<TR, VEC>(xv[u], v);
+                        unraw<TR, VEC>(dv[u], dy);
+                        sa += k.grad(p.act, alpha, v, dy, g);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) { d1[j] += s1[j]; d2[j] += s2[j]; }
+                        for (int j = 0; j < VEC; ++j) { s1[j] += g[j]; s2[j] = fmaf(g[j], v[j], s2[j]); }
+                    }
+                    x += N * xs; d += N * ds;
+                };
+                int i = 0;
+                for (; i + UB <= cnt; i += UB) batch(std::integral_constant<int, UB>{});
+                for (; i < cnt; ++i) batch(std::integral_constant<int, 1>{});
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) { sm[j * TPB + tid] += s1[j]; sm[(VEC + j) * TPB + tid] += s2[j]; }
                 da += sa;
-                q += (int64_t)cnt * l.rows;
+                left -= cnt;
             }
         }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) { sm[j * TPB + tid] = d1[j]; sm[(VEC + j) * TPB + tid] = d2[j]; }
         row_tree<2 * VEC>(sm, tid, l.row, l.rows, l.cols);
-        const int c0 = col0 * VEC, c1 = c0 + l.cols * VEC;
-        double* pc = p.part_c + ((int64_t)blockIdx.x * p.c + c0) * 2;
-        for (int ch = tid; ch < c1 - c0; ch += TPB) {
-            pc[2 * ch] = sm[(ch % VEC) * TPB + ch / VEC];
-            pc[2 * ch + 1] = sm[(VEC + ch % VEC) * TPB + ch / VEC];
-        }
-        for (int g = c0 / p.cg + tid; g <= (c1 - 1) / p.cg; g += TPB) {
-            double a = 0.0, b = 0.0;
-            for (int ch = max(c0, g * p.cg); ch < min(c1, (g + 1) * p.cg); ++ch) {
-                const double w = p.w ? p.w[ch] : 1.0f;
-                a += w * sm[((ch - c0) % VEC) * TPB + (ch - c0) / VEC];
-                b += w * sm[(VEC + (ch - c0) % VEC) * TPB + (ch - c0) / VEC];
-            }
-            gs[2 * g] += a; gs[2 * g + 1] += b;
-        }
+        spread_channels<VEC>(p, sm, l, col0 * VEC, p.part_c + ((int64_t)blockIdx.x * p.c + col0 * VEC) * 2, gs, 0);
         __syncthreads();
     }
     double* out = p.part + (int64_t)blockIdx.x * p.groups * 2;
@@ -367,85 +490,262 @@ __global__ __launch_bounds__(TPB) void gn_bwd_reduce_kernel(GnParams p) {
     }
 }
 
-// sums of n values at a stride by a whole workgroup, fixed order; thread 0 has the result
-__device__ __forceinline__ double block_sum(const double* q, int64_t n, int64_t stride, double* sm) {
-    double a = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += TPB) a += q[i * stride];
-    __syncthreads();
-    sm[threadIdx.x] = a;
-    row_tree<1>(sm, threadIdx.x, threadIdx.x, TPB, 1);
-    return sm[0];
+// Parameter gradients: workgroup k joins the channels [k * JC, (k + 1) * JC) of the n parts; the one behind the last, dalpha.
+constexpr int JC = 16;
+__device__ __forceinline__ void join_params(const GnParams& p, int k, int n, double* sm) {
+    const int tid = threadIdx.x, last = (p.c + JC - 1) / JC;
+    if (k < last) {
+        const int ch = k * JC + tid % JC, row = tid / JC;
+        double a = 0.0, b = 0.0;
+        if (ch < p.c) {
+#pragma unroll 4
+            for (int i = row; i < n; i += TPB / JC) {
+                const double2 v = reinterpret_cast<const double2*>(p.part_c)[(int64_t)i * p.c + ch];
+                a += v.x; b += v.y;
+            }
+        }
+        sm[tid] = a; sm[TPB + tid] = b;
+        row_tree<2>(sm, tid, row, TPB / JC, JC);
+        if (row == 0 && ch < p.c) {
+            if (p.db) p.db[ch] = (float)sm[tid];
+            if (p.dw) p.dw[ch] = (float)sm[TPB + tid];
+        }
+    } else {
+        double a = 0.0;
+        for (int i = tid; i < n; i += TPB) a += p.part_a[i];
+        sm[tid] = a;
+        row_tree<1>(sm, tid, tid, TPB, 1);
+        if (tid == 0) p.dalpha[0] = (float)sm[0];
+    }
 }
 
-// ---- backward, pass 2: dx; the workgroups behind the nb * B of them join the channel sums of all images --------------
+// ---- backward, pass 2: dx; the workgroups behind the nb * B of them join the parameter gradients -------------------
 template <class TR, int VEC>
 __global__ __launch_bounds__(TPB) void gn_bwd_apply_kernel(GnParams p) {
-    extern __shared__ float gm[];                                   // [groups][2] means of w g and w g xh
-    __shared__ double sm[TPB];
-    const int tid = threadIdx.x;
+    extern __shared__ float2 gm[];                                  // [groups] means of w g and w g xh
+    __shared__ double sm[2 * TPB];
     if ((int)blockIdx.x >= p.nb * p.B) {
-        const int ch = (int)blockIdx.x - p.nb * p.B;
-        const int64_t n = (int64_t)p.nb * p.S;
-        if (ch < p.c) {
-            const double a = block_sum(p.part_c + 2 * ch, n, 2 * p.c, sm);
-            if (tid == 0 && p.db) p.db[ch] = (float)a;
-            const double b = block_sum(p.part_c + 2 * ch + 1, n, 2 * p.c, sm);
-            if (tid == 0 && p.dw) p.dw[ch] = (float)b;
-        } else {
-            const double a = block_sum(p.part_a, n, 1, sm);
-            if (tid == 0) p.dalpha[0] = (float)a;
-        }
+        join_params(p, (int)blockIdx.x - p.nb * p.B, p.nb * p.S, sm);
         return;
     }
     const int n = blockIdx.x / p.B, bi = blockIdx.x % p.B;
     const double cnt = (double)p.npix * p.cg;
-    for (int g = tid; g < p.groups; g += TPB) {
-        double a = 0.0, b = 0.0;
-        const double* q = p.part + ((int64_t)n * p.S * p.groups + g) * 2;
-        for (int s = 0; s < p.S; ++s) { a += q[(int64_t)s * p.groups * 2]; b += q[(int64_t)s * p.groups * 2 + 1]; }
-        gm[2 * g] = (float)(a / cnt); gm[2 * g + 1] = (float)(b / cnt);
-    }
-    __syncthreads();
+    join_groups(p.part + (int64_t)n * p.S * p.groups * 2, p.S, p.groups, sm,
+                [&](int g, double a, double b) { gm[g] = make_float2((float)(a / cnt), (float)(b / cnt)); });
     const float alpha = p.alpha ? p.alpha[0] : 0.0f;
     const int64_t per = (p.npix + p.B - 1) / p.B;
     const int64_t p0 = bi * per, p1 = min(p.npix, p0 + per);
     const int cv = p.c / VEC;
     for (int col0 = 0; col0 < cv; col0 += TPB) {
-        const Lane l = lane_of(cv, col0);
+        const Lane l = lane_of(min(cv - col0, TPB));
         if (l.row >= l.rows) continue;
         const int ch0 = (col0 + l.col) * VEC;
         BwdConst<VEC> k;
         k.load(p, n, ch0);
         float m0[VEC], m1[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) { const int g = (ch0 + j) / p.cg; m0[j] = gm[2 * g]; m1[j] = gm[2 * g + 1]; }
-        const int64_t base = (int64_t)n * p.npix, off = (int64_t)ch0 * TR::ESZ;
-#pragma unroll 2
-        for (int64_t q = p0 + l.row; q < p1; q += l.rows) {
-            float v[VEC], d[VEC], u[VEC], g[VEC];
-            ldv<TR, VEC>(p.x.p + (base + q) * p.x.pitch + off, v);
-            ldv<TR, VEC>(p.dy.p + (base + q) * p.dy.pitch + off, d);
+        for (int j = 0; j < VEC; ++j) { const float2 m = gm[(ch0 + j) / p.cg]; m0[j] = m.x; m1[j] = m.y; }
+        const int64_t at = (int64_t)n * p.npix + p0 + l.row, off = (int64_t)ch0 * TR::ESZ;
+        const char* x = p.x.p + at * p.x.pitch + off;
+        const char* d = p.dy.p + at * p.dy.pitch + off;
+        char* o = p.out.p + at * p.out.pitch + off;
+        const int64_t xs = l.rows * p.x.pitch, ds = l.rows * p.dy.pitch, os = l.rows * p.out.pitch;
+        int64_t left = p0 + l.row < p1 ? (p1 - p0 - l.row + l.rows - 1) / l.rows : 0;
+        auto batch = [&](auto nu) {
+            constexpr int N = decltype(nu)::value;
+            Raw<TR, VEC> xv[N], dv[N];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) { v[j] = (v[j] - k.mean[j]) * k.rstd[j]; u[j] = fmaf(v[j], k.w[j], k.b[j]); }
-            act_grad<VEC>(p.act, alpha, u, d, g);
+            for (int u = 0; u < N; ++u) { xv[u] = ldr<TR, VEC>(x + u * xs); dv[u] = ldr<TR, VEC>(d + u * ds); }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) u[j] = k.rstd[j] * (fmaf(k.w[j], g[j], -m0[j]) - v[j] * m1[j]);
-            stv<TR, VEC>(p.out.p + (base + q) * p.out.pitch + off, u);
-        }
+            for (int u = 0; u < N; ++u) {
+                float v[VEC], dy[VEC], g[VEC];
+                unraw<TR, VEC>(xv[u], v);
+                unraw<TR, VEC>(dv[u], dy);
+                k.grad(p.act, alpha, v, dy, g);
+                k.dx(v, g, m0, m1, v);
+                stv<TR, VEC>(o + u * os, v);
+            }
+            x += N * xs; d += N * ds; o += N * os;
+        };
+        for (; left >= UB; left -= UB) batch(std::integral_constant<int, UB>{});
+        for (; left > 0; --left) batch(std::integral_constant<int, 1>{});
     }
 }
 
+// ---- small images: one launch, the data stays in registers between the sums and their use ----------------------------
+// Workgroup (n, slab) owns all pixels of p.B whole groups of image n (the last slab: what is left); a thread holds up to NV
+// vectors.  dynamic LDS: [p.B][2] doubles.
+struct Slab { int n, slab, g0, ng, c0; };
+__device__ __forceinline__ Slab slab_of(const GnParams& p) {
+    Slab b;
+    b.n = blockIdx.x / p.S; b.slab = blockIdx.x % p.S;
+    b.g0 = b.slab * p.B; b.ng = min(p.B, p.groups - b.g0); b.c0 = b.g0 * p.cg;
+    return b;
+}
+
+template <class TR, int VEC, int NV>
+__global__ __launch_bounds__(TPB) void gn_small_fwd_kernel(GnParams p) {
+    __shared__ double sm[2 * VEC * TPB];
+    extern __shared__ double gs[];
+    const Slab b = slab_of(p);
+    const Lane l = lane_of(b.ng * p.cg / VEC);
+    const int tid = threadIdx.x, npix = (int)p.npix, ch0 = b.c0 + l.col * VEC;
+    const int cnt = l.row < l.rows && l.row < npix ? (npix - l.row + l.rows - 1) / l.rows : 0;
+    const int64_t at = (int64_t)b.n * p.npix + l.row, off = (int64_t)ch0 * TR::ESZ;
+    const char* x = p.x.p + at * p.x.pitch + off;
+    Raw<TR, VEC> xv[NV];
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+        if (u < cnt) xv[u] = ldr<TR, VEC>(x + u * (l.rows * p.x.pitch));
+    for (int g = tid; g < 2 * b.ng; g += TPB) gs[g] = 0.0;
+    float k[VEC], s1[VEC], s2[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) k[j] = s1[j] = s2[j] = 0.0f;
+    if (cnt) unraw<TR, VEC>(xv[0], k);
+#pragma unroll
+    for (int u = 1; u < NV; ++u)
+        if (u < cnt) {
+            float v[VEC];
+            unraw<TR, VEC>(xv[u], v);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float d = v[j] - k[j];
+                s1[j] += d; s2[j] = fmaf(d, d, s2[j]);
+            }
+        }
+    double d1[VEC], d2[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { d1[j] = d2[j] = 0.0; about_zero(cnt, k[j], s1[j], s2[j], d1[j], d2[j]); }
+    add_groups<VEC>(sm, gs - 2 * b.g0, d1, d2, l, b.c0, p.cg);
+    float2* mr = reinterpret_cast<float2*>(sm);
+    for (int g = tid; g < b.ng; g += TPB) {
+        mr[g] = moments(gs[2 * g], gs[2 * g + 1], (double)p.npix * p.cg, p.eps);
+        reinterpret_cast<float2*>(p.stats)[(int64_t)b.n * p.groups + b.g0 + g] = mr[g];
+    }
+    __syncthreads();
+    if (!cnt) return;
+    const float alpha = p.alpha ? p.alpha[0] : 0.0f;
+    FwdConst<TR, VEC> c;
+    c.load(p, mr, b.g0, ch0);
+    const char* r = p.res.p ? p.res.p + at * p.res.pitch + off : nullptr;
+    char* o = p.out.p + at * p.out.pitch + off;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+        if (u < cnt) {
+            float v[VEC];
+            unraw<TR, VEC>(xv[u], v);
+            c.apply(p.act, alpha, v);
+            if (r) {
+                float q[VEC];
+                ldv<TR, VEC>(r + u * (l.rows * p.res.pitch), q);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] += q[j];
+            }
+            stv<TR, VEC>(o + u * (l.rows * p.out.pitch), v);
+        }
+}
+
+template <class TR, int VEC, int NV>
+__global__ __launch_bounds__(TPB) void gn_small_bwd_kernel(GnParams p) {
+    __shared__ double sm[2 * VEC * TPB];
+    extern __shared__ double gs[];
+    const Slab b = slab_of(p);
+    const Lane l = lane_of(b.ng * p.cg / VEC);
+    const int tid = threadIdx.x, npix = (int)p.npix, ch0 = b.c0 + l.col * VEC;
+    const int cnt = l.row < l.rows && l.row < npix ? (npix - l.row + l.rows - 1) / l.rows : 0;
+    const int64_t at = (int64_t)b.n * p.npix + l.row, off = (int64_t)ch0 * TR::ESZ;
+    const char* x = p.x.p + at * p.x.pitch + off;
+    const char* d = p.dy.p + at * p.dy.pitch + off;
+    Raw<TR, VEC> xv[NV], dv[NV];
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+        if (u < cnt) {
+            xv[u] = ldr<TR, VEC>(x + u * (l.rows * p.x.pitch));
+            dv[u] = ldr<TR, VEC>(d + u * (l.rows * p.dy.pitch));
+        }
+    const float alpha = p.alpha ? p.alpha[0] : 0.0f;
+    BwdConst<VEC> k;
+    if (cnt) k.load(p, b.n, ch0);
+    for (int g = tid; g < 2 * b.ng; g += TPB) gs[g] = 0.0;
+    float s1[VEC], s2[VEC], sa = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s1[j] = s2[j] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+        if (u < cnt) {
+            float v[VEC], dy[VEC], g[VEC];
+            unraw<TR, VEC>(xv[u], v);
+            unraw<TR, VEC>(dv[u], dy);
+            sa += k.grad(p.act, alpha, v, dy, g);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) { s1[j] += g[j]; s2[j] = fmaf(g[j], v[j], s2[j]); }
+        }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { sm[j * TPB + tid] = s1[j]; sm[(VEC + j) * TPB + tid] = s2[j]; }
+    row_tree<2 * VEC>(sm, tid, l.row, l.rows, l.cols);
+    spread_channels<VEC>(p, sm, l, b.c0, p.part_c + ((int64_t)b.n * p.c + b.c0) * 2, gs, b.g0);
+    __syncthreads();
+    if (p.part_a) {
+        sm[tid] = sa;
+        row_tree<1>(sm, tid, tid, TPB, 1);
+        if (tid == 0) p.part_a[blockIdx.x] = sm[0];
+    }
+    if (!cnt) return;
+    const double n = (double)p.npix * p.cg;
+    float m0[VEC], m1[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const int g = (ch0 + j) / p.cg - b.g0;
+        m0[j] = (float)(gs[2 * g] / n); m1[j] = (float)(gs[2 * g + 1] / n);
+    }
+    char* o = p.out.p + at * p.out.pitch + off;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+        if (u < cnt) {
+            float v[VEC], dy[VEC], g[VEC];
+            unraw<TR, VEC>(xv[u], v);
+            unraw<TR, VEC>(dv[u], dy);
+            k.grad(p.act, alpha, v, dy, g);
+            k.dx(v, g, m0, m1, v);
+            stv<TR, VEC>(o + u * (l.rows * p.out.pitch), v);
+        }
+}
+
+// parameter gradients behind gn_small_bwd_kernel: p.nb parts per channel, p.nb * p.S of dalpha
+__global__ __launch_bounds__(TPB) void gn_join_kernel(GnParams p) {
+    __shared__ double sm[2 * TPB];
+    const bool slope = (int)blockIdx.x >= (p.c + JC - 1) / JC;
+    join_params(p, blockIdx.x, slope ? p.nb * p.S : p.nb, sm);
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------
-// Splits of an image in the reduction passes: enough workgroups to fill the chip (2048 = 8 per CU), at least 32 KB of
-// the tensor per workgroup, and at most 4096 partial pairs for a workgroup of the second pass to join.
+// Splits of an image in both passes: enough workgroups to fill the chip (2048 = 8 per CU), at least 32 KB of the tensor per
+// workgroup, and at most 8192 pairs (128 KB, in L2) for a workgroup of the second pass to join.
 int splits(int esz, int nb, int64_t npix, int c, int groups) {
     const int64_t bytes = npix * c * esz;
     int64_t s = (2048 + nb - 1) / nb;
     s = s < bytes / 32768 ? s : bytes / 32768;
-    const int64_t cap = 4096 / groups > 8 ? 4096 / groups : 8;
-    s = s < cap ? s : cap;
+    s = s < 8192 / groups ? s : 8192 / groups;
     s = s < npix ? s : npix;
     return s < 1 ? 1 : (int)s;
+}
+
+// Small images: slabs of whole groups at least 64 bytes wide, held by 256 threads with at most `most` vectors each.
+// 16 x 16 x 256 bf16, one image: TODO
+struct Small { bool ok; int groups, slabs, nv; };
+Small small_of(int esz, int vec, int64_t npix, int c, int groups, int most) {
+    const int cg = c / groups;
+    Small q = {false, 1, 1, 1};
+    if (npix > 65536) return q;
+    while (q.groups < groups && (q.groups * cg * esz < 64 || q.groups * cg % vec)) ++q.groups;
+    const int cols = q.groups * cg / vec;                            // groups == all: c is a multiple of vec
+    if (cols > TPB) return q;
+    const int per = (int)((npix + TPB / cols - 1) / (TPB / cols));
+    if (per > most) return q;
+    q.slabs = (groups + q.groups - 1) / q.groups;
+    while (q.nv < per) q.nv *= 2;
+    q.ok = true;
+    return q;
 }
 
 int check_shape(const char* who, int dtype, int nb, int64_t npix, int c, int groups) {
@@ -470,6 +770,28 @@ int view_of(const char* who, const char* name, const mi_tensor* t, int c, int es
     return 0;
 }
 
+#define GN_SMALL_VEC(KERN, T, V, grid, lds)                                                                 \
+    do {                                                                                                    \
+        if (q.nv == 1) KERN<T, V, 1><<<grid, TPB, lds, st>>>(p);                                            \
+        else if (q.nv == 2) KERN<T, V, 2><<<grid, TPB, lds, st>>>(p);                                       \
+        else if (q.nv == 4) KERN<T, V, 4><<<grid, TPB, lds, st>>>(p);                                       \
+        else KERN<T, V, 8><<<grid, TPB, lds, st>>>(p);                                                      \
+    } while (0)
+#define GN_SMALL(KERN, grid, lds)                                                                           \
+    do {                                                                                                    \
+        if (dtype == 1) {                                                                                   \
+            if (vec == 8) GN_SMALL_VEC(KERN, BF16, 8, grid, lds);                                           \
+            else if (vec == 4) GN_SMALL_VEC(KERN, BF16, 4, grid, lds);                                      \
+            else if (vec == 2) GN_SMALL_VEC(KERN, BF16, 2, grid, lds);                                      \
+            else GN_SMALL_VEC(KERN, BF16, 1, grid, lds);                                                    \
+        } else {                                                                                            \
+            if (vec == 4) GN_SMALL_VEC(KERN, F32, 4, grid, lds);                                            \
+            else if (vec == 2) GN_SMALL_VEC(KERN, F32, 2, grid, lds);                                       \
+            else GN_SMALL_VEC(KERN, F32, 1, grid, lds);                                                     \
+        }                                                                                                   \
+        MI_HIP(hipGetLastError());                                                                          \
+    } while (0)
+
 #define GN_LAUNCH(KERN, grid, lds)                                                                          \
     do {                                                                                                    \
         if (dtype == 1) {                                                                                   \
@@ -492,6 +814,7 @@ extern "C" {
 size_t mi_groupnorm_act_workspace_bytes(int dtype, int nb, int64_t npix, int c, int groups, int backward) {
     if (check_shape(__func__, dtype, nb, npix, c, groups)) return 0;
     const size_t s = (size_t)nb * splits(dtype ? 2 : 4, nb, npix, c, groups);
+    // a small image's backward pass: [nb][c][2] and at most [nb][groups]
     return (s * groups * 2 + (backward ? s * c * 2 + s : 0)) * sizeof(double);
 }
 
@@ -502,6 +825,7 @@ int mi_groupnorm_act_fwd(int dtype, int nb, int64_t npix, int c, int groups, con
     MI_CHECK(act >= ACT_NONE && act <= ACT_PRELU, "unknown activation");
     MI_CHECK((act == ACT_PRELU) == (alpha != nullptr), "alpha belongs to prelu");
     MI_CHECK(stats && workspace, "null argument");
+    MI_CHECK((uintptr_t)workspace % 16 == 0 && (uintptr_t)stats % 8 == 0, "workspace or stats is not aligned");
     MI_CHECK(eps >= 0.0f, "eps must not be negative");
     GnParams p; memset(&p, 0, sizeof(p));
     const int esz = dtype ? 2 : 4;
@@ -512,8 +836,14 @@ int mi_groupnorm_act_fwd(int dtype, int nb, int64_t npix, int c, int groups, con
         if (int r = view_of(__func__, "res", res, c, esz, p.res, vec)) return r;
     p.w = weight; p.b = bias; p.alpha = alpha; p.stats = stats; p.part = (double*)workspace;
     p.nb = nb; p.npix = npix; p.c = c; p.groups = groups; p.cg = c / groups; p.act = act; p.eps = eps;
-    p.S = p.B = splits(esz, nb, npix, c, groups);
     hipStream_t st = (hipStream_t)stream;
+    const Small q = small_of(esz, vec, npix, c, groups, 8);
+    if (q.ok) {
+        p.S = q.slabs; p.B = q.groups;
+        GN_SMALL(gn_small_fwd_kernel, nb * p.S, q.groups * 2 * sizeof(double));
+        return 0;
+    }
+    p.S = p.B = splits(esz, nb, npix, c, groups);
     GN_LAUNCH(gn_stats_kernel, nb * p.S, groups * 2 * sizeof(double));
     GN_LAUNCH(gn_apply_kernel, nb * p.B, groups * 2 * sizeof(float));
     return 0;
@@ -527,6 +857,7 @@ int mi_groupnorm_act_bwd(int dtype, int nb, int64_t npix, int c, int groups, con
     MI_CHECK((act == ACT_PRELU) == (alpha != nullptr), "alpha belongs to prelu");
     MI_CHECK(!dalpha || alpha, "a gradient of alpha needs alpha");
     MI_CHECK(stats && workspace, "null argument");
+    MI_CHECK((uintptr_t)workspace % 16 == 0 && (uintptr_t)stats % 8 == 0, "workspace or stats is not aligned");
     GnParams p; memset(&p, 0, sizeof(p));
     const int esz = dtype ? 2 : 4;
     int vec = 16 / esz;
@@ -536,14 +867,25 @@ int mi_groupnorm_act_bwd(int dtype, int nb, int64_t npix, int c, int groups, con
     p.w = weight; p.b = bias; p.alpha = alpha; p.stats = const_cast<float*>(stats);
     p.dw = dweight; p.db = dbias; p.dalpha = dalpha;
     p.nb = nb; p.npix = npix; p.c = c; p.groups = groups; p.cg = c / groups; p.act = act;
+    hipStream_t st = (hipStream_t)stream;
+    const int joins = dweight || dbias || dalpha ? (c + JC - 1) / JC + (dalpha ? 1 : 0) : 0;
+    const Small q = small_of(esz, vec, npix, c, groups, 8);
+    if (q.ok) {
+        p.S = q.slabs; p.B = q.groups;
+        p.part_c = (double*)workspace;
+        p.part_a = dalpha ? p.part_c + (size_t)nb * c * 2 : nullptr;
+        GN_SMALL(gn_small_bwd_kernel, nb * p.S, q.groups * 2 * sizeof(double));
+        if (joins) gn_join_kernel<<<joins, TPB, 0, st>>>(p);
+        MI_HIP(hipGetLastError());
+        return 0;
+    }
     p.S = p.B = splits(esz, nb, npix, c, groups);
     const size_t s = (size_t)nb * p.S;
     p.part = (double*)workspace;
     p.part_c = p.part + s * groups * 2;
     p.part_a = dalpha ? p.part_c + s * c * 2 : nullptr;
-    hipStream_t st = (hipStream_t)stream;
     GN_LAUNCH(gn_bwd_reduce_kernel, nb * p.S, groups * 2 * sizeof(double));
-    GN_LAUNCH(gn_bwd_apply_kernel, nb * p.B + ((dweight || dbias || dalpha) ? c + (dalpha ? 1 : 0) : 0), groups * 2 * sizeof(float));
+    GN_LAUNCH(gn_bwd_apply_kernel, nb * p.B + joins, groups * 2 * sizeof(float));
     return 0;
 }
 

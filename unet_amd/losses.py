@@ -127,7 +127,7 @@ class _DistillFunction(torch.autograd.Function):
                 index.data_ptr(), temperature, red)
         with _lib.on_device(dev):
             saved = torch.empty(lib.mi_distill_loss_saved_bytes(args[0], rows, v, k), dtype=torch.uint8, device=dev)
-            _lib.check(lib.mi_distill_loss_fwd(*args, loss.data_ptr(), saved.data_ptr(), _lib.current_stream(dev)), "mi_distill_loss_fwd")
+            _lib.check(lib.mi_distill_loss_fwd(*args, loss.data_ptr(), saved.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_fwd")
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(logits, teacher, index, saved)
             ctx.cfg = (temperature, red)
@@ -146,7 +146,7 @@ class _DistillFunction(torch.autograd.Function):
         with _lib.on_device(dev):
             _lib.check(lib.mi_distill_loss_bwd(_DT[z.dtype], index.numel() // k, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(),
                                                _INDEX[index.dtype], index.data_ptr(), temperature, red, g.data_ptr(), saved.data_ptr(),
-                                               v, dz.data_ptr(), _lib.current_stream(dev)), "mi_distill_loss_bwd")
+                                               v, dz.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_bwd")
         return dz, None, None, None, None
 
 

@@ -7,6 +7,8 @@ Tensors are ``[N, (D,) H, W, C]`` contiguous, dtype ``torch.bfloat16`` or ``torc
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import math
 from typing import Optional
 
 import torch
@@ -223,19 +225,22 @@ def _pixels(t, name, like=None):
 
 
 def _view(t, pitch):
-    m = _lib.MiTensor()
-    m.ptr, m.pitch = t.data_ptr(), pitch
-    return m
+    return C.byref(_lib.MiTensor(t.data_ptr(), pitch))
 
 
 def _channel_param(t, n, x, name):
     if t is None:
         return None
-    if t.numel() != n or t.dim() != 1:
+    if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
     if t.device != x.device:
         raise ValueError(f"{name} is on {t.device}, expected {x.device}")
-    return t.detach().contiguous().float()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.detach().contiguous().float()
+
+
+@functools.lru_cache(maxsize=256)
+def _groupnorm_workspace(dt, nb, npix, c, groups, backward):
+    return _lib.load().mi_groupnorm_act_workspace_bytes(dt, nb, npix, c, groups, backward)
 
 
 def _groupnorm_args(x, groups, weight, bias, act, alpha):
@@ -249,13 +254,10 @@ def _groupnorm_args(x, groups, weight, bias, act, alpha):
         raise ValueError(f"act must be one of {sorted(_ACT)}, got {act!r}")
     if (alpha is None) == (act == "prelu"):
         raise ValueError("alpha (one slope) belongs to act='prelu' and to no other")
-    nb, c = x.shape[0], x.shape[-1]
-    groups = int(groups)
+    nb, c, groups = x.shape[0], x.shape[-1], int(groups)
     if c < 1 or groups < 1 or c % groups:
         raise ValueError(f"{groups} groups do not divide {c} channels")
-    npix = 1
-    for v in x.shape[1:-1]:
-        npix *= v
+    npix = math.prod(x.shape[1:-1])
     if npix == 0:
         raise ValueError("an image without pixels has no mean")
     return (nb, npix, c, groups, _channel_param(weight, c, x, "weight"), _channel_param(bias, c, x, "bias"),
@@ -276,11 +278,9 @@ def groupnorm_act_fwd(x, groups, weight=None, bias=None, act="silu", alpha=None,
         return out, stats
     lib, dt = _lib.load(), _DT[x.dtype]
     with _lib.on_device(x.device):
-        ws = torch.empty(lib.mi_groupnorm_act_workspace_bytes(dt, nb, npix, c, groups, 0), dtype=torch.uint8, device=x.device)
-        tx, to, tr = _view(x, xp), _view(out, c), _view(res, rp) if res is not None else None
-        _lib.check(lib.mi_groupnorm_act_fwd(dt, nb, npix, c, groups, C.byref(tx), _lib.ptr(weight), _lib.ptr(bias), _ACT[act],
-                                            _lib.ptr(alpha), C.byref(tr) if tr is not None else None, C.byref(to), float(eps),
-                                            stats.data_ptr(), ws.data_ptr(), _lib.current_stream(x.device)), "mi_groupnorm_act_fwd")
+        ws = torch.empty(_groupnorm_workspace(dt, nb, npix, c, groups, 0), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.mi_groupnorm_act_fwd(dt, nb, npix, c, groups, _view(x, xp), _lib.ptr(weight), _lib.ptr(bias), _ACT[act],
+                                            _lib.ptr(alpha), _view(res, rp) if res is not None else None, _view(out, c), eps, stats.data_ptr(), ws.data_ptr(), _lib.stream_of(x.device)), "mi_groupnorm_act_fwd")
     return out, stats
 
 
@@ -302,11 +302,10 @@ def groupnorm_act_bwd(dy, x, stats, groups, weight=None, bias=None, act="silu", 
         return dx, dw, db, da
     lib, dt = _lib.load(), _DT[x.dtype]
     with _lib.on_device(x.device):
-        ws = torch.empty(lib.mi_groupnorm_act_workspace_bytes(dt, nb, npix, c, groups, 1), dtype=torch.uint8, device=x.device)
-        tdy, tx, tdx = _view(dy, dp), _view(x, xp), _view(dx, c)
-        _lib.check(lib.mi_groupnorm_act_bwd(dt, nb, npix, c, groups, C.byref(tdy), C.byref(tx), stats.data_ptr(), _lib.ptr(weight),
-                                            _lib.ptr(bias), _ACT[act], _lib.ptr(alpha), C.byref(tdx), _lib.ptr(dw), _lib.ptr(db),
-                                            _lib.ptr(da), ws.data_ptr(), _lib.current_stream(x.device)), "mi_groupnorm_act_bwd")
+        ws = torch.empty(_groupnorm_workspace(dt, nb, npix, c, groups, 1), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.mi_groupnorm_act_bwd(dt, nb, npix, c, groups, _view(dy, dp), _view(x, xp), stats.data_ptr(), _lib.ptr(weight),
+                                            _lib.ptr(bias), _ACT[act], _lib.ptr(alpha), _view(dx, c), _lib.ptr(dw), _lib.ptr(db),
+                                            _lib.ptr(da), ws.data_ptr(), _lib.stream_of(x.device)), "mi_groupnorm_act_bwd")
     return dx, dw, db, da
 
 
@@ -331,5 +330,5 @@ def top_logits(logits, k):
     if rows:
         with _lib.on_device(x.device):
             _lib.check(_lib.load().mi_top_logits(_DT[x.dtype], rows, v, pitch, x.data_ptr(), k, values.data_ptr(), index.data_ptr(),
-                                                 _lib.current_stream(x.device)), "mi_top_logits")
+                                                 _lib.stream_of(x.device)), "mi_top_logits")
     return values, index
