@@ -25,7 +25,16 @@ namespace {
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_PRELU = 4 };
 constexpr int TPB = 256;
-constexpr int U = 4, UB = 2;         // vectors in flight per thread and tensor: forward, backward
+#ifndef GN_U
+#define GN_U 4
+#endif
+#ifndef GN_UB
+#define GN_UB 2
+#endif
+#ifndef GN_WG
+#define GN_WG 2048
+#endif
+constexpr int U = GN_U, UB = GN_UB; // vectors in flight per thread and tensor: forward, backward
 constexpr int CHUNK = 256;           // pixels a thread adds in fp32 before the sums move to fp64
 constexpr int MAX_C = 8192, MAX_G = 2048;
 
@@ -86,7 +95,26 @@ __device__ __forceinline__ void stv(char* p, const float* v) {
 __device__ __forceinline__ float sigmoid_f(float u) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
 }
-constexpr float SQRT_HALF = 0.70710678118654752f, INV_SQRT_2PI = 0.39894228040143268f;
+// Phi(u), the normal distribution function, and e = exp(-u^2 / 2).  With t = 1 / (1 + 0.2828 |u|) the scaled tail
+// Phi(-|u|) / (e t) is smooth in t; the polynomial below is a weighted least-squares fit of it in relative error, which is 1.3e-7
+// in exact arithmetic and 4.8e-7 in fp32 from 0 to 12, tail included (the library's erff takes twice the instructions:
+// GELU forward 32 x 256^2 x 32 bf16 108 -> 97 us, backward 32 x 256^2 x 16 103 -> 79).
+__device__ __forceinline__ float normal_cdf(float u, float& e) {
+    e = __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.28284272f, fabsf(u), 1.0f));
+    float s = 0.025144234f;
+    s = fmaf(s, t, -0.091504857f);
+    s = fmaf(s, t, 0.084634006f);
+    s = fmaf(s, t, -0.0028852099f);
+    s = fmaf(s, t, 0.070756972f);
+    s = fmaf(s, t, 0.084259167f);
+    s = fmaf(s, t, 0.10392314f);
+    s = fmaf(s, t, 0.11283468f);
+    s = fmaf(s, t, 0.11283793f);
+    const float tail = s * t * e;
+    return u > 0.0f ? 1.0f - tail : tail;
+}
+constexpr float INV_SQRT_2PI = 0.39894228040143268f;
 
 template <int VEC>
 __device__ __forceinline__ void act_apply(int act, float alpha, float* u) {
@@ -101,7 +129,10 @@ __device__ __forceinline__ void act_apply(int act, float alpha, float* u) {
         for (int j = 0; j < VEC; ++j) u[j] = u[j] > 0.0f ? u[j] : alpha * u[j];
     } else if (act == ACT_GELU) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) u[j] = 0.5f * u[j] * (1.0f + erff(u[j] * SQRT_HALF));
+        for (int j = 0; j < VEC; ++j) {
+            float e;
+            u[j] *= normal_cdf(u[j], e);
+        }
     }
 }
 // g[j] = dy[j] * act'(u[j]); returns sum of dy * u over u <= 0 (PReLU's slope gradient)
@@ -126,8 +157,9 @@ __device__ __forceinline__ float act_grad(int act, float alpha, const float* u, 
     } else if (act == ACT_GELU) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            const float phi = INV_SQRT_2PI * __builtin_amdgcn_exp2f(u[j] * u[j] * -0.72134752044448170f);
-            g[j] = dy[j] * (0.5f * (1.0f + erff(u[j] * SQRT_HALF)) + u[j] * phi);
+            float e;
+            const float c = normal_cdf(u[j], e);
+            g[j] = dy[j] * fmaf(u[j] * INV_SQRT_2PI, e, c);
         }
     } else {
 #pragma unroll
@@ -323,9 +355,14 @@ struct FwdConst {
 
 template <class TR, int VEC>
 __global__ __launch_bounds__(TPB) void gn_apply_kernel(GnParams p) {
+#ifdef GN_REV
+    const int blk = gridDim.x % 8 == 0 ? (gridDim.x / 8 - 1 - blockIdx.x / 8) * 8 + blockIdx.x % 8 : gridDim.x - 1 - blockIdx.x;
+#else
+    const int blk = blockIdx.x;
+#endif
     extern __shared__ float2 mr[];                                  // [groups] mean, rstd
     __shared__ double sm[2 * TPB];
-    const int n = blockIdx.x / p.B, bi = blockIdx.x % p.B;
+    const int n = blk / p.B, bi = blk % p.B;
     const double cnt = (double)p.npix * p.cg;
     join_groups(p.part + (int64_t)n * p.S * p.groups * 2, p.S, p.groups, sm, [&](int g, double a, double b) {
         mr[g] = moments(a, b, cnt, p.eps);
@@ -528,7 +565,13 @@ __global__ __launch_bounds__(TPB) void gn_bwd_apply_kernel(GnParams p) {
         join_params(p, (int)blockIdx.x - p.nb * p.B, p.nb * p.S, sm);
         return;
     }
-    const int n = blockIdx.x / p.B, bi = blockIdx.x % p.B;
+    const int nblk = p.nb * p.B;
+#ifdef GN_REV
+    const int blk = nblk % 8 == 0 ? (nblk / 8 - 1 - (int)blockIdx.x / 8) * 8 + (int)blockIdx.x % 8 : nblk - 1 - (int)blockIdx.x;
+#else
+    const int blk = blockIdx.x;
+#endif
+    const int n = blk / p.B, bi = blk % p.B;
     const double cnt = (double)p.npix * p.cg;
     join_groups(p.part + (int64_t)n * p.S * p.groups * 2, p.S, p.groups, sm,
                 [&](int g, double a, double b) { gm[g] = make_float2((float)(a / cnt), (float)(b / cnt)); });
@@ -721,9 +764,18 @@ __global__ __launch_bounds__(TPB) void gn_join_kernel(GnParams p) {
 // ---- host side ------------------------------------------------------------------------------------------------------
 // Splits of an image in both passes: enough workgroups to fill the chip (2048 = 8 per CU), at least 32 KB of the tensor per
 // workgroup, and at most 8192 pairs (128 KB, in L2) for a workgroup of the second pass to join.
-int splits(int esz, int nb, int64_t npix, int c, int groups) {
+#ifndef GN_WGB
+#define GN_WGB 512
+#endif
+#ifndef GN_WGBA
+#define GN_WGBA GN_WGB
+#endif
+#ifndef GN_WGA
+#define GN_WGA GN_WG
+#endif
+int splits(int esz, int nb, int64_t npix, int c, int groups, int wgs) {
     const int64_t bytes = npix * c * esz;
-    int64_t s = (2048 + nb - 1) / nb;
+    int64_t s = (wgs + nb - 1) / nb;
     s = s < bytes / 32768 ? s : bytes / 32768;
     s = s < 8192 / groups ? s : 8192 / groups;
     s = s < npix ? s : npix;
@@ -813,7 +865,7 @@ extern "C" {
 
 size_t mi_groupnorm_act_workspace_bytes(int dtype, int nb, int64_t npix, int c, int groups, int backward) {
     if (check_shape(__func__, dtype, nb, npix, c, groups)) return 0;
-    const size_t s = (size_t)nb * splits(dtype ? 2 : 4, nb, npix, c, groups);
+    const size_t s = (size_t)nb * splits(dtype ? 2 : 4, nb, npix, c, groups, backward ? GN_WGB : GN_WG);
     // a small image's backward pass: [nb][c][2] and at most [nb][groups]
     return (s * groups * 2 + (backward ? s * c * 2 + s : 0)) * sizeof(double);
 }
@@ -843,7 +895,7 @@ int mi_groupnorm_act_fwd(int dtype, int nb, int64_t npix, int c, int groups, con
         GN_SMALL(gn_small_fwd_kernel, nb * p.S, q.groups * 2 * sizeof(double));
         return 0;
     }
-    p.S = p.B = splits(esz, nb, npix, c, groups);
+    p.S = splits(esz, nb, npix, c, groups, GN_WG); p.B = splits(esz, nb, npix, c, groups, GN_WGA);
     GN_LAUNCH(gn_stats_kernel, nb * p.S, groups * 2 * sizeof(double));
     GN_LAUNCH(gn_apply_kernel, nb * p.B, groups * 2 * sizeof(float));
     return 0;
@@ -879,7 +931,7 @@ int mi_groupnorm_act_bwd(int dtype, int nb, int64_t npix, int c, int groups, con
         MI_HIP(hipGetLastError());
         return 0;
     }
-    p.S = p.B = splits(esz, nb, npix, c, groups);
+    p.S = splits(esz, nb, npix, c, groups, GN_WGB); p.B = splits(esz, nb, npix, c, groups, GN_WGBA);
     const size_t s = (size_t)nb * p.S;
     p.part = (double*)workspace;
     p.part_c = p.part + s * groups * 2;
