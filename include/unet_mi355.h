@@ -329,7 +329,7 @@ int mi_groupnorm_act_bwd(int dtype, int nb, int64_t npix, int c, int groups, con
  * as the largest).  values has the type of the logits.  1 <= k <= 256, k <= v <= 2^28. */
 int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, void* values, int32_t* index,
                   void* stream);
-/* Row loss T^2 * KL(q || p): q = softmax(teacher / T) over the used slots of the row's list, p = softmax(logits / T) over all v
+/* Row loss weight * T^2 * KL(q || p): q = softmax(teacher / T) over the used slots of the row's list, p = softmax(logits / T) over all v
  * classes.  A slot is unused when its index lies outside [0, v) or its teacher logit is -inf; a class may be listed
  * more than once (its weights add).  Rows without a used slot have loss 0 and gradient 0, whatever their logits are.
  * teacher [rows][k] (teacher_dtype 0 fp32 | 1 bf16), index [rows][k] (index_dtype 2 int64 | 3 int32), 1 <= k <= 256.
@@ -339,11 +339,18 @@ int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, const void* log
  * Results do not depend on the order in which workgroups run. */
 size_t mi_distill_loss_saved_bytes(int dtype, int64_t rows, int v, int k);
 int mi_distill_loss_fwd(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
-                        const void* teacher, int index_dtype, const void* index, float temperature, int reduction, float* loss,
+                        const void* teacher, int index_dtype, const void* index, float temperature, float weight, int reduction, float* loss,
                         void* saved, void* stream);
+/* Loss and gradient of long rows in one pass over the logits: mi_distill_loss_fwd that also writes dlogits for grad_out = 1
+ * (the mean and the sum).  mi_distill_loss_step_ready says for which sizes it exists (1) or not (0).  mi_distill_loss_bwd with
+ * after_step != 0 and the same dlogits then returns at once where grad_out[0] is 1 and writes the scaled gradient otherwise. */
+int mi_distill_loss_step_ready(int dtype, int64_t rows, int v, int k, int reduction);
+int mi_distill_loss_step(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
+                         const void* teacher, int index_dtype, const void* index, float temperature, float weight, int reduction, float* loss,
+                         void* saved, int64_t dpitch, void* dlogits, void* stream);
 int mi_distill_loss_bwd(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
-                        const void* teacher, int index_dtype, const void* index, float temperature, int reduction,
-                        const float* grad_out, const void* saved, int64_t dpitch, void* dlogits, void* stream);
+                        const void* teacher, int index_dtype, const void* index, float temperature, float weight, int reduction,
+                        const float* grad_out, const void* saved, int after_step, int64_t dpitch, void* dlogits, void* stream);
 
 #ifdef __cplusplus
 }

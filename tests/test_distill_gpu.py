@@ -141,12 +141,19 @@ def definition(z, t, i, temperature, reduction, gout):
     return loss, tol, dz.reshape(full), tol_dz.reshape(full)
 
 
-def check_loss(z, t, i, temperature, reduction, mode):
+def check_loss(z, t, i, temperature, reduction, mode, one=False):
     z = z.detach().requires_grad_(True)
-    out = unet_amd.TopLogitDistillationLoss(temperature, reduction)(z, t, i)
+    fn = unet_amd.TopLogitDistillationLoss(temperature, reduction)
+    with torch.no_grad():
+        alone = fn(z, t, i)                                # without a gradient to come
+    out = fn(z, t, i)
     g = torch.Generator().manual_seed(9)
-    gout = (torch.rand(out.shape, generator=g) + 0.5).to(z.device)
-    (dz,) = torch.autograd.grad(out, z, gout)
+    gout = torch.ones(out.shape) if one else torch.rand(out.shape, generator=g) + 0.5
+    gout = gout.to(z.device)
+    (dz,) = torch.autograd.grad(out, z, gout, retain_graph=True)
+    first = dz.clone()
+    (again,) = torch.autograd.grad(out, z, gout)           # a second backward call: the same numbers, another tensor
+    assert torch.equal(first, dz) and again.data_ptr() != dz.data_ptr()
     loss, tol, ref, tol_dz = definition(z, t, i, temperature, reduction, gout)
     assert out.dtype == torch.float32 and out.shape == loss.shape and dz.shape == z.shape and dz.dtype == z.dtype
     err = (out.detach().double().cpu() - loss).abs()
@@ -154,6 +161,9 @@ def check_loss(z, t, i, temperature, reduction, mode):
     bound = tol_dz * 1.01 + HALF_STEP[mode] * ref.abs() + 1e-37
     err = (dz.double().cpu() - ref).abs()
     assert (err <= bound).all(), float((err / bound).max())
+    for other, limit in ((alone, tol + 1e-37),):
+        assert ((other.double().cpu() - loss).abs() <= limit).all()
+    assert ((again.double().cpu() - ref).abs() <= bound).all()
     return out.detach(), dz
 
 
@@ -170,7 +180,8 @@ def lists(rows, v, k, g, dev, t_dtype=torch.float32, i_dtype=torch.int32, ragged
 
 
 LOSS = [(1, 1, 1), (5, 2, 1), (64, 3, 3), (300, 16, 4), (257, 21, 5), (70, 16, 256), (700, 64, 16), (1000, 133, 8), (33, 512, 64), (17, 1024, 33),
-        (17, 2048, 256), (9, 2049, 7), (9, 1023, 256), (5000, 7, 2), (3, 50001, 32), (1, 32001, 64), (4100, 2050, 3)]
+        (17, 2048, 256), (9, 2049, 7), (9, 1023, 256), (5000, 7, 2), (3, 50001, 32), (1, 32001, 64), (4100, 2050, 3), (7, 8200, 12), (5, 16390, 9), (3, 33000, 4),
+        (2, 70000, 8), (2, 131072, 5), (2, 131080, 5)]
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])
@@ -183,6 +194,7 @@ def test_loss_and_gradient(dev, mode, case):
                                                            ("none", 0.5, torch.float32, torch.int64))):
         t, i = lists(rows, v, k, g, dev, td, idt, ragged=rows > 1)
         check_loss(z, t, i, temperature, reduction, mode)
+        check_loss(z, t, i, temperature, reduction, mode, one=True)
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])
@@ -216,6 +228,7 @@ def test_masks_infinities_and_repeats(dev, mode, v):
     for reduction in ("mean", "sum", "none"):
         # row 11: equal logits at the type's lowest value are a uniform distribution
         out, dz = check_loss(z, t, i, 1.0, reduction, mode)
+        check_loss(z, t, i, 1.0, reduction, mode, one=True)
         assert not dz[2].any() and not dz[3].any() and not dz[4].any()
         assert torch.isfinite(dz).all()
     assert not out[2:5].any()
@@ -299,6 +312,21 @@ def test_gradient_against_differences(dev):
         d1, d2 = (f(h) - f(-h)) / (2 * h), (f(2 * h) - f(-2 * h)) / (4 * h)
         # fourth-order differences of a smooth function: h^4 / 30 of its fifth derivative (a cumulant of d, of order 10), rounding 1e-5 / h
         assert ((4 * d1 - d2) / 3 - (dz.double() * d.double()).sum(-1)).abs().max() < 1e-3
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("v", [48, 5000])
+def test_weight_scales_loss_and_gradient(dev, mode, v):
+    g = torch.Generator().manual_seed(v)
+    z = (torch.randn(9, v, generator=g) * 2).to(DT[mode]).to(dev).requires_grad_(True)
+    t, i = lists(9, v, 4, g, dev)
+    for reduction in ("mean", "sum", "none"):
+        one = unet_amd.TopLogitDistillationLoss(2.0, reduction)(z, t, i)
+        half = unet_amd.TopLogitDistillationLoss(2.0, reduction, weight=-0.5)(z, t, i)
+        assert torch.equal(half, -0.5 * one)               # a power of two: no rounding
+        (d1,) = torch.autograd.grad(one.sum(), z)
+        (d2,) = torch.autograd.grad(half.sum(), z)
+        assert torch.equal(d2, -0.5 * d1)
 
 
 def test_refusals(dev):

@@ -69,23 +69,36 @@ def test_top_logits_and_distillation_arguments_are_checked_on_the_host():
     assert size(1, 4, 16, 4) >= 32 and size(1, 4, 50000, 4) >= 64
     for bad in ((2, 4, 16, 4), (1, 0, 16, 4), (1, 4, 0, 4), (1, 4, 16, 0), (1, 4, 16, 257)):
         assert size(*bad) == 0 and lib.mi_last_error()
-    ok = dict(dtype=1, rows=4, v=16, pitch=16, z=4096, k=4, td=0, t=4096, idt=3, i=4096, temp=1.0, red=1, loss=4096, saved=4096, dp=16, dz=4096, g=4096)
+    ok = dict(dtype=1, rows=4, v=16, pitch=16, z=4096, k=4, td=0, t=4096, idt=3, i=4096, temp=1.0, w=1.0, red=1, loss=4096, saved=4096, dp=16, dz=4096, g=4096, after=0)
 
     def fwd(a):
-        return lib.mi_distill_loss_fwd(a["dtype"], a["rows"], a["v"], a["pitch"], a["z"], a["k"], a["td"], a["t"], a["idt"], a["i"], a["temp"], a["red"],
+        return lib.mi_distill_loss_fwd(a["dtype"], a["rows"], a["v"], a["pitch"], a["z"], a["k"], a["td"], a["t"], a["idt"], a["i"], a["temp"], a["w"], a["red"],
                                        a["loss"], a["saved"], None)
 
     def bwd(a):
-        return lib.mi_distill_loss_bwd(a["dtype"], a["rows"], a["v"], a["pitch"], a["z"], a["k"], a["td"], a["t"], a["idt"], a["i"], a["temp"], a["red"],
-                                       a["g"], a["saved"], a["dp"], a["dz"], None)
+        return lib.mi_distill_loss_bwd(a["dtype"], a["rows"], a["v"], a["pitch"], a["z"], a["k"], a["td"], a["t"], a["idt"], a["i"], a["temp"], a["w"], a["red"],
+                                       a["g"], a["saved"], a["after"], a["dp"], a["dz"], None)
 
     both = ((dict(dtype=-1), b"dtype"), (dict(td=2), b"teacher dtype"), (dict(idt=0), b"index dtype"), (dict(rows=0), b"row"), (dict(v=0), b"classes"),
             (dict(k=0), b"list"), (dict(k=257), b"list"), (dict(pitch=15), b"pitch"), (dict(z=None), b"null"), (dict(t=None), b"null"), (dict(i=None), b"null"),
             (dict(saved=None), b"null"), (dict(temp=0.0), b"temperature"), (dict(temp=-1.0), b"temperature"), (dict(temp=float("inf")), b"temperature"),
-            (dict(temp=float("nan")), b"temperature"), (dict(red=3), b"reduction"), (dict(z=4097), b"address"), (dict(t=4098), b"address"), (dict(i=4097), b"address"))
+            (dict(temp=float("nan")), b"temperature"), (dict(red=3), b"reduction"), (dict(w=float("nan")), b"weight"), (dict(z=4097), b"address"), (dict(t=4098), b"address"), (dict(i=4097), b"address"))
     for kw, text in both:
         for call in (fwd, bwd):
             assert call(dict(ok, **kw)) != 0 and text in lib.mi_last_error(), (kw, lib.mi_last_error())
+    def step(a):
+        return lib.mi_distill_loss_step(a["dtype"], a["rows"], a["v"], a["pitch"], a["z"], a["k"], a["td"], a["t"], a["idt"], a["i"], a["temp"], a["w"], a["red"],
+                                        a["loss"], a["saved"], a["dp"], a["dz"], None)
+
+    wide = dict(ok, v=5000, pitch=5000, dp=5000)
+    ready = lib.mi_distill_loss_step_ready
+    assert ready(1, 4, 5000, 4, 1) == 1 and ready(0, 4, 5000, 4, 2) == 1
+    assert ready(1, 4, 16, 4, 1) == 0 and ready(1, 4, 5000, 4, 0) == 0 and ready(1, 4, 200000, 4, 1) == 0 and ready(2, 4, 5000, 4, 1) == 0
+    assert step(ok) != 0 and b"step_ready" in lib.mi_last_error()
+    assert step(dict(wide, red=0)) != 0 and b"step_ready" in lib.mi_last_error()
+    assert bwd(dict(ok, after=1)) != 0 and b"step" in lib.mi_last_error()
+    for kw, text in both[:-3] + ((dict(dp=15), b"pitch"), (dict(dz=None), b"null"), (dict(loss=None), b"null"), (dict(saved=4100), b"aligned")):
+        assert step(dict(wide, **kw)) != 0 and text in lib.mi_last_error(), (kw, lib.mi_last_error())
     for kw, text in ((dict(dp=15), b"pitch"), (dict(dz=None), b"null"), (dict(g=None), b"null"), (dict(dz=4097), b"address")):
         assert bwd(dict(ok, **kw)) != 0 and text in lib.mi_last_error(), (kw, lib.mi_last_error())
     assert fwd(dict(ok, loss=None)) != 0 and b"null" in lib.mi_last_error()
@@ -97,6 +110,6 @@ def test_distillation_has_no_cpu_path_and_checks_its_options():
         unet_amd.TopLogitDistillationLoss()(z, t, i)
     with pytest.raises(RuntimeError):
         ops.top_logits(z, 2)
-    for bad in (dict(temperature=0), dict(temperature=-1), dict(temperature=float("inf")), dict(temperature=float("nan")), dict(reduction="batchmean")):
+    for bad in (dict(temperature=0), dict(temperature=-1), dict(temperature=float("inf")), dict(temperature=float("nan")), dict(reduction="batchmean"), dict(weight=float("inf"))):
         with pytest.raises(ValueError):
             unet_amd.TopLogitDistillationLoss(**bad)

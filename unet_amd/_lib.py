@@ -144,10 +144,13 @@ PROTOTYPES = {
                                        _P, _P, _P, C.c_int, _P, C.POINTER(MiTensor), _P, _P, _P, _P, _P]),
     "mi_top_logits": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, _P, _P, _P]),
     "mi_distill_loss_saved_bytes": (C.c_size_t, [C.c_int, C.c_int64, C.c_int, C.c_int]),
-    "mi_distill_loss_fwd": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, C.c_int, _P, C.c_int, _P, C.c_float,
+    "mi_distill_loss_fwd": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, C.c_int, _P, C.c_int, _P, C.c_float, C.c_float,
                                       C.c_int, _P, _P, _P]),
-    "mi_distill_loss_bwd": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, C.c_int, _P, C.c_int, _P, C.c_float,
-                                      C.c_int, _P, _P, C.c_int64, _P, _P]),
+    "mi_distill_loss_step_ready": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int]),
+    "mi_distill_loss_step": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, C.c_int, _P, C.c_int, _P, C.c_float, C.c_float,
+                                       C.c_int, _P, _P, C.c_int64, _P, _P]),
+    "mi_distill_loss_bwd": (C.c_int, [C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, C.c_int, _P, C.c_int, _P, C.c_float, C.c_float,
+                                      C.c_int, _P, _P, C.c_int, C.c_int64, _P, _P]),
 }
 
 

@@ -1,17 +1,19 @@
 // Distillation from a teacher's top logits: rows of V class logits z, per row a list of k teacher logits t with their
-// class indices i; temperature T.  Slots whose index lies outside [0, V) are unused, and so are those with t = -inf.
+// class indices i; temperature T, weight w.  Slots whose index lies outside [0, V) are unused, and so are those with t = -inf.
 //
 //   q = softmax over the used slots of t / T ,  log p = z / T - lse(z / T)
-//   row loss = T^2 sum_j q_j (log q_j - log p_{i_j}) ;  dz_v = T gout (p_v - sum_{j: i_j = v} q_j)
+//   row loss = w T^2 sum_j q_j (log q_j - log p_{i_j}) ;  dz_v = w T gout (p_v - sum_{j: i_j = v} q_j)
 //   mean: over the rows with a used slot; the other rows give a loss and a gradient of exactly 0, whatever z holds there.
 //
-// With zm = max z, tm = max t, e_j = exp((t_j - tm) / T): the row loss is T^2 (A / St - log St + log Sz) where
+// With zm = max z, tm = max t, e_j = exp((t_j - tm) / T): the row loss is w T^2 (A / St - log St + log Sz) where
 // A = sum e_j ((t_j - tm) - (z_{i_j} - zm)) / T, St = sum e_j and Sz = sum exp((z - zm) / T): one pass over the row, one
 // over the list, nothing that cancels.
 //
 // Bandwidth-bound: the forward pass cannot do without one read of z, the backward pass without one read and one write.
 //   short rows (up to ROW_REG bytes per lane group): L neighbouring lanes share a row and hold it in registers
 //   long rows : a workgroup per row, one pass with a running maximum and sum per thread
+//   long rows in training: the workgroup holds the row in registers and writes the gradient for gout = 1 in the same
+//                          launch (one read and one write in all); the backward pass recomputes it only for another gout
 #include <string.h>
 
 #include "rows.h"
@@ -30,12 +32,14 @@ struct DistParams {
     char* dz;
     int64_t rows, zp, dzp;            // pitches in bytes
     int v, k, t_bf16, i64, red, L;    // red: 0 none, 1 mean, 2 sum
-    float c, inv_t, T;                // log2(e) / T, 1 / T
+    float c, inv_t, wl, wg;           // log2(e) / T, 1 / T, weight * T^2 (loss), weight * T (gradient)
     float* loss;                      // [rows] (none) or [1]
     float2* stat;                     // long rows: {max z, Sz}
     double* sums;                     // {sum of the rows' losses, rows with a used slot}
     double* part;                     // [workgroups][2]
     int nparts;
+    double* counts;                   // [ncounts] rows with a used slot (training of long rows)
+    int ncounts, done;                // done: dz holds the gradient for gout = 1
     const float* gout;
 };
 
@@ -75,8 +79,8 @@ struct ListSum {
         a = lanes_sum(a, L);
         s = lanes_sum(s, L);
     }
-    __device__ __forceinline__ float loss(float sz, float T) const {
-        return T * T * (a / s + (__builtin_amdgcn_logf(sz) - __builtin_amdgcn_logf(s)) * (float)LN2);
+    __device__ __forceinline__ float loss(float sz, float scale) const {
+        return scale * (a / s + (__builtin_amdgcn_logf(sz) - __builtin_amdgcn_logf(s)) * (float)LN2);
     }
 };
 
@@ -118,18 +122,24 @@ struct Row {
     }
 };
 
+// {a, b} added over a workgroup of T threads in a fixed order; thread 0 has the sums
+template <int T>
+__device__ __forceinline__ double2 block_sum2(double a, double b) {
+    __shared__ double sm[2][T / 64];
+    for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) { sm[0][threadIdx.x >> 6] = a; sm[1][threadIdx.x >> 6] = b; }
+    __syncthreads();
+    a = b = 0.0;
+    if (threadIdx.x == 0)
+        for (int w = 0; w < T / 64; ++w) { a += sm[0][w]; b += sm[1][w]; }
+    return make_double2(a, b);
+}
 // (loss, count) of a workgroup's rows -> part[blockIdx.x]
+template <int T>
 __device__ __forceinline__ void block_part(const DistParams& p, double loss, double count) {
-    __shared__ double sm[2][TPB];
-    sm[0][threadIdx.x] = loss; sm[1][threadIdx.x] = count;
-    for (int h = TPB / 2; h > 0; h >>= 1) {
-        __syncthreads();
-        if ((int)threadIdx.x < h) {
-            sm[0][threadIdx.x] += sm[0][threadIdx.x + h];
-            sm[1][threadIdx.x] += sm[1][threadIdx.x + h];
-        }
-    }
-    if (threadIdx.x == 0) { p.part[2 * blockIdx.x] = sm[0][0]; p.part[2 * blockIdx.x + 1] = sm[1][0]; }
+    const double2 v = block_sum2<T>(loss, count);
+    if (threadIdx.x == 0) reinterpret_cast<double2*>(p.part)[blockIdx.x] = v;
 }
 
 // ---- short rows -----------------------------------------------------------------------------------------------------
@@ -152,12 +162,12 @@ __global__ __launch_bounds__(TPB) void distill_short_fwd(DistParams p) {
             }
         q.join(L, p.inv_t);
         if (l == 0 && in) {
-            const float row = q.some ? q.loss(s, p.T) : 0.0f;
+            const float row = q.some ? q.loss(s, p.wl) : 0.0f;
             if (p.red == 0) p.loss[r] = row;
             if (q.some) { loss += row; count += 1.0; }
         }
     }
-    if (p.red) block_part(p, loss, count);
+    if (p.red) block_part<TPB>(p, loss, count);
 }
 
 // weights of a row's list into LDS (L lanes, k slots): qi class or -1, qw weight summed over the slots of the same class,
@@ -194,7 +204,7 @@ __device__ __forceinline__ float weight_of(const int* qi, const float* qw, int k
     return w;
 }
 __device__ __forceinline__ float grad_scale(const DistParams& p, int64_t r) {
-    const float g = p.gout[p.red ? 0 : r] * p.T;
+    const float g = p.gout[p.red ? 0 : r] * p.wg;
     return p.red == 1 ? g / (float)p.sums[1] : g;
 }
 // LDS written by lanes of this wave is read by others of the same wave
@@ -246,70 +256,199 @@ __global__ __launch_bounds__(TPB) void distill_short_bwd(DistParams p) {
 }
 
 // ---- long rows: a workgroup per row ---------------------------------------------------------------------------------
+// A thread's running {maximum, sum of exp((z - maximum) / T)}.  The sum of a thread that saw nothing above -inf is 0, NaN if it
+// saw a NaN.
+struct RunMax {
+    float m = -INFINITY, s = 0.0f;
+    bool nan = false;
+    template <int N>
+    __device__ __forceinline__ void take(const float* x, float c) {
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
+        const float to = fmaxf(m, top);
+        if (to == -INFINITY) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) nan |= x[j] != x[j];
+            return;
+        }
+        float add = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) add += __builtin_amdgcn_exp2f((x[j] - to) * c);
+        s = m == to ? s + add : fmaf(s, s != 0.0f ? __builtin_amdgcn_exp2f((m - to) * c) : 1.0f, add);
+        m = to;
+    }
+    __device__ __forceinline__ void join_wave(float c) {
+        if (nan) s = NAN;
+        const float to = lanes_max(m, 64);
+        if (s != 0.0f && m != to) s *= __builtin_amdgcn_exp2f((m - to) * c);
+        s = lanes_sum(s, 64);
+        m = to;
+    }
+};
+// the waves' {m, s} joined (every thread of the calling wave): Sz of a row without a distribution is NaN
+template <int T>
+__device__ __forceinline__ float2 join_waves(const float* wm, const float* ws, float c) {
+    float bm = -INFINITY, bs = 0.0f;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) bm = fmaxf(bm, wm[w]);
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) bs += ws[w] != 0.0f ? ws[w] * __builtin_amdgcn_exp2f((wm[w] - bm) * c) : 0.0f;
+    return make_float2(bm, bm == -INFINITY ? NAN : bs);
+}
+// the loss of a row by one wave; lane 0 keeps the books
 template <class TR>
-__global__ __launch_bounds__(TPB) void distill_long_fwd(DistParams p) {
-    __shared__ float sm[2][TPB / 64];
+__device__ __forceinline__ void row_loss(const DistParams& p, int64_t r, const char* z, float2 st, double& loss, double& count) {
+    ListSum q;
+    for (int j = threadIdx.x & 63; j < p.k; j += 64) {
+        const int i = list_i(p, r * p.k + j);
+        if (i >= 0) q.add(list_t(p, r * p.k + j), (ld_one<TR>(z, i) - st.x) * p.inv_t, p.inv_t);
+    }
+    q.join(64, p.inv_t);
+    if ((threadIdx.x & 63) == 0) {
+        const float row = q.some ? q.loss(st.y, p.wl) : 0.0f;
+        p.stat[r] = st;
+        if (p.red == 0) p.loss[r] = row;
+        if (q.some) { loss += row; count += 1.0; }
+    }
+}
+
+template <class TR, int T>
+__global__ __launch_bounds__(T) void distill_long_fwd(DistParams p) {
+    __shared__ float wm[T / 64], ws[T / 64];
     double loss = 0.0, count = 0.0;
+    constexpr int UN = 4;                                         // vectors in flight per thread
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const char* z = p.z + r * p.zp;
-        float m = -INFINITY, s = 0.0f;
-        bool nan = false;
-        auto take = [&](const float* x, int n) {
-            float top = x[0];
-#pragma unroll
-            for (int j = 1; j < n; ++j) top = fmaxf(top, x[j]);
-            if (top > m) { s *= m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * p.c); m = top; }
-            if (m != -INFINITY) {
-#pragma unroll
-                for (int j = 0; j < n; ++j) s += __builtin_amdgcn_exp2f((x[j] - m) * p.c);
-            } else {
-#pragma unroll
-                for (int j = 0; j < n; ++j) nan |= x[j] != x[j];
-            }
-        };
+        RunMax q;
         const int nv = p.v / TR::VEC;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < nv; i += TPB) {
+        int i = threadIdx.x;
+        for (; i + (UN - 1) * T < nv; i += UN * T) {
+            uint4 raw[UN];
+            float x[UN * TR::VEC];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) raw[u] = ld_any<TR>(z + (int64_t)(i + u * T) * 16);
+#pragma unroll
+            for (int u = 0; u < UN; ++u) unpack_vec<TR>(raw[u], x + u * TR::VEC);
+            q.take<UN * TR::VEC>(x, p.c);
+        }
+        for (; i < nv; i += T) {
             float x[TR::VEC];
             unpack_vec<TR>(ld_any<TR>(z + (int64_t)i * 16), x);
-            take(x, TR::VEC);
+            q.take<TR::VEC>(x, p.c);
         }
-        for (int i = nv * TR::VEC + threadIdx.x; i < p.v; i += TPB) {
+        for (i = nv * TR::VEC + threadIdx.x; i < p.v; i += T) {
             const float x = ld_one<TR>(z, i);
-            take(&x, 1);
+            q.take<1>(&x, p.c);
         }
-        if (nan) s = NAN;
-        const float wm = lanes_max(m, 64);
-        s = lanes_sum(m == wm && m != -INFINITY ? s : s * (s != 0.0f ? __builtin_amdgcn_exp2f((m - wm) * p.c) : 1.0f), 64);
+        q.join_wave(p.c);
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) { sm[0][threadIdx.x >> 6] = wm; sm[1][threadIdx.x >> 6] = s; }
+        if ((threadIdx.x & 63) == 0) { wm[threadIdx.x >> 6] = q.m; ws[threadIdx.x >> 6] = q.s; }
         __syncthreads();
-        if (threadIdx.x < 64) {
-            float bm = -INFINITY, bs = 0.0f;
-#pragma unroll
-            for (int w = 0; w < TPB / 64; ++w) bm = fmaxf(bm, sm[0][w]);
-#pragma unroll
-            for (int w = 0; w < TPB / 64; ++w) {
-                const float sw = sm[1][w];
-                bs += sw != 0.0f ? sw * __builtin_amdgcn_exp2f((sm[0][w] - bm) * p.c) : 0.0f;
-            }
-            if (bm == -INFINITY) bs = NAN;                        // nothing but -inf (or NaN): no distribution
-            const int l = threadIdx.x;
-            ListSum q;
-            for (int j = l; j < p.k; j += 64) {
-                const int i = list_i(p, r * p.k + j);
-                if (i >= 0) q.add(list_t(p, r * p.k + j), (ld_one<TR>(z, i) - bm) * p.inv_t, p.inv_t);
-            }
-            q.join(64, p.inv_t);
-            if (l == 0) {
-                const float row = q.some ? q.loss(bs, p.T) : 0.0f;
-                p.stat[r] = make_float2(bm, bs);
-                if (p.red == 0) p.loss[r] = row;
-                if (q.some) { loss += row; count += 1.0; }
-            }
-        }
+        if (threadIdx.x < 64) row_loss<TR>(p, r, z, join_waves<T>(wm, ws, p.c), loss, count);
     }
-    if (p.red) block_part(p, loss, count);
+    if (p.red) block_part<T>(p, loss, count);
+}
+
+// rows with a used slot, per workgroup -> part[2 * blockIdx.x + 1] (where the loss of the same workgroups will lie)
+__global__ __launch_bounds__(TPB) void distill_count(DistParams p) {
+    double n = 0.0;
+    for (int64_t r = (int64_t)blockIdx.x * TPB + threadIdx.x; r < p.rows; r += (int64_t)gridDim.x * TPB) {
+        bool some = false;
+        for (int j = 0; j < p.k && !some; ++j) some = list_i(p, r * p.k + j) >= 0 && list_t(p, r * p.k + j) != -INFINITY;
+        n += some ? 1.0 : 0.0;
+    }
+    const double2 v = block_sum2<TPB>(n, 0.0);
+    if (threadIdx.x == 0) p.counts[blockIdx.x] = v.x;
+}
+
+// loss and gradient for gout = 1 of long rows: up to NV vectors of the row in every thread's registers
+template <class TR, int T, int NV>
+__global__ __launch_bounds__(T, 4) void distill_long_step(DistParams p) {
+    __shared__ float wm[T / 64], ws[T / 64], qw[MAX_K], scale_s;
+    __shared__ int qi[MAX_K], any;
+    const int tid = threadIdx.x;
+    double n = 0.0;
+    if (p.red == 1) {
+        for (int i = tid; i < p.ncounts; i += T) n += p.counts[i];
+        n = block_sum2<T>(n, 0.0).x;
+    }
+    if (tid == 0) scale_s = p.red == 1 ? p.wg / (float)(n > 0.0 ? n : 1.0) : p.wg;
+    double loss = 0.0, count = 0.0;
+    const int nv = p.v / TR::VEC;
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const char* z = p.z + r * p.zp;
+        char* dz = p.dz + r * p.dzp;
+        uint4 raw[NV];                                            // vectors behind the end: -inf
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            constexpr unsigned none = TR::ESZ == 2 ? 0xff80ff80u : 0xff800000u;
+            raw[u] = make_uint4(none, none, none, none);
+            if (u * T + tid < nv) raw[u] = ld_any<TR>(z + u * (T * 16) + (unsigned)tid * 16u);
+        }
+        const int et = nv * TR::VEC + tid;                        // fewer than a vector's worth behind the last one
+        const float tail = et < p.v ? ld_one<TR>(z, et) : -INFINITY;
+        __syncthreads();                                          // the lists of the row before have been read
+        if (tid < 64) {
+            const bool some = list_weights(p, r, true, 64, tid, qi, qw);
+            if (tid == 0) any = some;
+        }
+        // exponentials about the thread's own maximum (0 if it saw nothing above -inf); one factor per thread brings them to the row's
+        RunMax q;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            float x[TR::VEC];
+            unpack_vec<TR>(raw[u], x);
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) q.m = fmaxf(q.m, x[j]);
+        }
+        q.m = fmaxf(q.m, tail);
+        const float base = q.m == -INFINITY ? 0.0f : q.m;
+        constexpr bool KEEP = NV * TR::VEC <= 64;                 // else they are taken twice
+        float e[KEEP ? NV : 1][TR::VEC];
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w));   // unpack again: the row's floats do not fit
+            float* y = e[KEEP ? u : 0];
+            unpack_vec<TR>(raw[u], y);
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) { y[j] = __builtin_amdgcn_exp2f((y[j] - base) * p.c); q.s += y[j]; }
+        }
+        const float etail = __builtin_amdgcn_exp2f((tail - base) * p.c);
+        q.s += etail;
+        const float own = q.m;
+        q.join_wave(p.c);
+        if ((tid & 63) == 0) { wm[tid >> 6] = q.m; ws[tid >> 6] = q.s; }
+        __syncthreads();
+        const float2 st = join_waves<T>(wm, ws, p.c);
+        const bool some = any;
+        const float g = scale_s, f = g / st.y * (own == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((own - st.x) * p.c));
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            float* y = e[KEEP ? u : 0];
+            if (!KEEP) {
+                asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w));
+                unpack_vec<TR>(raw[u], y);
+#pragma unroll
+                for (int j = 0; j < TR::VEC; ++j) y[j] = __builtin_amdgcn_exp2f((y[j] - base) * p.c);
+            }
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) y[j] = some ? f * y[j] : 0.0f;
+            if (u * T + tid < nv) st_any(dz + u * (T * 16) + (unsigned)tid * 16u, pack_vec<TR>(y));
+        }
+        if (et < p.v) st_one<TR>(dz, et, some ? f * etail : 0.0f);
+        if (tid < 64) row_loss<TR>(p, r, z, st, loss, count);
+        __syncthreads();                                          // the classes of the list are written over
+        if (some)
+            for (int j = tid; j < p.k; j += T) {
+                const int i = qi[j];
+                if (i >= 0) {
+                    const float pr = __builtin_amdgcn_exp2f((ld_one<TR>(z, i) - st.x) * p.c) / st.y;
+                    st_one<TR>(dz, i, g * (pr - weight_of(qi, qw, p.k, i)));
+                }
+            }
+    }
+    block_part<T>(p, loss, count);
 }
 
 template <class TR>
@@ -317,6 +456,7 @@ __global__ __launch_bounds__(TPB) void distill_long_bwd(DistParams p) {
     __shared__ int qi[MAX_K];
     __shared__ float qw[MAX_K];
     __shared__ int any;
+    if (p.done && p.gout[0] == 1.0f) return;                      // dz holds this gradient already
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         __syncthreads();
         if (threadIdx.x < 64) {
@@ -353,27 +493,23 @@ __global__ __launch_bounds__(TPB) void distill_long_bwd(DistParams p) {
 }
 
 // sums of the workgroups' parts in a fixed order; the loss
-__global__ __launch_bounds__(TPB) void distill_final(DistParams p) {
-    __shared__ double sm[2][TPB];
+__global__ __launch_bounds__(1024) void distill_final(DistParams p) {
     double a = 0.0, b = 0.0;
-    for (int i = threadIdx.x; i < p.nparts; i += TPB) { a += p.part[2 * i]; b += p.part[2 * i + 1]; }
-    sm[0][threadIdx.x] = a; sm[1][threadIdx.x] = b;
-    for (int h = TPB / 2; h > 0; h >>= 1) {
-        __syncthreads();
-        if ((int)threadIdx.x < h) {
-            sm[0][threadIdx.x] += sm[0][threadIdx.x + h];
-            sm[1][threadIdx.x] += sm[1][threadIdx.x + h];
-        }
+    for (int i = threadIdx.x; i < p.nparts; i += 1024) {
+        const double2 v = reinterpret_cast<const double2*>(p.part)[i];
+        a += v.x; b += v.y;
     }
+    const double2 v = block_sum2<1024>(a, b);
     if (threadIdx.x == 0) {
-        const double n = sm[1][0] > 0.0 ? sm[1][0] : 1.0;         // no row with a used slot: loss 0
-        p.sums[0] = sm[0][0]; p.sums[1] = n;
-        p.loss[0] = (float)(p.red == 1 ? sm[0][0] / n : sm[0][0]);
+        const double n = v.y > 0.0 ? v.y : 1.0;                   // no row with a used slot: loss 0
+        p.sums[0] = v.x; p.sums[1] = n;
+        p.loss[0] = (float)(p.red == 1 ? v.x / n : v.x);
     }
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
-struct Plan { bool is_long; int L, nv, blocks; };
+// Workgroups of a long row's kernels: TODO
+struct Plan { bool is_long; int L, nv, blocks, T, step_t, step_nv; };
 
 // Short rows: the fewest lanes whose registers (NVMAX vectors each) hold the row and whose rows' lists and class
 // weights leave the workgroup within 32 KB of LDS.
@@ -385,13 +521,17 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
     while (q.L < 64 && (nvec > q.L * NVMAX || (TPB / q.L) * (2 * k + v) * 4 > 32768)) q.L *= 2;
     q.nv = 1;
     while (q.nv * q.L < nvec) q.nv *= 2;
+    q.T = rows < 512 ? 1024 : TPB;
+    q.step_t = nvec <= 2048 ? 256 : nvec <= 4096 ? 512 : 1024;
+    q.step_nv = nvec <= 1024 ? 4 : nvec <= 8192 ? 8 : nvec <= 16384 ? 16 : 0;
     const int64_t per = q.is_long ? 1 : TPB / q.L, b = (rows + per - 1) / per;
-    q.blocks = (int)(b < 4096 ? b : 4096);
+    q.blocks = (int)(b < 2048 ? b : 2048);
     return q;
 }
+constexpr int COUNTS = 256;
 
 int check_args(const char* who, int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int t_dtype,
-               const void* teacher, int i_dtype, const void* index, float temperature, int reduction) {
+               const void* teacher, int i_dtype, const void* index, float temperature, float weight, int reduction) {
     auto bad = [&](const char* m) { mi_set_error(std::string(who) + ": " + m); return -1; };
     if (dtype != 0 && dtype != 1) return bad("dtype must be 0 or 1");
     if (t_dtype != 0 && t_dtype != 1) return bad("teacher dtype must be 0 or 1");
@@ -405,6 +545,7 @@ int check_args(const char* who, int dtype, int64_t rows, int v, int64_t pitch, c
     if ((uintptr_t)logits % esz || (uintptr_t)teacher % (t_dtype ? 2 : 4) || (uintptr_t)index % (i_dtype == 2 ? 8 : 4))
         return bad("address is not a multiple of the element size");
     if (!(temperature > 0.0f) || !(temperature < INFINITY)) return bad("temperature must be positive and finite");
+    if (!(weight - weight == 0.0f)) return bad("weight must be finite");
     if (reduction < 0 || reduction > 2) return bad("unknown reduction");
     return 0;
 }
@@ -424,13 +565,16 @@ int check_args(const char* who, int dtype, int64_t rows, int v, int64_t pitch, c
     } while (0)
 
 void fill(DistParams& p, const Plan& q, int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int t_dtype,
-          const void* teacher, int i_dtype, const void* index, float temperature, int reduction, void* saved) {
+          const void* teacher, int i_dtype, const void* index, float temperature, float weight, int reduction, void* saved) {
     memset(&p, 0, sizeof(p));
     p.z = (const char*)logits; p.t = (const char*)teacher; p.idx = (const char*)index;
     p.rows = rows; p.v = v; p.k = k; p.zp = pitch * (dtype ? 2 : 4); p.t_bf16 = t_dtype; p.i64 = i_dtype == 2; p.red = reduction;
-    p.L = q.L; p.T = temperature; p.inv_t = 1.0f / temperature; p.c = (float)(1.4426950408889634 / (double)temperature);
+    p.L = q.L; p.wl = weight * temperature * temperature; p.wg = weight * temperature; p.inv_t = 1.0f / temperature; p.c = (float)(1.4426950408889634 / (double)temperature);
     p.sums = (double*)saved; p.part = p.sums + 2; p.nparts = q.blocks;
-    p.stat = (float2*)(p.part + 2 * q.blocks);
+    p.counts = p.part + 2 * q.blocks;
+    const int64_t c = (rows + TPB - 1) / TPB;
+    p.ncounts = (int)(c < COUNTS ? c : COUNTS);
+    p.stat = (float2*)(p.counts + (q.is_long ? COUNTS : 0));
 }
 
 }  // namespace
@@ -443,45 +587,92 @@ size_t mi_distill_loss_saved_bytes(int dtype, int64_t rows, int v, int k) {
         return 0;
     }
     const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);
-    return sizeof(double) * (2 + 2 * (size_t)q.blocks) + (q.is_long ? sizeof(float2) * (size_t)rows : 0);
+    return sizeof(double) * (2 + 2 * (size_t)q.blocks) + (q.is_long ? sizeof(double) * COUNTS + sizeof(float2) * (size_t)rows : 0);
 }
 
 int mi_distill_loss_fwd(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
-                        const void* teacher, int index_dtype, const void* index, float temperature, int reduction, float* loss,
+                        const void* teacher, int index_dtype, const void* index, float temperature, float weight, int reduction, float* loss,
                         void* saved, void* stream) {
-    if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, reduction)) return r;
+    if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction)) return r;
     MI_CHECK(loss && saved, "null argument");
     MI_CHECK((uintptr_t)saved % 8 == 0 && (uintptr_t)loss % 4 == 0, "saved or loss is not aligned");
     const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);
     DistParams p;
-    fill(p, q, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, reduction, saved);
+    fill(p, q, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction, saved);
     p.loss = loss;
     hipStream_t st = (hipStream_t)stream;
     if (q.is_long) {
-        if (dtype == 1) distill_long_fwd<BF16><<<q.blocks, TPB, 0, st>>>(p);
-        else distill_long_fwd<F32><<<q.blocks, TPB, 0, st>>>(p);
+        if (dtype == 1) {
+            if (q.T == 1024) distill_long_fwd<BF16, 1024><<<q.blocks, 1024, 0, st>>>(p);
+            else distill_long_fwd<BF16, TPB><<<q.blocks, TPB, 0, st>>>(p);
+        } else {
+            if (q.T == 1024) distill_long_fwd<F32, 1024><<<q.blocks, 1024, 0, st>>>(p);
+            else distill_long_fwd<F32, TPB><<<q.blocks, TPB, 0, st>>>(p);
+        }
         MI_HIP(hipGetLastError());
     } else {
         SHORT_LAUNCH(distill_short_fwd, 0);
     }
     if (reduction) {
-        distill_final<<<1, TPB, 0, st>>>(p);
+        distill_final<<<1, 1024, 0, st>>>(p);
         MI_HIP(hipGetLastError());
     }
     return 0;
 }
 
+int mi_distill_loss_step_ready(int dtype, int64_t rows, int v, int k, int reduction) {
+    if ((dtype != 0 && dtype != 1) || rows <= 0 || v <= 0 || k <= 0 || k > MAX_K || reduction <= 0 || reduction > 2) return 0;
+    const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);
+    return q.is_long && q.step_nv > 0;
+}
+
+int mi_distill_loss_step(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
+                         const void* teacher, int index_dtype, const void* index, float temperature, float weight, int reduction, float* loss,
+                         void* saved, int64_t dpitch, void* dlogits, void* stream) {
+    if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction)) return r;
+    MI_CHECK(loss && saved && dlogits, "null argument");
+    MI_CHECK((uintptr_t)saved % 8 == 0 && (uintptr_t)loss % 4 == 0, "saved or loss is not aligned");
+    MI_CHECK(dpitch >= v, "pitch of the gradient must cover the classes");
+    MI_CHECK((uintptr_t)dlogits % (dtype ? 2 : 4) == 0, "address is not a multiple of the element size");
+    MI_CHECK(mi_distill_loss_step_ready(dtype, rows, v, k, reduction), "not for these sizes or this reduction (mi_distill_loss_step_ready)");
+    const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);
+    DistParams p;
+    fill(p, q, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction, saved);
+    p.loss = loss; p.dz = (char*)dlogits; p.dzp = dpitch * (dtype ? 2 : 4);
+    hipStream_t st = (hipStream_t)stream;
+    if (reduction == 1) {
+        distill_count<<<p.ncounts, TPB, 0, st>>>(p);
+        MI_HIP(hipGetLastError());
+    }
+#define STEP_LAUNCH(TR)                                                                                        \
+    do {                                                                                                       \
+        if (q.step_t == 256 && q.step_nv == 4) distill_long_step<TR, 256, 4><<<q.blocks, 256, 0, st>>>(p);     \
+        else if (q.step_t == 256) distill_long_step<TR, 256, 8><<<q.blocks, 256, 0, st>>>(p);                  \
+        else if (q.step_t == 512) distill_long_step<TR, 512, 8><<<q.blocks, 512, 0, st>>>(p);                  \
+        else if (q.step_nv == 8) distill_long_step<TR, 1024, 8><<<q.blocks, 1024, 0, st>>>(p);                 \
+        else distill_long_step<TR, 1024, 16><<<q.blocks, 1024, 0, st>>>(p);                                    \
+    } while (0)
+    if (dtype == 1) STEP_LAUNCH(BF16);
+    else STEP_LAUNCH(F32);
+    MI_HIP(hipGetLastError());
+    distill_final<<<1, 1024, 0, st>>>(p);
+    MI_HIP(hipGetLastError());
+    return 0;
+}
+
 int mi_distill_loss_bwd(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
-                        const void* teacher, int index_dtype, const void* index, float temperature, int reduction,
-                        const float* grad_out, const void* saved, int64_t dpitch, void* dlogits, void* stream) {
-    if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, reduction)) return r;
+                        const void* teacher, int index_dtype, const void* index, float temperature, float weight, int reduction,
+                        const float* grad_out, const void* saved, int after_step, int64_t dpitch, void* dlogits, void* stream) {
+    if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction)) return r;
     MI_CHECK(grad_out && saved && dlogits, "null argument");
     MI_CHECK((uintptr_t)saved % 8 == 0 && (uintptr_t)grad_out % 4 == 0, "saved or grad_out is not aligned");
     MI_CHECK(dpitch >= v, "pitch of the gradient must cover the classes");
     MI_CHECK((uintptr_t)dlogits % (dtype ? 2 : 4) == 0, "address is not a multiple of the element size");
     const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);
     DistParams p;
-    fill(p, q, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, reduction, const_cast<void*>(saved));
+    fill(p, q, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction, const_cast<void*>(saved));
+    MI_CHECK(!after_step || mi_distill_loss_step_ready(dtype, rows, v, k, reduction), "no mi_distill_loss_step for these arguments");
+    p.done = after_step != 0;
     p.gout = grad_out; p.dz = (char*)dlogits; p.dzp = dpitch * (dtype ? 2 : 4);
     hipStream_t st = (hipStream_t)stream;
     if (q.is_long) {

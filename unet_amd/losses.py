@@ -5,6 +5,8 @@ the top logits of a teacher.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn as nn
 
@@ -115,44 +117,62 @@ _REDUCTION = {"none": 0, "mean": 1, "sum": 2}
 _INDEX = {torch.int64: 2, torch.int32: 3}
 
 
+@functools.lru_cache(maxsize=256)
+def _distill_sizes(dt, rows, v, k, red):
+    lib = _lib.load()
+    return lib.mi_distill_loss_saved_bytes(dt, rows, v, k), bool(lib.mi_distill_loss_step_ready(dt, rows, v, k, red))
+
+
 class _DistillFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher, index, temperature, red):
+    def forward(ctx, logits, teacher, index, temperature, weight, red):
         lib, dev = _lib.load(), logits.device
         z, pitch = _pixels(logits, "input")
         v, k = z.shape[-1], index.shape[-1]
         rows = index.numel() // k
         loss = torch.empty(index.shape[:-1] if red == 0 else (), dtype=torch.float32, device=dev)
-        args = (_DT[z.dtype], rows, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(), _INDEX[index.dtype],
-                index.data_ptr(), temperature, red)
+        dt = _DT[z.dtype]
+        nbytes, in_one = _distill_sizes(dt, rows, v, k, red)
+        args = (dt, rows, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(), _INDEX[index.dtype],
+                index.data_ptr(), temperature, weight, red)
+        train = ctx.needs_input_grad[0]
+        dz = None
         with _lib.on_device(dev):
-            saved = torch.empty(lib.mi_distill_loss_saved_bytes(args[0], rows, v, k), dtype=torch.uint8, device=dev)
-            _lib.check(lib.mi_distill_loss_fwd(*args, loss.data_ptr(), saved.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_fwd")
-        if ctx.needs_input_grad[0]:
+            saved = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            if train and in_one:
+                dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
+                _lib.check(lib.mi_distill_loss_step(*args, loss.data_ptr(), saved.data_ptr(), v, dz.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_step")
+            else:
+                _lib.check(lib.mi_distill_loss_fwd(*args, loss.data_ptr(), saved.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_fwd")
+        if train:
             ctx.save_for_backward(logits, teacher, index, saved)
-            ctx.cfg = (temperature, red)
+            ctx.cfg = (temperature, weight, red)
+            ctx.dz = dz      # the gradient for gout = 1; given away by the first backward call
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout):
         logits, teacher, index, saved = ctx.saved_tensors
-        temperature, red = ctx.cfg
+        temperature, weight, red = ctx.cfg
         lib, dev = _lib.load(), logits.device
         z, pitch = _pixels(logits, "input")
         v, k = z.shape[-1], index.shape[-1]
-        dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
+        dz, ctx.dz = ctx.dz, None
+        done = dz is not None
+        if not done:
+            dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
         g = gout.contiguous().float()
         with _lib.on_device(dev):
             _lib.check(lib.mi_distill_loss_bwd(_DT[z.dtype], index.numel() // k, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(),
-                                               _INDEX[index.dtype], index.data_ptr(), temperature, red, g.data_ptr(), saved.data_ptr(),
-                                               v, dz.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_bwd")
-        return dz, None, None, None, None
+                                               _INDEX[index.dtype], index.data_ptr(), temperature, weight, red, g.data_ptr(), saved.data_ptr(),
+                                               1 if done else 0, v, dz.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_bwd")
+        return dz, None, None, None, None, None
 
 
 class TopLogitDistillationLoss(nn.Module):
     """Trains a student on the top logits of a teacher (``ops.top_logits``):
-    ``temperature**2 * KL(q || softmax(input / temperature))`` per pixel, where ``q`` is the softmax of the pixel's listed
+    ``weight * temperature**2 * KL(q || softmax(input / temperature))`` per pixel, where ``q`` is the softmax of the pixel's listed
     teacher logits over ``temperature``.
 
     ``forward(input, teacher_logits, teacher_index)``: ``input`` [.., V] class logits of the student, channels last, fp32 or
@@ -160,16 +180,22 @@ class TopLogitDistillationLoss(nn.Module):
     [.., k] (int32 or int64), k at most 256.  A slot whose index lies outside [0, V), or whose logit is -inf, is unused: -1
     fills up short lists and leaves out pixels.  The weights of a class listed twice add.  ``reduction``: "mean" over the pixels with a used slot (0 if
     there are none), "sum", or "none" (one loss per pixel, 0 where no slot is used).  The gradient flows to ``input`` alone.
+
+    With more classes than 64 lanes hold (2048 bf16, 1024 fp32) the forward call of a training step writes the gradient along, for
+    an upstream gradient of 1: ``backward`` then has nothing left to do, and computes it again for any other (give ``weight``
+    instead of multiplying the loss).
     """
 
-    def __init__(self, temperature=1.0, reduction="mean"):
+    def __init__(self, temperature=1.0, reduction="mean", weight=1.0):
         super().__init__()
-        temperature = float(temperature)
+        temperature, weight = float(temperature), float(weight)
         if not 0.0 < temperature < float("inf"):
             raise ValueError(f"temperature must be positive and finite, got {temperature}")
+        if not abs(weight) < float("inf"):
+            raise ValueError(f"weight must be finite, got {weight}")
         if reduction not in _REDUCTION:
             raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
-        self.temperature, self.reduction = temperature, reduction
+        self.temperature, self.reduction, self.weight = temperature, reduction, weight
 
     def forward(self, input: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor) -> torch.Tensor:
         x = input.as_subclass(torch.Tensor) if type(input) is not torch.Tensor else input
@@ -196,4 +222,4 @@ class TopLogitDistillationLoss(nn.Module):
         if i.numel() == 0:
             total = x.float().sum(-1)                              # nothing to learn from: zeros that know the input
             return total if red == 0 else total.sum()
-        return _DistillFunction.apply(x, t.contiguous(), i.contiguous(), self.temperature, red)
+        return _DistillFunction.apply(x, t.contiguous(), i.contiguous(), self.temperature, self.weight, red)
