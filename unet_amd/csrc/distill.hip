@@ -22,6 +22,7 @@
 namespace {
 
 constexpr int TPB = 256;
+constexpr int STEP_WGS = 1024;        // workgroups of the step kernel (its rows are prefetched from one to the next)
 constexpr int MAX_K = 256;
 constexpr int NVMAX = 4;              // 16-byte vectors of a row that a lane holds
 constexpr float LOG2E = 1.4426950408889634f;
@@ -171,8 +172,8 @@ __global__ __launch_bounds__(TPB) void distill_short_fwd(DistParams p) {
 }
 
 // weights of a row's list into LDS (L lanes, k slots): qi class or -1, qw weight summed over the slots of the same class,
-// in the order of the list.  Returns whether a slot is used.
-__device__ __forceinline__ bool list_weights(const DistParams& p, int64_t r, bool in, int L, int l, int* qi, float* qw) {
+// in the order of the list, qt teacher logit (may be qw).  Returns whether a slot is used.
+__device__ __forceinline__ bool list_weights(const DistParams& p, int64_t r, bool in, int L, int l, int* qi, float* qw, float* qt) {
     float m = -INFINITY;
     bool some = false;
     if (in)
@@ -181,14 +182,14 @@ __device__ __forceinline__ bool list_weights(const DistParams& p, int64_t r, boo
             const float t = list_t(p, r * p.k + j);
             if (t == -INFINITY) i = -1;
             if (i >= 0) { m = fmaxf(m, t); some = true; }
-            qi[j] = i; qw[j] = t;
+            qi[j] = i; qt[j] = t;
         }
     m = lanes_max(m, L);
     some = (bool)lanes_max(some ? 1.0f : 0.0f, L);
     float s = 0.0f;
     if (in)
         for (int j = l; j < p.k; j += L) {
-            const float e = qi[j] >= 0 ? __builtin_amdgcn_exp2f((qw[j] - m) * p.c) : 0.0f;
+            const float e = qi[j] >= 0 ? __builtin_amdgcn_exp2f((qt[j] - m) * p.c) : 0.0f;
             qw[j] = e; s += e;
         }
     s = lanes_sum(s, L);
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(TPB) void distill_short_bwd(DistParams p) {
         x.load(p.z + (in ? r : 0) * p.zp, p.v, L, l);
         const float m = x.max_of(L), s = x.exp_of(m, p.c, L);
         for (int i = l; i < p.v; i += L) acc[i] = 0.0f;
-        const bool some = list_weights(p, r, in, L, l, qi, qw);
+        const bool some = list_weights(p, r, in, L, l, qi, qw, qw);
         wave_sync();
         if (in && some)
             for (int j = l; j < p.k; j += L)
@@ -350,22 +351,29 @@ __global__ __launch_bounds__(T) void distill_long_fwd(DistParams p) {
     if (p.red) block_part<T>(p, loss, count);
 }
 
-// rows with a used slot, per workgroup -> part[2 * blockIdx.x + 1] (where the loss of the same workgroups will lie)
-__global__ __launch_bounds__(TPB) void distill_count(DistParams p) {
+// rows with a used slot, per workgroup
+__global__ __launch_bounds__(64) void distill_count(DistParams p) {
     double n = 0.0;
-    for (int64_t r = (int64_t)blockIdx.x * TPB + threadIdx.x; r < p.rows; r += (int64_t)gridDim.x * TPB) {
+    for (int64_t r = (int64_t)blockIdx.x * 64 + threadIdx.x; r < p.rows; r += (int64_t)gridDim.x * 64) {
         bool some = false;
-        for (int j = 0; j < p.k && !some; ++j) some = list_i(p, r * p.k + j) >= 0 && list_t(p, r * p.k + j) != -INFINITY;
+        for (int j = 0; j < p.k && !some; ++j) some = (list_i(p, r * p.k + j) >= 0) & (list_t(p, r * p.k + j) != -INFINITY);
         n += some ? 1.0 : 0.0;
     }
-    const double2 v = block_sum2<TPB>(n, 0.0);
-    if (threadIdx.x == 0) p.counts[blockIdx.x] = v.x;
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    if (threadIdx.x == 0) p.counts[blockIdx.x] = n;
 }
 
-// loss and gradient for gout = 1 of long rows: up to NV vectors of the row in every thread's registers
+// the compiler takes the value as new: what was computed from it before is not kept in registers
+__device__ __forceinline__ void hold(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+
+// Loss and gradient for gout = 1 of long rows: up to NV vectors of the row in every thread's registers.  The list and the
+// student's logits of its classes are fetched while the row is on its way, so that no wave waits for memory once it is there; as
+// a vector's gradient is stored, the same vector of the next row is requested.  The exponentials are taken twice: kept, they
+// need twice the registers of the bf16 row, and fewer rows in flight cost more than the arithmetic (4096 x 32768 bf16 step: 160 us
+// kept, 138 taken twice, 190 with two passes over memory).
 template <class TR, int T, int NV>
 __global__ __launch_bounds__(T, 4) void distill_long_step(DistParams p) {
-    __shared__ float wm[T / 64], ws[T / 64], qw[MAX_K], scale_s;
+    __shared__ float wm[T / 64], ws[T / 64], qw[MAX_K], qt[MAX_K], qz[MAX_K], scale_s;
     __shared__ int qi[MAX_K], any;
     const int tid = threadIdx.x;
     double n = 0.0;
@@ -375,25 +383,30 @@ __global__ __launch_bounds__(T, 4) void distill_long_step(DistParams p) {
     }
     if (tid == 0) scale_s = p.red == 1 ? p.wg / (float)(n > 0.0 ? n : 1.0) : p.wg;
     double loss = 0.0, count = 0.0;
-    const int nv = p.v / TR::VEC;
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const int nv = p.v / TR::VEC, et = nv * TR::VEC + tid;        // et: fewer than a vector's worth behind the last vector
+    uint4 raw[NV];                                                // vectors behind the end: -inf
+    float tail = -INFINITY;
+    auto fetch = [&](const char* z, int u) {
+        constexpr unsigned none = TR::ESZ == 2 ? 0xff80ff80u : 0xff800000u;
+        raw[u] = make_uint4(none, none, none, none);
+        if (u * T + tid < nv) raw[u] = ld_any<TR>(z + u * (T * 16) + (unsigned)tid * 16u);
+    };
+    int64_t r = blockIdx.x;
+    if (r < p.rows) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) fetch(p.z + r * p.zp, u);
+        tail = et < p.v ? ld_one<TR>(p.z + r * p.zp, et) : -INFINITY;
+    }
+    for (; r < p.rows; r += gridDim.x) {
         const char* z = p.z + r * p.zp;
         char* dz = p.dz + r * p.dzp;
-        uint4 raw[NV];                                            // vectors behind the end: -inf
-#pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            constexpr unsigned none = TR::ESZ == 2 ? 0xff80ff80u : 0xff800000u;
-            raw[u] = make_uint4(none, none, none, none);
-            if (u * T + tid < nv) raw[u] = ld_any<TR>(z + u * (T * 16) + (unsigned)tid * 16u);
-        }
-        const int et = nv * TR::VEC + tid;                        // fewer than a vector's worth behind the last one
-        const float tail = et < p.v ? ld_one<TR>(z, et) : -INFINITY;
-        __syncthreads();                                          // the lists of the row before have been read
+        __syncthreads();                                          // the list of the row before has been read
         if (tid < 64) {
-            const bool some = list_weights(p, r, true, 64, tid, qi, qw);
+            const bool some = list_weights(p, r, true, 64, tid, qi, qw, qt);
+            for (int j = tid; j < p.k; j += 64) qz[j] = qi[j] >= 0 ? ld_one<TR>(z, qi[j]) : 0.0f;
             if (tid == 0) any = some;
         }
-        // exponentials about the thread's own maximum (0 if it saw nothing above -inf); one factor per thread brings them to the row's
+        // the sum about the thread's own maximum (0 if it saw nothing above -inf), brought to the row's maximum by the join
         RunMax q;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
@@ -404,48 +417,52 @@ __global__ __launch_bounds__(T, 4) void distill_long_step(DistParams p) {
         }
         q.m = fmaxf(q.m, tail);
         const float base = q.m == -INFINITY ? 0.0f : q.m;
-        constexpr bool KEEP = NV * TR::VEC <= 64;                 // else they are taken twice
-        float e[KEEP ? NV : 1][TR::VEC];
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w));   // unpack again: the row's floats do not fit
-            float* y = e[KEEP ? u : 0];
+            hold(raw[u]);
+            float y[TR::VEC];
             unpack_vec<TR>(raw[u], y);
 #pragma unroll
             for (int j = 0; j < TR::VEC; ++j) { y[j] = __builtin_amdgcn_exp2f((y[j] - base) * p.c); q.s += y[j]; }
         }
-        const float etail = __builtin_amdgcn_exp2f((tail - base) * p.c);
-        q.s += etail;
-        const float own = q.m;
+        q.s += __builtin_amdgcn_exp2f((tail - base) * p.c);
         q.join_wave(p.c);
         if ((tid & 63) == 0) { wm[tid >> 6] = q.m; ws[tid >> 6] = q.s; }
         __syncthreads();
         const float2 st = join_waves<T>(wm, ws, p.c);
         const bool some = any;
-        const float g = scale_s, f = g / st.y * (own == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((own - st.x) * p.c));
+        const float g = scale_s, f = g / st.y;
+        const bool more = r + gridDim.x < p.rows;
+        const char* zn = p.z + (r + gridDim.x) * p.zp;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            float* y = e[KEEP ? u : 0];
-            if (!KEEP) {
-                asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w));
-                unpack_vec<TR>(raw[u], y);
+            hold(raw[u]);
+            float y[TR::VEC];
+            unpack_vec<TR>(raw[u], y);
 #pragma unroll
-                for (int j = 0; j < TR::VEC; ++j) y[j] = __builtin_amdgcn_exp2f((y[j] - base) * p.c);
-            }
-#pragma unroll
-            for (int j = 0; j < TR::VEC; ++j) y[j] = some ? f * y[j] : 0.0f;
+            for (int j = 0; j < TR::VEC; ++j) y[j] = some ? f * __builtin_amdgcn_exp2f((y[j] - st.x) * p.c) : 0.0f;
             if (u * T + tid < nv) st_any(dz + u * (T * 16) + (unsigned)tid * 16u, pack_vec<TR>(y));
+            if (more) fetch(zn, u);
         }
-        if (et < p.v) st_one<TR>(dz, et, some ? f * etail : 0.0f);
-        if (tid < 64) row_loss<TR>(p, r, z, st, loss, count);
+        if (et < p.v) {
+            st_one<TR>(dz, et, some ? f * __builtin_amdgcn_exp2f((tail - st.x) * p.c) : 0.0f);
+            if (more) tail = ld_one<TR>(zn, et);
+        }
+        if (tid < 64) {
+            ListSum ls;
+            for (int j = tid; j < p.k; j += 64)
+                if (qi[j] >= 0) ls.add(qt[j], (qz[j] - st.x) * p.inv_t, p.inv_t);
+            ls.join(64, p.inv_t);
+            if (tid == 0) {
+                p.stat[r] = st;
+                if (ls.some) { loss += ls.loss(st.y, p.wl); count += 1.0; }
+            }
+        }
         __syncthreads();                                          // the classes of the list are written over
         if (some)
             for (int j = tid; j < p.k; j += T) {
                 const int i = qi[j];
-                if (i >= 0) {
-                    const float pr = __builtin_amdgcn_exp2f((ld_one<TR>(z, i) - st.x) * p.c) / st.y;
-                    st_one<TR>(dz, i, g * (pr - weight_of(qi, qw, p.k, i)));
-                }
+                if (i >= 0) st_one<TR>(dz, i, g * (__builtin_amdgcn_exp2f((qz[j] - st.x) * p.c) / st.y - weight_of(qi, qw, p.k, i)));
             }
     }
     block_part<T>(p, loss, count);
@@ -460,7 +477,7 @@ __global__ __launch_bounds__(TPB) void distill_long_bwd(DistParams p) {
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         __syncthreads();
         if (threadIdx.x < 64) {
-            const bool some = list_weights(p, r, true, 64, threadIdx.x, qi, qw);
+            const bool some = list_weights(p, r, true, 64, threadIdx.x, qi, qw, qw);
             if (threadIdx.x == 0) any = some;
         }
         __syncthreads();
@@ -492,7 +509,9 @@ __global__ __launch_bounds__(TPB) void distill_long_bwd(DistParams p) {
     }
 }
 
-// sums of the workgroups' parts in a fixed order; the loss
+// Sums of the workgroups' parts in a fixed order; the loss.  A launch of its own: the last workgroup of the kernel before
+// could do it behind a device-wide fence, but that writes the L2 back once per workgroup (4096 x 32768 bf16 step, 512
+// workgroups: 182 us against 160).
 __global__ __launch_bounds__(1024) void distill_final(DistParams p) {
     double a = 0.0, b = 0.0;
     for (int i = threadIdx.x; i < p.nparts; i += 1024) {
@@ -508,7 +527,8 @@ __global__ __launch_bounds__(1024) void distill_final(DistParams p) {
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
-// Workgroups of a long row's kernels: TODO
+// Long rows: forward with 1024 threads a row where rows alone do not fill the chip (5 x 32001 fp32: 13.1 -> 7.8 us), else 256.
+// Step: the fewest threads that hold the row with 4 or 8 vectors each, up to 1024 threads with 16 (262144 bytes of row).
 struct Plan { bool is_long; int L, nv, blocks, T, step_t, step_nv; };
 
 // Short rows: the fewest lanes whose registers (NVMAX vectors each) hold the row and whose rows' lists and class
@@ -528,7 +548,7 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
     q.blocks = (int)(b < 2048 ? b : 2048);
     return q;
 }
-constexpr int COUNTS = 256;
+constexpr int COUNTS = 512;
 
 int check_args(const char* who, int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int t_dtype,
                const void* teacher, int i_dtype, const void* index, float temperature, float weight, int reduction) {
@@ -572,7 +592,7 @@ void fill(DistParams& p, const Plan& q, int dtype, int64_t rows, int v, int64_t 
     p.L = q.L; p.wl = weight * temperature * temperature; p.wg = weight * temperature; p.inv_t = 1.0f / temperature; p.c = (float)(1.4426950408889634 / (double)temperature);
     p.sums = (double*)saved; p.part = p.sums + 2; p.nparts = q.blocks;
     p.counts = p.part + 2 * q.blocks;
-    const int64_t c = (rows + TPB - 1) / TPB;
+    const int64_t c = (rows + 63) / 64;
     p.ncounts = (int)(c < COUNTS ? c : COUNTS);
     p.stat = (float2*)(p.counts + (q.is_long ? COUNTS : 0));
 }
@@ -640,17 +660,18 @@ int mi_distill_loss_step(int dtype, int64_t rows, int v, int64_t pitch, const vo
     fill(p, q, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction, saved);
     p.loss = loss; p.dz = (char*)dlogits; p.dzp = dpitch * (dtype ? 2 : 4);
     hipStream_t st = (hipStream_t)stream;
+    p.nparts = q.blocks < STEP_WGS ? q.blocks : STEP_WGS;
     if (reduction == 1) {
-        distill_count<<<p.ncounts, TPB, 0, st>>>(p);
+        distill_count<<<p.ncounts, 64, 0, st>>>(p);
         MI_HIP(hipGetLastError());
     }
 #define STEP_LAUNCH(TR)                                                                                        \
     do {                                                                                                       \
-        if (q.step_t == 256 && q.step_nv == 4) distill_long_step<TR, 256, 4><<<q.blocks, 256, 0, st>>>(p);     \
-        else if (q.step_t == 256) distill_long_step<TR, 256, 8><<<q.blocks, 256, 0, st>>>(p);                  \
-        else if (q.step_t == 512) distill_long_step<TR, 512, 8><<<q.blocks, 512, 0, st>>>(p);                  \
-        else if (q.step_nv == 8) distill_long_step<TR, 1024, 8><<<q.blocks, 1024, 0, st>>>(p);                 \
-        else distill_long_step<TR, 1024, 16><<<q.blocks, 1024, 0, st>>>(p);                                    \
+        if (q.step_t == 256 && q.step_nv == 4) distill_long_step<TR, 256, 4><<<p.nparts, 256, 0, st>>>(p);     \
+        else if (q.step_t == 256) distill_long_step<TR, 256, 8><<<p.nparts, 256, 0, st>>>(p);                  \
+        else if (q.step_t == 512) distill_long_step<TR, 512, 8><<<p.nparts, 512, 0, st>>>(p);                  \
+        else if (q.step_nv == 8) distill_long_step<TR, 1024, 8><<<p.nparts, 1024, 0, st>>>(p);                 \
+        else distill_long_step<TR, 1024, 16><<<p.nparts, 1024, 0, st>>>(p);                                    \
     } while (0)
     if (dtype == 1) STEP_LAUNCH(BF16);
     else STEP_LAUNCH(F32);
@@ -676,8 +697,9 @@ int mi_distill_loss_bwd(int dtype, int64_t rows, int v, int64_t pitch, const voi
     p.gout = grad_out; p.dz = (char*)dlogits; p.dzp = dpitch * (dtype ? 2 : 4);
     hipStream_t st = (hipStream_t)stream;
     if (q.is_long) {
-        if (dtype == 1) distill_long_bwd<BF16><<<q.blocks, TPB, 0, st>>>(p);
-        else distill_long_bwd<F32><<<q.blocks, TPB, 0, st>>>(p);
+        const int blocks = p.done && q.blocks > 512 ? 512 : q.blocks;  // mostly there to leave again
+        if (dtype == 1) distill_long_bwd<BF16><<<blocks, TPB, 0, st>>>(p);
+        else distill_long_bwd<F32><<<blocks, TPB, 0, st>>>(p);
         MI_HIP(hipGetLastError());
     } else {
         const int lds = (TPB / q.L) * (2 * k + v) * 4;
