@@ -363,9 +363,6 @@ __global__ __launch_bounds__(64) void distill_count(DistParams p) {
     if (threadIdx.x == 0) p.counts[blockIdx.x] = n;
 }
 
-// the compiler takes the value as new: what was computed from it before is not kept in registers
-__device__ __forceinline__ void hold(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
-
 // Loss and gradient for gout = 1 of long rows: up to NV vectors of the row in every thread's registers.  The list and the
 // student's logits of its classes are fetched while the row is on its way, so that no wave waits for memory once it is there; as
 // a vector's gradient is stored, the same vector of the next row is requested.  The exponentials are taken twice: kept, they

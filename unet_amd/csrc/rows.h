@@ -25,6 +25,9 @@ __device__ __forceinline__ void st_one(char* p, int64_t i, float v) {
     else reinterpret_cast<float*>(p)[i] = v;
 }
 
+// the compiler takes the value as new: what was computed from it before is not kept in registers
+__device__ __forceinline__ void hold(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+
 // maximum / sum over the L neighbouring lanes that share a row (L a power of two)
 __device__ __forceinline__ float lanes_max(float v, int L) {
     for (int o = L >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));

@@ -5,11 +5,13 @@
 // value and stands for "none".
 //
 // Bandwidth-bound: the rows have to be read once.
-//   short lists of short rows: L neighbouring lanes hold a row in registers and take the largest out k times
-//   everything else: a workgroup per row.  Every thread finds the largest key of its part; at least k classes lie at or
-//   above the k-th largest of these maxima.  The row is read again and the classes from there on are gathered in LDS;
-//   a class's place is the number of gathered full keys above its own.  Rows with so many equal values that they do not
-//   fit get the exact k-th largest full key by halving the interval of full keys.
+//   top_short: lists of a few entries; L neighbouring lanes hold a row in registers and take the largest out k times
+//   top_wave : a wave holds the row; the k-th largest key is found bit by bit, by counting the keys from there on, the k classes
+//              are gathered in LDS (equal keys by ascending class) and placed by the number of full keys above their own
+//   top_long : a workgroup streams the row and keeps the largest key of every thread's part.  At least k classes lie at or above
+//              the k-th largest of the maxima of groups of threads; only threads that saw such a class have theirs read again
+//              (from L2), the classes from there on are gathered in LDS and placed.  Rows with so many equal values that they do
+//              not fit get the exact k-th largest key, the classes above it and the first ones at it
 #include <string.h>
 
 #include "rows.h"
@@ -20,14 +22,17 @@ namespace {
 constexpr int TPB = 256;
 constexpr int MAX_K = 256;
 constexpr int NVMAX = 4;
-constexpr int CAP = 1024;             // gathered classes
+#ifndef TROWS
+#define TROWS 512
+#endif
+constexpr int CAP = 2048;             // gathered classes of a long row
 
 struct TopParams {
     const char* x;
     char* val;
     int* idx;
     int64_t rows, xp;
-    int v, k, L;
+    int v, k, L, G;
 };
 
 __device__ __forceinline__ unsigned key_of(float f) {
@@ -47,6 +52,24 @@ __device__ __forceinline__ void emit(const TopParams& p, int64_t r, int place, i
     p.idx[at] = i;
 }
 
+// the keys of a row in the registers of L lanes: vector i of lane l is vector i * L + l; behind the end 0
+template <class TR, int NV>
+__device__ __forceinline__ void load_keys(const char* x, int v, int L, int l, unsigned (&key)[NV][TR::VEC]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e0 = (i * L + l) * TR::VEC;
+        if (e0 + TR::VEC <= v) {
+            float f[TR::VEC];
+            unpack_vec<TR>(ld_any<TR>(x + (int64_t)e0 * TR::ESZ), f);
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) key[i][j] = key_of(f[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) key[i][j] = e0 + j < v ? key_of(ld_one<TR>(x, e0 + j)) : 0u;
+        }
+    }
+}
+
 template <class TR, int NV>
 __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
     const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L;
@@ -55,19 +78,7 @@ __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
         const bool in = r < p.rows;
         const char* x = p.x + (in ? r : 0) * p.xp;
         unsigned key[NV][TR::VEC];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e0 = (i * L + l) * TR::VEC;
-            if (e0 + TR::VEC <= p.v) {
-                float f[TR::VEC];
-                unpack_vec<TR>(ld_any<TR>(x + (int64_t)e0 * TR::ESZ), f);
-#pragma unroll
-                for (int j = 0; j < TR::VEC; ++j) key[i][j] = key_of(f[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < TR::VEC; ++j) key[i][j] = e0 + j < p.v ? key_of(ld_one<TR>(x, e0 + j)) : 0u;
-            }
-        }
+        load_keys<TR, NV>(x, p.v, L, l, key);
         for (int n = 0; n < p.k; ++n) {
             unsigned best = 0;
             int at = 0x7fffffff;
@@ -91,114 +102,296 @@ __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
     }
 }
 
-// f(key, class) for the classes of a row, TPB threads side by side
-template <class TR, class F>
+// ---- a wave per row -----------------------------------------------------------------------------------------------------
+// exclusive prefix sum over the lanes; all: the sum
+__device__ __forceinline__ int lanes_before(int v, int& all) {
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(s, o, 64);
+        s += (int)(threadIdx.x & 63) >= o ? u : 0;
+    }
+    all = __shfl(s, 63, 64);
+    return s - v;
+}
+template <class TR, int NV>
+__global__ __launch_bounds__(TPB) void top_wave(TopParams p) {
+    __shared__ u64 list[TPB / 64][MAX_K];
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    u64* mine = list[w];
+    for (int64_t r = (int64_t)blockIdx.x * (TPB / 64) + w; r < p.rows; r += (int64_t)gridDim.x * (TPB / 64)) {
+        const char* x = p.x + r * p.xp;
+        unsigned key[NV][TR::VEC];
+        load_keys<TR, NV>(x, p.v, 64, l, key);
+        unsigned t = 0;                                            // the largest number that k keys reach
+#pragma unroll 1
+        for (int bit = 31; bit >= 32 - 8 * TR::ESZ; --bit) {       // the lower half of a bf16 key follows from its sign
+            const unsigned want = t | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < TR::VEC; ++j) n += __popcll(__ballot(key[i][j] >= want));
+            if (n >= p.k) t = want;
+        }
+        // above: keys whose compared bits exceed t; equal: the first ones by class fill the list
+        const unsigned mask = TR::ESZ == 2 ? 0xffff0000u : 0xffffffffu;
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) above += __popcll(__ballot((key[i][j] & mask) > t));
+        int na = 0, ne = above;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            int ca = 0, ce = 0;
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) {
+                ca += (key[i][j] & mask) > t ? 1 : 0;
+                ce += key[i][j] && (key[i][j] & mask) == t ? 1 : 0;
+            }
+            int all;
+            const int before = lanes_before(ca | ce << 16, all);
+            int pa = na + (before & 0xffff), pe = ne + (before >> 16);
+            na += all & 0xffff; ne += all >> 16;
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) {
+                const unsigned kk = key[i][j] & mask;
+                const int cls = (i * 64 + l) * TR::VEC + j;
+                if (kk > t) mine[pa++] = full_key(kk, cls);
+                else if (key[i][j] && kk == t) { if (pe < p.k) mine[pe] = full_key(kk, cls); ++pe; }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        for (int a = l; a < p.k; a += 64) {
+            const u64 f = mine[a];
+            int place = 0;
+            for (int b = 0; b < p.k; ++b) place += mine[b] > f ? 1 : 0;
+            emit<TR>(p, r, place, (int)~(unsigned)f);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---- a workgroup per row ------------------------------------------------------------------------------------------------
+// Largest key of 16-byte vectors without making the keys: the bits of a value, with the lower ones turned over if it is
+// negative, order as signed numbers, two bf16 at a time, except that NaN with a sign lies below -inf; the smallest such number
+// tells whether there is one.  2.5 (bf16) and 5 (fp32) instructions per class instead of 9.
+typedef short s2 __attribute__((ext_vector_type(2)));
+template <class TR> struct BestOf;
+template <> struct BestOf<BF16> {
+    s2 hi = {-32768, -32768}, lo = {32767, 32767};
+    __device__ __forceinline__ void word(unsigned w) {
+        s2 v = __builtin_bit_cast(s2, w);
+        v ^= (v >> 15) & (short)0x7fff;
+        hi = __builtin_elementwise_max(hi, v);
+        lo = __builtin_elementwise_min(lo, v);
+    }
+    __device__ __forceinline__ unsigned key() const {
+        short h = hi.x > hi.y ? hi.x : hi.y;
+        const short l = lo.x < lo.y ? lo.x : lo.y;
+        if (l < (short)0x807f) return 0xffffffffu;                 // below -inf
+        if (h == -32768) return 0;                                 // nothing seen
+        h ^= (h >> 15) & 0x7fff;
+        return key_of(bf16_to_f32((unsigned short)h));
+    }
+};
+template <> struct BestOf<F32> {
+    int hi = (int)0x80000000, lo = 0x7fffffff;
+    __device__ __forceinline__ void word(unsigned w) {
+        const int v = (int)w ^ (((int)w >> 31) & 0x7fffffff);
+        hi = max(hi, v); lo = min(lo, v);
+    }
+    __device__ __forceinline__ unsigned key() const {
+        if (lo < (int)0x807fffff) return 0xffffffffu;
+        if (hi == (int)0x80000000) return 0;
+        return key_of(__uint_as_float((unsigned)(hi ^ ((hi >> 31) & 0x7fffffff))));
+    }
+};
+template <class TR>
+__device__ __forceinline__ void best_vec(BestOf<TR>& b, const uint4& v) { b.word(v.x); b.word(v.y); b.word(v.z); b.word(v.w); }
+
+// the largest number that k of N * 64 keys reach, by one wave (0: fewer than k are there)
+template <class TR, int N>
+__device__ __forceinline__ unsigned reach(const unsigned* top, int k) {
+    unsigned key[N], t = 0;
+#pragma unroll
+    for (int w = 0; w < N; ++w) key[w] = top[w * 64 + (threadIdx.x & 63)];
+#pragma unroll 1
+    for (int bit = 31; bit >= 32 - 8 * TR::ESZ; --bit) {           // the lower half of a bf16 key follows from its sign
+        const unsigned want = t | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int w = 0; w < N; ++w) n += __popcll(__ballot(key[w] >= want));
+        if (n >= k) t = want;
+    }
+    return t;
+}
+
+// f(key, class) for the classes of a row, T threads side by side
+template <class TR, int T, class F>
 __device__ __forceinline__ void each(const char* x, int v, F f) {
     const int nv = v / TR::VEC;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += TPB) {
-        float u[TR::VEC];
-        unpack_vec<TR>(ld_any<TR>(x + (int64_t)i * 16), u);
+    for (int i = threadIdx.x; i < nv; i += T) {
+        float y[TR::VEC];
+        unpack_vec<TR>(ld_any<TR>(x + (int64_t)i * 16), y);
 #pragma unroll
-        for (int j = 0; j < TR::VEC; ++j) f(key_of(u[j]), i * TR::VEC + j);
+        for (int j = 0; j < TR::VEC; ++j) f(key_of(y[j]), i * TR::VEC + j);
     }
-    for (int i = nv * TR::VEC + threadIdx.x; i < v; i += TPB) f(key_of(ld_one<TR>(x, i)), i);
+    for (int i = nv * TR::VEC + threadIdx.x; i < v; i += T) f(key_of(ld_one<TR>(x, i)), i);
 }
 
-// number of classes of the row with a full key >= lo, in every thread
-template <class TR>
-__device__ int count_from(const char* x, int v, u64 lo, int* sm) {
-    int n = 0;
-    each<TR>(x, v, [&](unsigned key, int i) { n += full_key(key, i) >= lo ? 1 : 0; });
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+template <int T>
+__device__ __forceinline__ int block_count(int c, int* sm) {
+    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = n;
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = c;
     __syncthreads();
-    n = 0;
-#pragma unroll
-    for (int w = 0; w < TPB / 64; ++w) n += sm[w];
-    return n;
+    c = 0;
+    for (int w = 0; w < T / 64; ++w) c += sm[w];
+    return c;
 }
 
-template <class TR>
-__global__ __launch_bounds__(TPB) void top_long(TopParams p) {
+// Exactly the k classes of a row with more than CAP classes at or above key t: the k-th largest key by halving, the classes above
+// it in any order, and as many at it as are missing, by ascending class, T classes at a time until there are enough.
+template <class TR, int T>
+__device__ __noinline__ void gather_ties(const char* x, int v, int k, unsigned t, u64* cand, int* count, int* sm) {
+    unsigned hi = 0xffffffffu;                                     // k classes reach t
+    bool first = true;                                             // with many equal values t mostly is the key already
+    while (t < hi) {
+        const unsigned mid = first ? t + 1 : t + (hi - t) / 2 + ((hi - t) & 1);
+        first = false;
+        int c = 0;
+        each<TR, T>(x, v, [&](unsigned key, int) { c += key >= mid ? 1 : 0; });
+        if (block_count<T>(c, sm) >= k) t = mid;
+        else hi = mid - 1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) *count = 0;
+    __syncthreads();
+    each<TR, T>(x, v, [&](unsigned key, int i) { if (key > t) cand[atomicAdd(count, 1)] = full_key(key, i); });
+    __syncthreads();
+    int n = *count;                                                // fewer than k
+    for (int i0 = 0; n < k && i0 < v; i0 += T) {
+        const int i = i0 + threadIdx.x;
+        const bool f = i < v && key_of(ld_one<TR>(x, i)) == t;
+        const u64 ball = __ballot(f);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = __popcll(ball);
+        __syncthreads();
+        int at = n + __popcll(ball & ((1ull << (threadIdx.x & 63)) - 1));
+        for (int w = 0; w < T / 64; ++w) {
+            if (w < (int)threadIdx.x >> 6) at += sm[w];
+            n += sm[w];
+        }
+        if (f && at < k) cand[at] = full_key(t, i);
+    }
+    __syncthreads();
+}
+
+template <class TR, int T>
+__global__ __launch_bounds__(T) void top_long(TopParams p) {
     __shared__ u64 cand[CAP];
-    __shared__ unsigned top[TPB];
-    __shared__ unsigned thr_s;
-    __shared__ int count_s, sm[TPB / 64];
+    __shared__ unsigned top[T], thr_s;
+    __shared__ unsigned short hot[T];
+    __shared__ int count_s, hot_s, sm[T / 64];
+    const int tid = threadIdx.x, nv = p.v / TR::VEC, per = (nv + T - 1) / T, et = nv * TR::VEC + tid;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const char* x = p.x + r * p.xp;
-        u64 lo = 0;
-        if (p.v > CAP) {
-            unsigned best = 0;
-            each<TR>(x, p.v, [&](unsigned key, int) { best = key > best ? key : best; });
-            top[threadIdx.x] = best;
-            __syncthreads();
-            if (threadIdx.x < 64) {
-                // the k-th largest of the maxima, bit by bit: the largest number that k of them reach
-                unsigned t = 0;
-                for (int bit = 31; bit >= 0; --bit) {
-                    const unsigned want = t | (1u << bit);
-                    int n = 0;
+        constexpr int UN = 8;                                      // vectors in flight per thread
+        BestOf<TR> b;
+        int i = tid;
+        for (; i + (UN - 1) * T < nv; i += UN * T) {
+            uint4 raw[UN];
 #pragma unroll
-                    for (int w = 0; w < TPB / 64; ++w) n += __popcll(__ballot(top[w * 64 + threadIdx.x] >= want));
-                    if (n >= p.k) t = want;
-                }
-                if (threadIdx.x == 0) thr_s = t;
-            }
-            __syncthreads();
-            lo = (u64)thr_s << 32;
+            for (int u = 0; u < UN; ++u) raw[u] = ld_any<TR>(x + (int64_t)(i + u * T) * 16);
+#pragma unroll
+            for (int u = 0; u < UN; ++u) best_vec(b, raw[u]);
         }
-        int n = 0;
-        for (int tries = 0;; ++tries) {
-            if (threadIdx.x == 0) count_s = 0;
-            __syncthreads();
-            each<TR>(x, p.v, [&](unsigned key, int i) {
-                const u64 f = full_key(key, i);
-                if (f >= lo) {
-                    const int at = atomicAdd(&count_s, 1);
-                    if (at < CAP) cand[at] = f;
-                }
-            });
-            __syncthreads();
-            n = count_s;
-            if (n <= CAP || tries) break;                          // the second time exactly k are gathered
-            u64 hi = ~0ull;                                        // count(lo) > CAP >= k; full keys differ
-            while (lo < hi) {                                      // the largest full key that k classes reach
-                const u64 mid = lo + (hi - lo) / 2 + ((hi - lo) & 1);
-                if (count_from<TR>(x, p.v, mid, sm) >= p.k) lo = mid;
-                else hi = mid - 1;
-            }
-            __syncthreads();
+        for (; i < nv; i += T) best_vec(b, ld_any<TR>(x + (int64_t)i * 16));
+        const unsigned tail = et < p.v ? key_of(ld_one<TR>(x, et)) : 0u;      // fewer than a vector's worth
+        const unsigned best = max(b.key(), tail);
+        // G maxima of T / G neighbouring threads each
+        unsigned group = best;
+        for (int o = T / p.G >> 1; o > 0; o >>= 1) group = max(group, __shfl_xor(group, o, 64));
+        if (tid % (T / p.G) == 0) top[tid / (T / p.G)] = group;
+        if (tid == 0) count_s = hot_s = 0;
+        __syncthreads();
+        if (tid < 64) {
+            const unsigned t = p.G == 64 ? reach<TR, 1>(top, p.k) : p.G == 128 ? reach<TR, 2>(top, p.k) : p.G == 256 ? reach<TR, 4>(top, p.k) : reach<TR, 8>(top, p.k);
+            if (tid == 0) thr_s = t;
         }
-        n = n < CAP ? n : CAP;
-        for (int a = threadIdx.x; a < n; a += TPB) {
+        __syncthreads();
+        const unsigned t = thr_s;
+        auto add = [&](unsigned key, int cls) {
+            if (key >= t) {
+                const int at = atomicAdd(&count_s, 1);
+                if (at < CAP) cand[at] = full_key(key, cls);
+            }
+        };
+        if (best >= t && best) hot[atomicAdd(&hot_s, 1)] = (unsigned short)tid;
+        if (tail) add(tail, et);
+        __syncthreads();
+        const int items = hot_s * per;
+        for (int m = tid; m < items; m += T) {
+            const int at = (m % per) * T + hot[m / per];
+            if (at < nv) {
+                float y[TR::VEC];
+                unpack_vec<TR>(ld_any<TR>(x + (int64_t)at * 16), y);
+#pragma unroll
+                for (int j = 0; j < TR::VEC; ++j) add(key_of(y[j]), at * TR::VEC + j);
+            }
+        }
+        __syncthreads();
+        int n = count_s;
+        if (n > CAP) {
+            gather_ties<TR, T>(x, p.v, p.k, t, cand, &count_s, sm);
+            n = p.k;
+        }
+        for (int a = tid; a < n; a += T) {
             const u64 f = cand[a];
             int place = 0;
-            for (int b = 0; b < n; ++b) place += cand[b] > f ? 1 : 0;
+            for (int c = 0; c < n; ++c) place += cand[c] > f ? 1 : 0;
             if (place < p.k) emit<TR>(p, r, place, (int)~(unsigned)f);
         }
         __syncthreads();
     }
 }
 
-struct Plan { bool is_long; int L, nv, blocks; };
-// Taking the largest out costs about 3 operations per held class and 10 per lane exchange for every entry of the list:
-// lists of up to 16 entries of rows that 64 lanes hold; everything else is a workgroup's.
+enum { SHORT, WAVE, LONG };
+struct Plan { int kind, L, nv, T, G, blocks; };
 Plan plan_of(int esz, int64_t rows, int v, int k) {
-    Plan q;
+    Plan q = {SHORT, 1, 1, TPB, 0, 0};
     const int vec = 16 / esz, nvec = (v + vec - 1) / vec;
-    q.is_long = nvec > 64 * NVMAX || k > 16;
-    q.L = 1;
-    while (q.L < 64 && nvec > q.L * NVMAX) q.L *= 2;
-    q.nv = 1;
-    while (q.nv < NVMAX && q.nv * q.L < nvec) q.nv *= 2;
-    const int64_t per = q.is_long ? 1 : TPB / q.L, b = (rows + per - 1) / per;
+    int64_t per = 1;
+    if (nvec <= 64 * NVMAX) {
+        while (q.L < 64 && nvec > q.L * NVMAX) q.L *= 2;
+        // instructions of a wave per row: k times 3 per held class and 10 per exchange between lanes, for 64 / L rows at once,
+        // against 3 per held class and bit, and the placing
+        const int e1 = (nvec + q.L - 1) / q.L * vec, e2 = (nvec + 63) / 64 * vec;
+        int lg = 0;
+        while ((1 << lg) < q.L) ++lg;
+        const int64_t take = (int64_t)k * (3 * e1 + 10 * lg + 8) * q.L / 64, search = 8 * esz * 3 * e2 + 100 + (int64_t)k * ((k + 63) / 64) * 4;
+        q.kind = take <= search ? SHORT : WAVE;
+        if (q.kind == WAVE) q.L = 64;
+        while (q.nv < NVMAX && q.nv * q.L < nvec) q.nv *= 2;
+        per = TPB / q.L;
+    } else {
+        // few rows, or lists longer than 128 (whose G needs them): 1024 threads.  G maxima, at least 1.5 per entry: the classes
+        // gathered are then few (G log(G / (G - k)) of them on average: 44 for k = 32, 355 for k = 256)
+        q.kind = LONG;
+        q.T = rows >= TROWS && k <= 128 ? 256 : 1024;
+        q.G = 64;
+        while (q.G < q.T && q.G < k + k / 2) q.G *= 2;
+    }
+    const int64_t b = (rows + per - 1) / per;
     q.blocks = (int)(b < 16384 ? b : 16384);
     return q;
 }
 
-#define SHORT_LAUNCH(KERN)                                                                     \
+#define NV_LAUNCH(KERN)                                                                        \
     do {                                                                                       \
         if (dtype == 1) {                                                                      \
             if (q.nv == 1) KERN<BF16, 1><<<q.blocks, TPB, 0, st>>>(p);                         \
@@ -210,7 +403,6 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
             else KERN<F32, 4><<<q.blocks, TPB, 0, st>>>(p);                                    \
         }                                                                                      \
     } while (0)
-
 }  // namespace
 
 extern "C" int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, void* values, int32_t* index,
@@ -226,13 +418,18 @@ extern "C" int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, cons
     const Plan q = plan_of((int)esz, rows, v, k);
     TopParams p;
     p.x = (const char*)logits; p.val = (char*)values; p.idx = index;
-    p.rows = rows; p.xp = pitch * (int64_t)esz; p.v = v; p.k = k; p.L = q.L;
+    p.rows = rows; p.xp = pitch * (int64_t)esz; p.v = v; p.k = k; p.L = q.L; p.G = q.G;
     hipStream_t st = (hipStream_t)stream;
-    if (q.is_long) {
-        if (dtype == 1) top_long<BF16><<<q.blocks, TPB, 0, st>>>(p);
-        else top_long<F32><<<q.blocks, TPB, 0, st>>>(p);
+    if (q.kind == SHORT) {
+        NV_LAUNCH(top_short);
+    } else if (q.kind == WAVE) {
+        NV_LAUNCH(top_wave);
+    } else if (q.T == 256) {
+        if (dtype == 1) top_long<BF16, 256><<<q.blocks, 256, 0, st>>>(p);
+        else top_long<F32, 256><<<q.blocks, 256, 0, st>>>(p);
     } else {
-        SHORT_LAUNCH(top_short);
+        if (dtype == 1) top_long<BF16, 1024><<<q.blocks, 1024, 0, st>>>(p);
+        else top_long<F32, 1024><<<q.blocks, 1024, 0, st>>>(p);
     }
     MI_HIP(hipGetLastError());
     return 0;
