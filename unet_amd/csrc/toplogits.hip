@@ -22,17 +22,13 @@ namespace {
 constexpr int TPB = 256;
 constexpr int MAX_K = 256;
 constexpr int NVMAX = 4;
-#ifndef TROWS
-#define TROWS 512
-#endif
-constexpr int CAP = 2048;             // gathered classes of a long row
 
 struct TopParams {
     const char* x;
     char* val;
     int* idx;
     int64_t rows, xp;
-    int v, k, L, G;
+    int v, k, L, G, by_lanes;
 };
 
 __device__ __forceinline__ unsigned key_of(float f) {
@@ -70,35 +66,73 @@ __device__ __forceinline__ void load_keys(const char* x, int v, int L, int l, un
     }
 }
 
+// The classes found go through LDS (dynamic, [workgroup's rows][k]): the results of a wave's rows are one piece of the output and
+// leave it with neighbouring lanes at neighbouring addresses.
+// bf16: key and class fit one word, (key, 65535 - class), so that a maximum is one instruction.
 template <class TR, int NV>
 __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
-    const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L;
+    extern __shared__ unsigned short found[];
+    const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    unsigned short* mine = found + (threadIdx.x / L) * p.k;
+    const unsigned short* waves = found + wave * (64 / L) * p.k;
     for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += (int64_t)gridDim.x * per) {
         const int64_t r = r0 + threadIdx.x / L;
-        const bool in = r < p.rows;
-        const char* x = p.x + (in ? r : 0) * p.xp;
+        const char* x = p.x + (r < p.rows ? r : 0) * p.xp;
         unsigned key[NV][TR::VEC];
         load_keys<TR, NV>(x, p.v, L, l, key);
-        for (int n = 0; n < p.k; ++n) {
-            unsigned best = 0;
-            int at = 0x7fffffff;
-#pragma unroll
-            for (int i = 0; i < NV; ++i)                           // ascending classes: the first of equal keys wins
-#pragma unroll
-                for (int j = 0; j < TR::VEC; ++j)
-                    if (key[i][j] > best) { best = key[i][j]; at = (i * L + l) * TR::VEC + j; }
-            for (int o = L >> 1; o > 0; o >>= 1) {
-                const unsigned ob = __shfl_xor(best, o, 64);
-                const int oa = __shfl_xor(at, o, 64);
-                if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-            }
+        if constexpr (TR::ESZ == 2) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < TR::VEC; ++j)
-                    if ((i * L + l) * TR::VEC + j == at) key[i][j] = 0u;
-            if (in && l == (n & (L - 1))) emit<TR>(p, r, n, at);
+                for (int j = 0; j < TR::VEC; ++j) {
+                    const unsigned cls = 0xffffu - (unsigned)((i * L + l) * TR::VEC + j);
+                    key[i][j] = key[i][j] ? (key[i][j] & 0xffff0000u) | cls : 0u;
+                }
+            for (int n = 0; n < p.k; ++n) {
+                unsigned best = 0;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < TR::VEC; ++j) best = max(best, key[i][j]);
+                for (int o = L >> 1; o > 0; o >>= 1) best = max(best, __shfl_xor(best, o, 64));
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < TR::VEC; ++j) key[i][j] = key[i][j] == best ? 0u : key[i][j];
+                if (l == 0) mine[n] = (unsigned short)(0xffffu - (best & 0xffffu));
+            }
+        } else {
+            for (int n = 0; n < p.k; ++n) {
+                unsigned best = 0;
+                int at = 0x7fffffff;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)                       // ascending classes: the first of equal keys wins
+#pragma unroll
+                    for (int j = 0; j < TR::VEC; ++j)
+                        if (key[i][j] > best) { best = key[i][j]; at = (i * L + l) * TR::VEC + j; }
+                for (int o = L >> 1; o > 0; o >>= 1) {
+                    const unsigned ob = __shfl_xor(best, o, 64);
+                    const int oa = __shfl_xor(at, o, 64);
+                    if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
+                }
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < TR::VEC; ++j)
+                        if ((i * L + l) * TR::VEC + j == at) key[i][j] = 0u;
+                if (l == 0) mine[n] = (unsigned short)at;
+            }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        const int64_t w0 = r0 + wave * (64 / L);                   // first row of the wave
+        const int outs = (int)max((int64_t)0, min((int64_t)(64 / L), p.rows - w0)) * p.k;
+        for (int o = lane; o < outs; o += 64) {
+            const int row = o / p.k;
+            emit<TR>(p, w0 + row, o - row * p.k, waves[o]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -114,6 +148,22 @@ __device__ __forceinline__ int lanes_before(int v, int& all) {
     all = __shfl(s, 63, 64);
     return s - v;
 }
+// the k largest of n full keys in LDS to their places, by one wave
+template <class TR>
+__device__ __forceinline__ void place_all(const TopParams& p, int64_t r, int l, const u64* mine, int n) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    for (int a = l; a < n; a += 64) {
+        const u64 f = mine[a];
+        int place = 0;
+#pragma unroll 4
+        for (int b = 0; b < n; ++b) place += mine[b] > f ? 1 : 0;
+        if (place < p.k) emit<TR>(p, r, place, (int)~(unsigned)f);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+}
+
 template <class TR, int NV>
 __global__ __launch_bounds__(TPB) void top_wave(TopParams p) {
     __shared__ u64 list[TPB / 64][MAX_K];
@@ -123,6 +173,35 @@ __global__ __launch_bounds__(TPB) void top_wave(TopParams p) {
         const char* x = p.x + r * p.xp;
         unsigned key[NV][TR::VEC];
         load_keys<TR, NV>(x, p.v, 64, l, key);
+        if (p.by_lanes) {
+            // at least k classes lie at or above the k-th largest of the lanes' maxima: on average 44 for k = 32
+            unsigned best = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < TR::VEC; ++j) best = max(best, key[i][j]);
+            unsigned t = 0;
+#pragma unroll 1
+            for (int bit = 31; bit >= 32 - 8 * TR::ESZ; --bit) {
+                const unsigned want = t | (1u << bit);
+                if (__popcll(__ballot(best >= want)) >= p.k) t = want;
+            }
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < TR::VEC; ++j) {
+                    const bool f = key[i][j] >= t && key[i][j];
+                    const u64 ball = __ballot(f);
+                    const int at = n + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(ball >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)ball, 0));
+                    if (f && at < MAX_K) mine[at] = full_key(key[i][j], (i * 64 + l) * TR::VEC + j);
+                    n += __popcll(ball);
+                }
+            if (n <= MAX_K) {                                      // the same for the whole wave
+                place_all<TR>(p, r, l, mine, n);
+                continue;
+            }
+        }
         unsigned t = 0;                                            // the largest number that k keys reach
 #pragma unroll 1
         for (int bit = 31; bit >= 32 - 8 * TR::ESZ; --bit) {       // the lower half of a bf16 key follows from its sign
@@ -162,16 +241,7 @@ __global__ __launch_bounds__(TPB) void top_wave(TopParams p) {
                 else if (key[i][j] && kk == t) { if (pe < p.k) mine[pe] = full_key(kk, cls); ++pe; }
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-        __builtin_amdgcn_wave_barrier();
-        for (int a = l; a < p.k; a += 64) {
-            const u64 f = mine[a];
-            int place = 0;
-            for (int b = 0; b < p.k; ++b) place += mine[b] > f ? 1 : 0;
-            emit<TR>(p, r, place, (int)~(unsigned)f);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-        __builtin_amdgcn_wave_barrier();
+        place_all<TR>(p, r, l, mine, p.k);
     }
 }
 
@@ -254,7 +324,7 @@ __device__ __forceinline__ int block_count(int c, int* sm) {
     return c;
 }
 
-// Exactly the k classes of a row with more than CAP classes at or above key t: the k-th largest key by halving, the classes above
+// Exactly the k classes of a row with too many classes at or above key t: the k-th largest key by halving, the classes above
 // it in any order, and as many at it as are missing, by ascending class, T classes at a time until there are enough.
 template <class TR, int T>
 __device__ __noinline__ void gather_ties(const char* x, int v, int k, unsigned t, u64* cand, int* count, int* sm) {
@@ -293,6 +363,7 @@ __device__ __noinline__ void gather_ties(const char* x, int v, int k, unsigned t
 
 template <class TR, int T>
 __global__ __launch_bounds__(T) void top_long(TopParams p) {
+    constexpr int CAP = T <= 512 ? 4 * T : 2048;                   // classes gathered, 12 times the usual number
     __shared__ u64 cand[CAP];
     __shared__ unsigned top[T], thr_s;
     __shared__ unsigned short hot[T];
@@ -361,28 +432,34 @@ __global__ __launch_bounds__(T) void top_long(TopParams p) {
 }
 
 enum { SHORT, WAVE, LONG };
-struct Plan { int kind, L, nv, T, G, blocks; };
+struct Plan { int kind, L, nv, T, G, blocks, by_lanes; };
 Plan plan_of(int esz, int64_t rows, int v, int k) {
-    Plan q = {SHORT, 1, 1, TPB, 0, 0};
+    Plan q = {SHORT, 1, 1, TPB, 0, 0, 0};
     const int vec = 16 / esz, nvec = (v + vec - 1) / vec;
     int64_t per = 1;
     if (nvec <= 64 * NVMAX) {
         while (q.L < 64 && nvec > q.L * NVMAX) q.L *= 2;
-        // instructions of a wave per row: k times 3 per held class and 10 per exchange between lanes, for 64 / L rows at once,
-        // against 3 per held class and bit, and the placing
-        const int e1 = (nvec + q.L - 1) / q.L * vec, e2 = (nvec + 63) / 64 * vec;
+        // instructions of a wave per row: k times 3 (bf16) or 6 (fp32) per held class and 10 per exchange between lanes, for
+        // 64 / L rows at once, against 4 per bit and 12 per held class (k <= 32, by the lanes' maxima) or 3 per held class and bit, and the placing.
+        // 50000 rows of 512 bf16 classes, 16 of them: 50 us by search alone, 29 with the lanes' maxima; 100000 x 133 fp32, 5: 38 taken out
+        int n1 = 1, n2 = 1;
+        while (n1 * q.L < nvec) n1 *= 2;
+        while (n2 * 64 < nvec) n2 *= 2;
+        const int e1 = n1 * vec, e2 = n2 * vec;
         int lg = 0;
         while ((1 << lg) < q.L) ++lg;
-        const int64_t take = (int64_t)k * (3 * e1 + 10 * lg + 8) * q.L / 64, search = 8 * esz * 3 * e2 + 100 + (int64_t)k * ((k + 63) / 64) * 4;
-        q.kind = take <= search ? SHORT : WAVE;
+        q.by_lanes = k <= 32 && 2 * nvec >= 3 * k;                 // enough lanes hold something
+        const int64_t take = ((int64_t)k * ((esz == 2 ? 3 : 6) * e1 + 10 * lg + 8) + 8 * e1) * q.L / 64, search = q.by_lanes ? 8 * esz * 4 + 12 * e2 + 6 * k + 100 : 8 * esz * 3 * e2 + 100 + (int64_t)k * ((k + 63) / 64) * 4;
+        q.kind = take <= search && k <= 32 ? SHORT : WAVE;             // 32: 16 KB of LDS
         if (q.kind == WAVE) q.L = 64;
         while (q.nv < NVMAX && q.nv * q.L < nvec) q.nv *= 2;
         per = TPB / q.L;
     } else {
-        // few rows, or lists longer than 128 (whose G needs them): 1024 threads.  G maxima, at least 1.5 per entry: the classes
-        // gathered are then few (G log(G / (G - k)) of them on average: 44 for k = 32, 355 for k = 256)
+        // Few rows: 1024 threads each.  Else few enough threads that each has some vectors, as many rows as possible being on their
+        // way: 30000 x 4000 bf16, 8 of them: 128 threads 83 us, 256 98, 512 166; 2048 x 50001, 32: 128 threads 78, 256 64, 512 63.
+        // G maxima, at least 1.5 per entry: the classes gathered are then few (G log(G / (G - k)) of them on average: 44 for k = 32, 355 for 256)
         q.kind = LONG;
-        q.T = rows >= TROWS && k <= 128 ? 256 : 1024;
+        q.T = rows < 512 ? 1024 : nvec <= 1024 && k <= 85 ? 128 : nvec <= 4096 && k <= 170 ? 256 : 512;
         q.G = 64;
         while (q.G < q.T && q.G < k + k / 2) q.G *= 2;
     }
@@ -391,16 +468,16 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
     return q;
 }
 
-#define NV_LAUNCH(KERN)                                                                        \
+#define NV_LAUNCH(KERN, lds)                                                                      \
     do {                                                                                       \
         if (dtype == 1) {                                                                      \
-            if (q.nv == 1) KERN<BF16, 1><<<q.blocks, TPB, 0, st>>>(p);                         \
-            else if (q.nv == 2) KERN<BF16, 2><<<q.blocks, TPB, 0, st>>>(p);                    \
-            else KERN<BF16, 4><<<q.blocks, TPB, 0, st>>>(p);                                   \
+            if (q.nv == 1) KERN<BF16, 1><<<q.blocks, TPB, lds, st>>>(p);                         \
+            else if (q.nv == 2) KERN<BF16, 2><<<q.blocks, TPB, lds, st>>>(p);                    \
+            else KERN<BF16, 4><<<q.blocks, TPB, lds, st>>>(p);                                   \
         } else {                                                                               \
-            if (q.nv == 1) KERN<F32, 1><<<q.blocks, TPB, 0, st>>>(p);                          \
-            else if (q.nv == 2) KERN<F32, 2><<<q.blocks, TPB, 0, st>>>(p);                     \
-            else KERN<F32, 4><<<q.blocks, TPB, 0, st>>>(p);                                    \
+            if (q.nv == 1) KERN<F32, 1><<<q.blocks, TPB, lds, st>>>(p);                          \
+            else if (q.nv == 2) KERN<F32, 2><<<q.blocks, TPB, lds, st>>>(p);                     \
+            else KERN<F32, 4><<<q.blocks, TPB, lds, st>>>(p);                                    \
         }                                                                                      \
     } while (0)
 }  // namespace
@@ -418,15 +495,21 @@ extern "C" int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, cons
     const Plan q = plan_of((int)esz, rows, v, k);
     TopParams p;
     p.x = (const char*)logits; p.val = (char*)values; p.idx = index;
-    p.rows = rows; p.xp = pitch * (int64_t)esz; p.v = v; p.k = k; p.L = q.L; p.G = q.G;
+    p.rows = rows; p.xp = pitch * (int64_t)esz; p.v = v; p.k = k; p.L = q.L; p.G = q.G; p.by_lanes = q.by_lanes;
     hipStream_t st = (hipStream_t)stream;
     if (q.kind == SHORT) {
-        NV_LAUNCH(top_short);
+        NV_LAUNCH(top_short, TPB / q.L * k * 2);
     } else if (q.kind == WAVE) {
-        NV_LAUNCH(top_wave);
+        NV_LAUNCH(top_wave, 0);
+    } else if (q.T == 128) {
+        if (dtype == 1) top_long<BF16, 128><<<q.blocks, 128, 0, st>>>(p);
+        else top_long<F32, 128><<<q.blocks, 128, 0, st>>>(p);
     } else if (q.T == 256) {
         if (dtype == 1) top_long<BF16, 256><<<q.blocks, 256, 0, st>>>(p);
         else top_long<F32, 256><<<q.blocks, 256, 0, st>>>(p);
+    } else if (q.T == 512) {
+        if (dtype == 1) top_long<BF16, 512><<<q.blocks, 512, 0, st>>>(p);
+        else top_long<F32, 512><<<q.blocks, 512, 0, st>>>(p);
     } else {
         if (dtype == 1) top_long<BF16, 1024><<<q.blocks, 1024, 0, st>>>(p);
         else top_long<F32, 1024><<<q.blocks, 1024, 0, st>>>(p);
