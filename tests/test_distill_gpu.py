@@ -183,7 +183,8 @@ def lists(rows, v, k, g, dev, t_dtype=torch.float32, i_dtype=torch.int32, ragged
 
 LOSS = [(1, 1, 1), (5, 2, 1), (64, 3, 3), (300, 16, 4), (257, 21, 5), (70, 16, 256), (700, 64, 16), (1000, 133, 8), (33, 512, 64), (17, 1024, 33),
         (17, 2048, 256), (9, 2049, 7), (9, 1023, 256), (5000, 7, 2), (3, 50001, 32), (1, 32001, 64), (4100, 2050, 3), (7, 8200, 12), (5, 16390, 9), (3, 33000, 4),
-        (2, 70000, 8), (2, 131072, 5), (2, 131080, 5)]
+        (2, 70000, 8), (2, 131072, 5), (2, 131080, 5),
+        (520, 9000, 4), (513, 34000, 3), (600, 29, 12), (2, 5, 1), (2050, 16, 1), (90, 2043, 2), (300, 1021, 17)]
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])

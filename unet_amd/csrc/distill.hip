@@ -22,7 +22,6 @@
 namespace {
 
 constexpr int TPB = 256;
-constexpr int STEP_WGS = 1024;        // workgroups of the step kernel (its rows are prefetched from one to the next)
 constexpr int MAX_K = 256;
 constexpr int NVMAX = 4;              // 16-byte vectors of a row that a lane holds
 constexpr float LOG2E = 1.4426950408889634f;
@@ -85,21 +84,41 @@ struct ListSum {
     }
 };
 
-// one row in the registers of L lanes: vector i of lane l is vector i * L + l of the row; classes behind the end are -inf
+// One row in the registers of L lanes: vector i of lane l is vector i * L + l of the row; classes behind the end are -inf.
+// `fetch` only requests it (a row's last, partial vector as the 16 bytes that end with the row), `take` makes floats of it.
 template <class TR, int NV>
 struct Row {
     float x[NV][TR::VEC];
-    __device__ __forceinline__ void load(const char* z, int v, int L, int l) {
+    static __device__ __forceinline__ void fetch(uint4 (&raw)[NV], const char* z, int v, int L, int l) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int e0 = (i * L + l) * TR::VEC;
-            if (e0 + TR::VEC <= v) {
-                unpack_vec<TR>(ld_any<TR>(z + (int64_t)e0 * TR::ESZ), x[i]);
-            } else {
+            if (e0 < v && v >= TR::VEC) raw[i] = ld_any<TR>(z + (int64_t)min(e0, v - TR::VEC) * TR::ESZ);
+        }
+    }
+    __device__ __forceinline__ void take(const uint4 (&raw)[NV], const char* z, int v, int L, int l) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e0 = (i * L + l) * TR::VEC;
+            if (v < TR::VEC) {
 #pragma unroll
                 for (int j = 0; j < TR::VEC; ++j) x[i][j] = e0 + j < v ? ld_one<TR>(z, e0 + j) : -INFINITY;
+                continue;
             }
+            uint4 w = raw[i];
+            if (v % TR::VEC) {                                    // the same for all lanes
+                const int over = e0 + TR::VEC - v;                // > 0: the partial vector, its first class lies `over` up
+                if (over > 0) w = down<TR>(w, over);
+            }
+            unpack_vec<TR>(w, x[i]);
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) x[i][j] = e0 + j < v ? x[i][j] : -INFINITY;
         }
+    }
+    __device__ __forceinline__ void load(const char* z, int v, int L, int l) {
+        uint4 raw[NV];
+        fetch(raw, z, v, L, l);
+        take(raw, z, v, L, l);
     }
     __device__ __forceinline__ float max_of(int L) const {
         float m = -INFINITY;
@@ -144,23 +163,67 @@ __device__ __forceinline__ void block_part(const DistParams& p, double loss, dou
 }
 
 // ---- short rows -----------------------------------------------------------------------------------------------------
-template <class TR, int NV>
+// SL slots of a row's list in the registers of a lane: slot j of the list is slot j / L of lane j % L.  `fetch` only requests them.
+template <int SL>
+struct Slots {
+    unsigned lo[SL], hi[SL], t[SL];
+    __device__ __forceinline__ void fetch(const DistParams& p, int64_t r, bool in, int L, int l) {
+#pragma unroll
+        for (int n = 0; n < SL; ++n) {
+            const int j = n * L + l;
+            lo[n] = hi[n] = 0xffffffffu;
+            t[n] = 0u;
+            if (in && j < p.k) {
+                const int64_t at = r * p.k + j;
+                if (p.i64) {
+                    const uint2 u = reinterpret_cast<const uint2*>(p.idx)[at];
+                    lo[n] = u.x; hi[n] = u.y;
+                } else {
+                    lo[n] = reinterpret_cast<const unsigned*>(p.idx)[at];
+                    hi[n] = 0u;
+                }
+                if (p.t_bf16) t[n] = reinterpret_cast<const unsigned short*>(p.t)[at];
+                else t[n] = reinterpret_cast<const unsigned*>(p.t)[at];
+            }
+        }
+    }
+    __device__ __forceinline__ float teacher(const DistParams& p, int n) const { return __uint_as_float(p.t_bf16 ? t[n] << 16 : t[n]); }
+    // class, -1: unused (v is at most 2^28: a negative 32-bit index is too large as well)
+    __device__ __forceinline__ int cls(const DistParams& p, int n) const {
+        return hi[n] == 0u && lo[n] < (unsigned)p.v && teacher(p, n) != -INFINITY ? (int)lo[n] : -1;
+    }
+};
+
+// the logits and the list are requested one row ahead
+template <class TR, int NV, int SL>
 __global__ __launch_bounds__(TPB) void distill_short_fwd(DistParams p) {
     const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L;
     double loss = 0.0, count = 0.0;
-    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += (int64_t)gridDim.x * per) {
-        const int64_t r = r0 + threadIdx.x / L;
+    const int64_t step = (int64_t)gridDim.x * per;
+    int64_t r = (int64_t)blockIdx.x * per + threadIdx.x / L;
+    uint4 raw[NV];
+    Slots<SL> next;
+    auto fetch = [&](int64_t row) {
+        const bool in = row < p.rows;
+        Row<TR, NV>::fetch(raw, p.z + (in ? row : 0) * p.zp, p.v, L, l);
+        next.fetch(p, row, in, L, l);
+    };
+    fetch(r);
+    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += step, r += step) {
         const bool in = r < p.rows;
         const char* z = p.z + (in ? r : 0) * p.zp;
         Row<TR, NV> x;
-        x.load(z, p.v, L, l);
+        x.take(raw, z, p.v, L, l);
+        const Slots<SL> now = next;
+        float zi[SL];
+#pragma unroll
+        for (int n = 0; n < SL; ++n) zi[n] = now.cls(p, n) >= 0 ? ld_one<TR>(z, now.cls(p, n)) : 0.0f;
+        if (r0 + step < p.rows) fetch(r + step);
         const float m = x.max_of(L), s = x.exp_of(m, p.c, L);
         ListSum q;
-        if (in)
-            for (int j = l; j < p.k; j += L) {
-                const int i = list_i(p, r * p.k + j);
-                if (i >= 0) q.add(list_t(p, r * p.k + j), (ld_one<TR>(z, i) - m) * p.inv_t, p.inv_t);
-            }
+#pragma unroll
+        for (int n = 0; n < SL; ++n)
+            if (now.cls(p, n) >= 0) q.add(now.teacher(p, n), (zi[n] - m) * p.inv_t, p.inv_t);
         q.join(L, p.inv_t);
         if (l == 0 && in) {
             const float row = q.some ? q.loss(s, p.wl) : 0.0f;
@@ -171,8 +234,7 @@ __global__ __launch_bounds__(TPB) void distill_short_fwd(DistParams p) {
     if (p.red) block_part<TPB>(p, loss, count);
 }
 
-// weights of a row's list into LDS (L lanes, k slots): qi class or -1, qw weight summed over the slots of the same class,
-// in the order of the list, qt teacher logit (may be qw).  Returns whether a slot is used.
+// weights of a row's list into LDS (L lanes, k slots): qi class or -1, qw weight, qt teacher logit (may be qw).  Returns whether a slot is used.
 __device__ __forceinline__ bool list_weights(const DistParams& p, int64_t r, bool in, int L, int l, int* qi, float* qw, float* qt) {
     float m = -INFINITY;
     bool some = false;
@@ -214,43 +276,128 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
+template <class TR, int NV, class F>
+__device__ __forceinline__ void store_row(char* dz, int v, int L, int l, F f) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e0 = (i * L + l) * TR::VEC;
+        float __attribute__((aligned(16))) d[TR::VEC];
+        f(i, e0, d);
+        if (e0 + TR::VEC <= v) {
+            st_any(dz + (int64_t)e0 * TR::ESZ, pack_vec<TR>(d));
+        } else {
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j)
+                if (e0 + j < v) st_one<TR>(dz, e0 + j, d[j]);
+        }
+    }
+}
+
+// the list in registers; every slot's weight is taken off the class it names by comparing, in the order of the list
+template <class TR, int NV, int SL>
+__global__ __launch_bounds__(TPB) void distill_short_bwd_reg(DistParams p) {
+    const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L, first = (threadIdx.x & 63) - l;
+    const int64_t step = (int64_t)gridDim.x * per;
+    int64_t r = (int64_t)blockIdx.x * per + threadIdx.x / L;
+    uint4 raw[NV];
+    Slots<SL> next;
+    auto fetch = [&](int64_t row) {
+        const bool in = row < p.rows;
+        Row<TR, NV>::fetch(raw, p.z + (in ? row : 0) * p.zp, p.v, L, l);
+        next.fetch(p, row, in, L, l);
+    };
+    fetch(r);
+    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += step, r += step) {
+        const bool in = r < p.rows;
+        Row<TR, NV> x;
+        x.take(raw, p.z + (in ? r : 0) * p.zp, p.v, L, l);
+        const Slots<SL> now = next;
+        if (r0 + step < p.rows) fetch(r + step);
+        const float m = x.max_of(L), s = x.exp_of(m, p.c, L);
+        float tm = -INFINITY, q[SL], total = 0.0f;
+        int cls[SL];
+        bool some = false;
+#pragma unroll
+        for (int n = 0; n < SL; ++n) {
+            cls[n] = now.cls(p, n);
+            if (cls[n] >= 0) { tm = fmaxf(tm, now.teacher(p, n)); some = true; }
+        }
+        tm = lanes_max(tm, L);
+        some = (bool)lanes_max(some ? 1.0f : 0.0f, L);
+#pragma unroll
+        for (int n = 0; n < SL; ++n) {
+            q[n] = cls[n] >= 0 ? __builtin_amdgcn_exp2f((now.teacher(p, n) - tm) * p.c) : 0.0f;
+            total += q[n];
+        }
+        total = lanes_sum(total, L);
+        const float g = in ? grad_scale(p, r) : 0.0f, inv = 1.0f / s, qs = 1.0f / total;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) x.x[i][j] *= inv;
+#pragma unroll
+        for (int n = 0; n < SL; ++n) {
+            const float w = q[n] * qs;
+            for (int o = 0; o < L && n * L + o < p.k; ++o) {       // the same for all lanes
+                const int c = L == 1 ? cls[n] : __shfl(cls[n], first + o, 64);
+                const float wo = L == 1 ? w : __shfl(w, first + o, 64);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < TR::VEC; ++j) x.x[i][j] -= c == (i * L + l) * TR::VEC + j ? wo : 0.0f;
+            }
+        }
+        if (in)
+            store_row<TR, NV>(p.dz + r * p.dzp, p.v, L, l, [&](int i, int, float* d) {
+#pragma unroll
+                for (int j = 0; j < TR::VEC; ++j) d[j] = some ? g * x.x[i][j] : 0.0f;
+            });
+    }
+}
+
+// floats of LDS per row of the kernel below: class weights (whole vectors), classes and weights of the slots; 16-byte rows
+__host__ __device__ __forceinline__ int lds_row(int vec, int v, int k) { return (v + vec - 1) / vec * vec + (2 * k + 3) / 4 * 4; }
+
+// any list: the slots' weights are put down at their classes in LDS
 template <class TR, int NV>
 __global__ __launch_bounds__(TPB) void distill_short_bwd(DistParams p) {
-    extern __shared__ float lds[];                                // per row: qi [k], qw [k], acc [v]
-    const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L, slot = threadIdx.x / L;
-    int* qi = reinterpret_cast<int*>(lds) + (int64_t)slot * (2 * p.k + p.v);
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L, slot = threadIdx.x / L, va = (p.v + TR::VEC - 1) / TR::VEC * TR::VEC;
+    float* acc = lds + slot * lds_row(TR::VEC, p.v, p.k);
+    int* qi = reinterpret_cast<int*>(acc + va);
     float* qw = reinterpret_cast<float*>(qi) + p.k;
-    float* acc = qw + p.k;
     for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += (int64_t)gridDim.x * per) {
         const int64_t r = r0 + slot;
         const bool in = r < p.rows;
-        Row<TR, NV> x;
-        x.load(p.z + (in ? r : 0) * p.zp, p.v, L, l);
-        const float m = x.max_of(L), s = x.exp_of(m, p.c, L);
-        for (int i = l; i < p.v; i += L) acc[i] = 0.0f;
+        uint4 raw[NV];
+        const char* z = p.z + (in ? r : 0) * p.zp;
+        Row<TR, NV>::fetch(raw, z, p.v, L, l);
+        for (int i = 4 * l; i < va; i += 4 * L) *reinterpret_cast<float4*>(acc + i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         const bool some = list_weights(p, r, in, L, l, qi, qw, qw);
         wave_sync();
+        bool twice = false;                                       // a class that already has a weight
         if (in && some)
             for (int j = l; j < p.k; j += L)
+                if (qi[j] >= 0) twice |= atomicExch(acc + qi[j], qw[j]) != 0.0f;
+        if (lanes_max(twice ? 1.0f : 0.0f, L) != 0.0f) {
+            wave_sync();
+            for (int j = l; j < p.k; j += L)
                 if (qi[j] >= 0) acc[qi[j]] = weight_of(qi, qw, p.k, qi[j]);
+        }
+        Row<TR, NV> x;
+        x.take(raw, z, p.v, L, l);
+        const float m = x.max_of(L), s = x.exp_of(m, p.c, L);
         wave_sync();
         if (in) {
             const float g = grad_scale(p, r), inv = 1.0f / s;
-            char* dz = p.dz + r * p.dzp;
+            store_row<TR, NV>(p.dz + r * p.dzp, p.v, L, l, [&](int i, int e0, float* d) {
+                if (e0 < p.v) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e0 = (i * L + l) * TR::VEC;
-                float d[TR::VEC];
-#pragma unroll
-                for (int j = 0; j < TR::VEC; ++j) d[j] = some && e0 + j < p.v ? g * (x.x[i][j] * inv - acc[e0 + j]) : 0.0f;
-                if (e0 + TR::VEC <= p.v) {
-                    st_any(dz + (int64_t)e0 * TR::ESZ, pack_vec<TR>(d));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < TR::VEC; ++j)
-                        if (e0 + j < p.v) st_one<TR>(dz, e0 + j, d[j]);
+                    for (int j = 0; j < TR::VEC; j += 4) *reinterpret_cast<float4*>(d + j) = *reinterpret_cast<const float4*>(acc + e0 + j);
                 }
-            }
+#pragma unroll
+                for (int j = 0; j < TR::VEC; ++j) d[j] = some ? g * fmaf(x.x[i][j], inv, -d[j]) : 0.0f;
+            });
         }
         wave_sync();
     }
@@ -524,25 +671,52 @@ __global__ __launch_bounds__(1024) void distill_final(DistParams p) {
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
-// Long rows: forward with 1024 threads a row where rows alone do not fill the chip (5 x 32001 fp32: 13.1 -> 7.8 us), else 256.
-// Step: the fewest threads that hold the row with 4 or 8 vectors each, up to 1024 threads with 16 (262144 bytes of row).
-struct Plan { bool is_long; int L, nv, blocks, T, step_t, step_nv; };
-
-// Short rows: the fewest lanes whose registers (NVMAX vectors each) hold the row and whose rows' lists and class
-// weights leave the workgroup within 32 KB of LDS.
+// Short rows: the fewest lanes whose registers (NVMAX vectors each) hold the row and, 4 slots each, its list.  The backward
+// pass compares every held class with every slot while that is cheap (k * held classes <= REG_WORK: 2 M rows of 16 bf16 classes, 4
+// slots 103 us a step, 151 through LDS; 50000 x 512, 16 slots 79 and 72), else it goes through LDS, with the rows of a workgroup
+// within 32 KB.
+// Long rows, forward: a wave per row up to 1024 vectors, 256 threads behind that, 1024 where rows alone do not fill the chip (5 x
+// 32001 fp32: 256 threads 13.1 us, 1024 7.8).  Step: the fewest threads of 64, 256, 512, 1024 that hold the row with at
+// most 16 vectors each (262144 bytes of row).
+constexpr int REG_WORK = 128;
+struct Plan {
+    bool is_long;
+    int L, nv, sl;                   // short rows
+    int lds_L, lds_nv;               // the backward pass through LDS; lds_L 0: not used
+    int T, blocks;                   // threads and workgroups of the forward pass
+    int step_t, step_nv, step_blocks;
+    int bwd_blocks, parts;
+};
 Plan plan_of(int esz, int64_t rows, int v, int k) {
     Plan q;
+    memset(&q, 0, sizeof(q));
     const int vec = 16 / esz, nvec = (v + vec - 1) / vec;
+    auto least = [&](int64_t per, int64_t cap) { const int64_t b = (rows + per - 1) / per; return (int)(b < cap ? b : cap); };
+    auto vectors = [&](int L) { int n = 1; while (n * L < nvec) n *= 2; return n; };
     q.is_long = nvec > 64 * NVMAX;
-    q.L = 1;
-    while (q.L < 64 && (nvec > q.L * NVMAX || (TPB / q.L) * (2 * k + v) * 4 > 32768)) q.L *= 2;
-    q.nv = 1;
-    while (q.nv * q.L < nvec) q.nv *= 2;
-    q.T = rows < 512 ? 1024 : TPB;
-    q.step_t = nvec <= 2048 ? 256 : nvec <= 4096 ? 512 : 1024;
-    q.step_nv = nvec <= 1024 ? 4 : nvec <= 8192 ? 8 : nvec <= 16384 ? 16 : 0;
-    const int64_t per = q.is_long ? 1 : TPB / q.L, b = (rows + per - 1) / per;
-    q.blocks = (int)(b < 2048 ? b : 2048);
+    if (!q.is_long) {
+        q.L = 1;
+        while (q.L < 64 && (nvec > q.L * NVMAX || k > 4 * q.L)) q.L *= 2;
+        q.nv = vectors(q.L);
+        q.sl = k <= q.L ? 1 : 4;
+        q.blocks = q.bwd_blocks = q.parts = least(TPB / q.L, 2048);
+        if (k * q.nv * vec > REG_WORK) {
+            q.lds_L = 1;
+            while (q.lds_L < 64 && (nvec > q.lds_L * NVMAX || (TPB / q.lds_L) * lds_row(vec, v, k) * 4 > 32768)) q.lds_L *= 2;
+            q.lds_nv = vectors(q.lds_L);
+            q.bwd_blocks = least(TPB / q.lds_L, 2048);
+        }
+        return q;
+    }
+    q.T = rows < 512 ? 1024 : nvec <= 1024 ? 64 : TPB;
+    q.blocks = least(1, q.T == 64 ? 8192 : 2048);
+    q.bwd_blocks = least(1, 2048);
+    if (nvec <= 16384) {
+        q.step_t = rows < 512 ? 1024 : nvec <= 1024 ? 64 : nvec <= 4096 ? 256 : nvec <= 8192 ? 512 : 1024;
+        q.step_nv = nvec <= 4 * q.step_t ? 4 : nvec <= 8 * q.step_t ? 8 : 16;
+        q.step_blocks = least(1, q.step_t == 64 ? 4096 : 1024);
+    }
+    q.parts = q.blocks > q.step_blocks ? q.blocks : q.step_blocks;
     return q;
 }
 constexpr int COUNTS = 512;
@@ -567,28 +741,29 @@ int check_args(const char* who, int dtype, int64_t rows, int v, int64_t pitch, c
     return 0;
 }
 
-#define SHORT_LAUNCH(KERN, lds)                                                                \
-    do {                                                                                       \
-        if (dtype == 1) {                                                                      \
-            if (q.nv == 1) KERN<BF16, 1><<<q.blocks, TPB, lds, st>>>(p);                       \
-            else if (q.nv == 2) KERN<BF16, 2><<<q.blocks, TPB, lds, st>>>(p);                  \
-            else KERN<BF16, 4><<<q.blocks, TPB, lds, st>>>(p);                                 \
-        } else {                                                                               \
-            if (q.nv == 1) KERN<F32, 1><<<q.blocks, TPB, lds, st>>>(p);                        \
-            else if (q.nv == 2) KERN<F32, 2><<<q.blocks, TPB, lds, st>>>(p);                   \
-            else KERN<F32, 4><<<q.blocks, TPB, lds, st>>>(p);                                  \
-        }                                                                                      \
-        MI_HIP(hipGetLastError());                                                             \
+#define SHORT_NV(KERN, nv, grid, lds, ...)                                                                     \
+    do {                                                                                                       \
+        if (dtype == 1) {                                                                                      \
+            if (nv == 1) KERN<BF16, 1 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                                 \
+            else if (nv == 2) KERN<BF16, 2 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                            \
+            else KERN<BF16, 4 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                                         \
+        } else {                                                                                               \
+            if (nv == 1) KERN<F32, 1 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                                  \
+            else if (nv == 2) KERN<F32, 2 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                             \
+            else KERN<F32, 4 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                                          \
+        }                                                                                                      \
+        MI_HIP(hipGetLastError());                                                                             \
     } while (0)
+#define COMMA ,
 
 void fill(DistParams& p, const Plan& q, int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int t_dtype,
           const void* teacher, int i_dtype, const void* index, float temperature, float weight, int reduction, void* saved) {
     memset(&p, 0, sizeof(p));
     p.z = (const char*)logits; p.t = (const char*)teacher; p.idx = (const char*)index;
     p.rows = rows; p.v = v; p.k = k; p.zp = pitch * (dtype ? 2 : 4); p.t_bf16 = t_dtype; p.i64 = i_dtype == 2; p.red = reduction;
-    p.L = q.L; p.wl = weight * temperature * temperature; p.wg = weight * temperature; p.inv_t = 1.0f / temperature; p.c = (float)(1.4426950408889634 / (double)temperature);
-    p.sums = (double*)saved; p.part = p.sums + 2; p.nparts = q.blocks;
-    p.counts = p.part + 2 * q.blocks;
+    p.L = q.L; p.nparts = q.blocks; p.wl = weight * temperature * temperature; p.wg = weight * temperature; p.inv_t = 1.0f / temperature; p.c = (float)(1.4426950408889634 / (double)temperature);
+    p.sums = (double*)saved; p.part = p.sums + 2;
+    p.counts = p.part + 2 * q.parts;
     const int64_t c = (rows + 63) / 64;
     p.ncounts = (int)(c < COUNTS ? c : COUNTS);
     p.stat = (float2*)(p.counts + (q.is_long ? COUNTS : 0));
@@ -604,7 +779,7 @@ size_t mi_distill_loss_saved_bytes(int dtype, int64_t rows, int v, int k) {
         return 0;
     }
     const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);
-    return sizeof(double) * (2 + 2 * (size_t)q.blocks) + (q.is_long ? sizeof(double) * COUNTS + sizeof(float2) * (size_t)rows : 0);
+    return sizeof(double) * (2 + 2 * (size_t)q.parts) + (q.is_long ? sizeof(double) * COUNTS + sizeof(float2) * (size_t)rows : 0);
 }
 
 int mi_distill_loss_fwd(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
@@ -620,15 +795,18 @@ int mi_distill_loss_fwd(int dtype, int64_t rows, int v, int64_t pitch, const voi
     hipStream_t st = (hipStream_t)stream;
     if (q.is_long) {
         if (dtype == 1) {
-            if (q.T == 1024) distill_long_fwd<BF16, 1024><<<q.blocks, 1024, 0, st>>>(p);
-            else distill_long_fwd<BF16, TPB><<<q.blocks, TPB, 0, st>>>(p);
+            if (q.T == 64) distill_long_fwd<BF16, 64><<<q.blocks, 64, 0, st>>>(p);
+            else if (q.T == TPB) distill_long_fwd<BF16, TPB><<<q.blocks, TPB, 0, st>>>(p);
+            else distill_long_fwd<BF16, 1024><<<q.blocks, 1024, 0, st>>>(p);
         } else {
-            if (q.T == 1024) distill_long_fwd<F32, 1024><<<q.blocks, 1024, 0, st>>>(p);
-            else distill_long_fwd<F32, TPB><<<q.blocks, TPB, 0, st>>>(p);
+            if (q.T == 64) distill_long_fwd<F32, 64><<<q.blocks, 64, 0, st>>>(p);
+            else if (q.T == TPB) distill_long_fwd<F32, TPB><<<q.blocks, TPB, 0, st>>>(p);
+            else distill_long_fwd<F32, 1024><<<q.blocks, 1024, 0, st>>>(p);
         }
         MI_HIP(hipGetLastError());
     } else {
-        SHORT_LAUNCH(distill_short_fwd, 0);
+        if (q.sl == 1) SHORT_NV(distill_short_fwd, q.nv, q.blocks, 0, COMMA 1);
+        else SHORT_NV(distill_short_fwd, q.nv, q.blocks, 0, COMMA 4);
     }
     if (reduction) {
         distill_final<<<1, 1024, 0, st>>>(p);
@@ -640,7 +818,7 @@ int mi_distill_loss_fwd(int dtype, int64_t rows, int v, int64_t pitch, const voi
 int mi_distill_loss_step_ready(int dtype, int64_t rows, int v, int k, int reduction) {
     if ((dtype != 0 && dtype != 1) || rows <= 0 || v <= 0 || k <= 0 || k > MAX_K || reduction <= 0 || reduction > 2) return 0;
     const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);
-    return q.is_long && q.step_nv > 0;
+    return q.step_nv > 0;
 }
 
 int mi_distill_loss_step(int dtype, int64_t rows, int v, int64_t pitch, const void* logits, int k, int teacher_dtype,
@@ -657,18 +835,22 @@ int mi_distill_loss_step(int dtype, int64_t rows, int v, int64_t pitch, const vo
     fill(p, q, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction, saved);
     p.loss = loss; p.dz = (char*)dlogits; p.dzp = dpitch * (dtype ? 2 : 4);
     hipStream_t st = (hipStream_t)stream;
-    p.nparts = q.blocks < STEP_WGS ? q.blocks : STEP_WGS;
+    p.nparts = q.step_blocks;
     if (reduction == 1) {
         distill_count<<<p.ncounts, 64, 0, st>>>(p);
         MI_HIP(hipGetLastError());
     }
+#define STEP_ONE(TR, T_, NV_) if (q.step_t == T_ && q.step_nv == NV_) distill_long_step<TR, T_, NV_><<<p.nparts, T_, 0, st>>>(p)
 #define STEP_LAUNCH(TR)                                                                                        \
     do {                                                                                                       \
-        if (q.step_t == 256 && q.step_nv == 4) distill_long_step<TR, 256, 4><<<p.nparts, 256, 0, st>>>(p);     \
-        else if (q.step_t == 256) distill_long_step<TR, 256, 8><<<p.nparts, 256, 0, st>>>(p);                  \
-        else if (q.step_t == 512) distill_long_step<TR, 512, 8><<<p.nparts, 512, 0, st>>>(p);                  \
-        else if (q.step_nv == 8) distill_long_step<TR, 1024, 8><<<p.nparts, 1024, 0, st>>>(p);                 \
-        else distill_long_step<TR, 1024, 16><<<p.nparts, 1024, 0, st>>>(p);                                    \
+        STEP_ONE(TR, 64, 8);                                                                                   \
+        STEP_ONE(TR, 64, 16);                                                                                  \
+        STEP_ONE(TR, 256, 8);                                                                                  \
+        STEP_ONE(TR, 256, 16);                                                                                 \
+        STEP_ONE(TR, 512, 16);                                                                                 \
+        STEP_ONE(TR, 1024, 4);                                                                                 \
+        STEP_ONE(TR, 1024, 8);                                                                                 \
+        STEP_ONE(TR, 1024, 16);                                                                                \
     } while (0)
     if (dtype == 1) STEP_LAUNCH(BF16);
     else STEP_LAUNCH(F32);
@@ -694,13 +876,19 @@ int mi_distill_loss_bwd(int dtype, int64_t rows, int v, int64_t pitch, const voi
     p.gout = grad_out; p.dz = (char*)dlogits; p.dzp = dpitch * (dtype ? 2 : 4);
     hipStream_t st = (hipStream_t)stream;
     if (q.is_long) {
-        const int blocks = p.done && q.blocks > 512 ? 512 : q.blocks;  // mostly there to leave again
+        const int blocks = p.done && q.bwd_blocks > 512 ? 512 : q.bwd_blocks;  // mostly there to leave again
         if (dtype == 1) distill_long_bwd<BF16><<<blocks, TPB, 0, st>>>(p);
         else distill_long_bwd<F32><<<blocks, TPB, 0, st>>>(p);
         MI_HIP(hipGetLastError());
     } else {
-        const int lds = (TPB / q.L) * (2 * k + v) * 4;
-        SHORT_LAUNCH(distill_short_bwd, lds);
+        if (q.lds_L) {
+            p.L = q.lds_L;
+            SHORT_NV(distill_short_bwd, q.lds_nv, q.bwd_blocks, (TPB / q.lds_L) * lds_row(dtype ? 8 : 4, v, k) * 4, );
+        } else if (q.sl == 1) {
+            SHORT_NV(distill_short_bwd_reg, q.nv, q.bwd_blocks, 0, COMMA 1);
+        } else {
+            SHORT_NV(distill_short_bwd_reg, q.nv, q.bwd_blocks, 0, COMMA 4);
+        }
     }
     return 0;
 }

@@ -25,6 +25,18 @@ __device__ __forceinline__ void st_one(char* p, int64_t i, float v) {
     else reinterpret_cast<float*>(p)[i] = v;
 }
 
+// a vector moved down by n elements (0 < n < VEC)
+template <class TR>
+__device__ __forceinline__ uint4 down(uint4 w, int n) {
+    const int bits = n * TR::ESZ * 8;
+    if (bits & 64) { w.x = w.z; w.y = w.w; }
+    if (bits & 32) { w.x = w.y; w.y = w.z; w.z = w.w; }
+    if (TR::ESZ == 2 && (bits & 16)) {
+        w.x = w.x >> 16 | w.y << 16; w.y = w.y >> 16 | w.z << 16; w.z = w.z >> 16 | w.w << 16; w.w >>= 16;
+    }
+    return w;
+}
+
 // the compiler takes the value as new: what was computed from it before is not kept in registers
 __device__ __forceinline__ void hold(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
 
