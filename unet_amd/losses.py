@@ -123,31 +123,33 @@ def _distill_sizes(dt, rows, v, k, red):
     return lib.mi_distill_loss_saved_bytes(dt, rows, v, k), bool(lib.mi_distill_loss_step_ready(dt, rows, v, k, red))
 
 
+def _distill_call(logits, teacher, index, temperature, weight, red, train):
+    """The forward call: (loss, what the backward call reads, the gradient for an upstream gradient of 1 or None)."""
+    lib, dev = _lib.load(), logits.device
+    z, pitch = _pixels(logits, "input")
+    v, k = z.shape[-1], index.shape[-1]
+    rows = index.numel() // k
+    dt = _DT[z.dtype]
+    nbytes, in_one = _distill_sizes(dt, rows, v, k, red)
+    loss = teacher.new_empty(index.shape[:-1] if red == 0 else (), dtype=torch.float32)
+    saved = index.new_empty(nbytes, dtype=torch.uint8)
+    args = (dt, rows, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(), _INDEX[index.dtype],
+            index.data_ptr(), temperature, weight, red, loss.data_ptr(), saved.data_ptr())
+    with _lib.on_device(dev):
+        if train and in_one:
+            dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
+            _lib.check(lib.mi_distill_loss_step(*args, v, dz.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_step")
+            return loss, saved, dz
+        _lib.check(lib.mi_distill_loss_fwd(*args, _lib.stream_of(dev)), "mi_distill_loss_fwd")
+    return loss, saved, None
+
+
 class _DistillFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher, index, temperature, weight, red):
-        lib, dev = _lib.load(), logits.device
-        z, pitch = _pixels(logits, "input")
-        v, k = z.shape[-1], index.shape[-1]
-        rows = index.numel() // k
-        loss = torch.empty(index.shape[:-1] if red == 0 else (), dtype=torch.float32, device=dev)
-        dt = _DT[z.dtype]
-        nbytes, in_one = _distill_sizes(dt, rows, v, k, red)
-        args = (dt, rows, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(), _INDEX[index.dtype],
-                index.data_ptr(), temperature, weight, red)
-        train = ctx.needs_input_grad[0]
-        dz = None
-        with _lib.on_device(dev):
-            saved = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            if train and in_one:
-                dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
-                _lib.check(lib.mi_distill_loss_step(*args, loss.data_ptr(), saved.data_ptr(), v, dz.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_step")
-            else:
-                _lib.check(lib.mi_distill_loss_fwd(*args, loss.data_ptr(), saved.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_fwd")
-        if train:
-            ctx.save_for_backward(logits, teacher, index, saved)
-            ctx.cfg = (temperature, weight, red)
-            ctx.dz = dz      # the gradient for gout = 1; given away by the first backward call
+        loss, saved, ctx.dz = _distill_call(logits, teacher, index, temperature, weight, red, True)
+        ctx.save_for_backward(logits, teacher, index, saved)
+        ctx.cfg = (temperature, weight, red)
         return loss
 
     @staticmethod
@@ -158,11 +160,11 @@ class _DistillFunction(torch.autograd.Function):
         lib, dev = _lib.load(), logits.device
         z, pitch = _pixels(logits, "input")
         v, k = z.shape[-1], index.shape[-1]
-        dz, ctx.dz = ctx.dz, None
+        dz, ctx.dz = ctx.dz, None        # given away by the first backward call
         done = dz is not None
         if not done:
             dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
-        g = gout.contiguous().float()
+        g = gout if gout.dtype == torch.float32 and gout.is_contiguous() else gout.contiguous().float()
         with _lib.on_device(dev):
             _lib.check(lib.mi_distill_loss_bwd(_DT[z.dtype], index.numel() // k, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(),
                                                _INDEX[index.dtype], index.data_ptr(), temperature, weight, red, g.data_ptr(), saved.data_ptr(),
@@ -222,4 +224,7 @@ class TopLogitDistillationLoss(nn.Module):
         if i.numel() == 0:
             total = x.float().sum(-1)                              # nothing to learn from: zeros that know the input
             return total if red == 0 else total.sum()
-        return _DistillFunction.apply(x, t.contiguous(), i.contiguous(), self.temperature, self.weight, red)
+        t, i = t.contiguous(), i.contiguous()
+        if x.requires_grad and torch.is_grad_enabled():
+            return _DistillFunction.apply(x, t, i, self.temperature, self.weight, red)
+        return _distill_call(x, t, i, self.temperature, self.weight, red, False)[0]

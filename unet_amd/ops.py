@@ -270,15 +270,15 @@ def groupnorm_act_fwd(x, groups, weight=None, bias=None, act="silu", alpha=None,
     ``alpha`` are read as fp32.  Returns (y, stats [N, groups, 2] fp32: mean and 1 / sqrt(variance + eps), for the backward call)."""
     nb, npix, c, groups, weight, bias, alpha = _groupnorm_args(x, groups, weight, bias, act, alpha)
     x, xp = _pixels(x, "x")
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(nb, groups, 2, dtype=torch.float32, device=x.device)
+    out = x.new_empty(x.shape)
+    stats = x.new_empty((nb, groups, 2), dtype=torch.float32)
     if res is not None:
         res, rp = _pixels(res, "res", x)
     if nb == 0:
         return out, stats
     lib, dt = _lib.load(), _DT[x.dtype]
     with _lib.on_device(x.device):
-        ws = torch.empty(_groupnorm_workspace(dt, nb, npix, c, groups, 0), dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(_groupnorm_workspace(dt, nb, npix, c, groups, 0), dtype=torch.uint8)
         _lib.check(lib.mi_groupnorm_act_fwd(dt, nb, npix, c, groups, _view(x, xp), _lib.ptr(weight), _lib.ptr(bias), _ACT[act],
                                             _lib.ptr(alpha), _view(res, rp) if res is not None else None, _view(out, c), eps, stats.data_ptr(), ws.data_ptr(), _lib.stream_of(x.device)), "mi_groupnorm_act_fwd")
     return out, stats
@@ -293,16 +293,16 @@ def groupnorm_act_bwd(dy, x, stats, groups, weight=None, bias=None, act="silu", 
     if tuple(stats.shape) != (nb, groups, 2) or stats.dtype != torch.float32 or stats.device != x.device:
         raise ValueError(f"stats must be the fp32 tensor [{nb}, {groups}, 2] of the forward call")
     stats = stats.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    new = torch.zeros if nb == 0 else torch.empty
-    dw = new(c, dtype=torch.float32, device=x.device) if weight is not None else None
-    db = new(c, dtype=torch.float32, device=x.device) if bias is not None else None
-    da = new(1, dtype=torch.float32, device=x.device) if alpha is not None else None
+    dx = x.new_empty(x.shape)
+    new = x.new_zeros if nb == 0 else x.new_empty
+    dw = new(c, dtype=torch.float32) if weight is not None else None
+    db = new(c, dtype=torch.float32) if bias is not None else None
+    da = new(1, dtype=torch.float32) if alpha is not None else None
     if nb == 0:
         return dx, dw, db, da
     lib, dt = _lib.load(), _DT[x.dtype]
     with _lib.on_device(x.device):
-        ws = torch.empty(_groupnorm_workspace(dt, nb, npix, c, groups, 1), dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(_groupnorm_workspace(dt, nb, npix, c, groups, 1), dtype=torch.uint8)
         _lib.check(lib.mi_groupnorm_act_bwd(dt, nb, npix, c, groups, _view(dy, dp), _view(x, xp), stats.data_ptr(), _lib.ptr(weight),
                                             _lib.ptr(bias), _ACT[act], _lib.ptr(alpha), _view(dx, c), _lib.ptr(dw), _lib.ptr(db),
                                             _lib.ptr(da), ws.data_ptr(), _lib.stream_of(x.device)), "mi_groupnorm_act_bwd")
@@ -324,8 +324,8 @@ def top_logits(logits, k):
         raise ValueError(f"k must be in 1 .. {min(v, 256)} for {v} classes, got {k}")
     x, pitch = _pixels(logits, "logits")
     shape = logits.shape[:-1] + (k,)
-    values = torch.empty(shape, dtype=x.dtype, device=x.device)
-    index = torch.empty(shape, dtype=torch.int32, device=x.device)
+    values = x.new_empty(shape)
+    index = x.new_empty(shape, dtype=torch.int32)
     rows = index.numel() // k
     if rows:
         with _lib.on_device(x.device):
