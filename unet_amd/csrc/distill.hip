@@ -514,7 +514,8 @@ __global__ __launch_bounds__(64) void distill_count(DistParams p) {
 // student's logits of its classes are fetched while the row is on its way, so that no wave waits for memory once it is there; as
 // a vector's gradient is stored, the same vector of the next row is requested.  The exponentials are taken twice: kept, they
 // need twice the registers of the bf16 row, and fewer rows in flight cost more than the arithmetic (4096 x 32768 bf16 step: 160 us
-// kept, 138 taken twice, 190 with two passes over memory).
+// kept, 138 taken twice, 190 with two passes over memory).  Logits and gradient pass the caches by: 137 -> 123 us (the gradient alone
+// 131).
 template <class TR, int T, int NV>
 __global__ __launch_bounds__(T, 4) void distill_long_step(DistParams p) {
     __shared__ float wm[T / 64], ws[T / 64], qw[MAX_K], qt[MAX_K], qz[MAX_K], scale_s;
@@ -533,7 +534,7 @@ __global__ __launch_bounds__(T, 4) void distill_long_step(DistParams p) {
     auto fetch = [&](const char* z, int u) {
         constexpr unsigned none = TR::ESZ == 2 ? 0xff80ff80u : 0xff800000u;
         raw[u] = make_uint4(none, none, none, none);
-        if (u * T + tid < nv) raw[u] = ld_any<TR>(z + u * (T * 16) + (unsigned)tid * 16u);
+        if (u * T + tid < nv) raw[u] = ld_any_nt<TR>(z + u * (T * 16) + (unsigned)tid * 16u);
     };
     int64_t r = blockIdx.x;
     if (r < p.rows) {
@@ -585,7 +586,7 @@ __global__ __launch_bounds__(T, 4) void distill_long_step(DistParams p) {
             unpack_vec<TR>(raw[u], y);
 #pragma unroll
             for (int j = 0; j < TR::VEC; ++j) y[j] = some ? f * __builtin_amdgcn_exp2f((y[j] - st.x) * p.c) : 0.0f;
-            if (u * T + tid < nv) st_any(dz + u * (T * 16) + (unsigned)tid * 16u, pack_vec<TR>(y));
+            if (u * T + tid < nv) st_any_nt(dz + u * (T * 16) + (unsigned)tid * 16u, pack_vec<TR>(y));
             if (more) fetch(zn, u);
         }
         if (et < p.v) {
@@ -634,10 +635,10 @@ __global__ __launch_bounds__(TPB) void distill_long_bwd(DistParams p) {
 #pragma unroll 4
         for (int i = threadIdx.x; i < nv; i += TPB) {
             float x[TR::VEC];
-            unpack_vec<TR>(ld_any<TR>(z + (int64_t)i * 16), x);
+            unpack_vec<TR>(ld_any_nt<TR>(z + (int64_t)i * 16), x);
 #pragma unroll
             for (int j = 0; j < TR::VEC; ++j) x[j] = some ? f * __builtin_amdgcn_exp2f((x[j] - st.x) * p.c) : 0.0f;
-            st_any(dz + (int64_t)i * 16, pack_vec<TR>(x));
+            st_any_nt(dz + (int64_t)i * 16, pack_vec<TR>(x));
         }
         for (int i = nv * TR::VEC + threadIdx.x; i < p.v; i += TPB)
             st_one<TR>(dz, i, some ? f * __builtin_amdgcn_exp2f((ld_one<TR>(z, i) - st.x) * p.c) : 0.0f);

@@ -25,16 +25,7 @@ namespace {
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_PRELU = 4 };
 constexpr int TPB = 256;
-#ifndef GN_U
-#define GN_U 4
-#endif
-#ifndef GN_UB
-#define GN_UB 2
-#endif
-#ifndef GN_WG
-#define GN_WG 2048
-#endif
-constexpr int U = GN_U, UB = GN_UB; // vectors in flight per thread and tensor: forward, backward
+constexpr int U = 4, UB = 2;         // vectors in flight per thread and tensor: forward, backward
 constexpr int CHUNK = 256;           // pixels a thread adds in fp32 before the sums move to fp64
 constexpr int MAX_C = 8192, MAX_G = 2048;
 
@@ -177,6 +168,33 @@ template <> struct RawOf<2> { typedef unsigned short T; };
 template <class TR, int VEC> using Raw = typename RawOf<VEC * TR::ESZ>::T;
 template <class TR, int VEC>
 __device__ __forceinline__ Raw<TR, VEC> ldr(const char* p) { return *reinterpret_cast<const Raw<TR, VEC>*>(p); }
+// The second passes read their tensors for the last time and write more than the caches hold of use to the next kernel:
+// past the caches (32 x 256^2 x 32 bf16 forward 89 -> 77 us, 32 x 256^2 x 16 backward 72 -> 63, 3-D fp32 backward 60 -> 49; with an
+// elementwise reader of the result behind the call 137 -> 130 us at 128 MiB a tensor and no difference from 8 to 96 MiB).
+typedef unsigned nvec4 __attribute__((ext_vector_type(4)));
+typedef unsigned nvec2 __attribute__((ext_vector_type(2)));
+template <class TR, int VEC>
+__device__ __forceinline__ Raw<TR, VEC> ldr_nt(const char* p) {
+    typedef Raw<TR, VEC> R;
+    if constexpr (sizeof(R) == 16) {
+        const nvec4 v = __builtin_nontemporal_load(reinterpret_cast<const nvec4*>(p));
+        return make_uint4(v.x, v.y, v.z, v.w);
+    } else if constexpr (sizeof(R) == 8) {
+        const nvec2 v = __builtin_nontemporal_load(reinterpret_cast<const nvec2*>(p));
+        return make_uint2(v.x, v.y);
+    } else {
+        return __builtin_nontemporal_load(reinterpret_cast<const R*>(p));
+    }
+}
+template <class TR, int VEC>
+__device__ __forceinline__ void stv_nt(char* p, const float* v) {
+    typedef Raw<TR, VEC> R;
+    R r;
+    stv<TR, VEC>(reinterpret_cast<char*>(&r), v);
+    if constexpr (sizeof(R) == 16) __builtin_nontemporal_store((nvec4){r.x, r.y, r.z, r.w}, reinterpret_cast<nvec4*>(p));
+    else if constexpr (sizeof(R) == 8) __builtin_nontemporal_store((nvec2){r.x, r.y}, reinterpret_cast<nvec2*>(p));
+    else __builtin_nontemporal_store(r, reinterpret_cast<R*>(p));
+}
 template <class TR, int VEC>
 __device__ __forceinline__ void unraw(const Raw<TR, VEC>& r, float* v) {
     Raw<TR, VEC> t = r;
@@ -355,14 +373,9 @@ struct FwdConst {
 
 template <class TR, int VEC>
 __global__ __launch_bounds__(TPB) void gn_apply_kernel(GnParams p) {
-#ifdef GN_REV
-    const int blk = gridDim.x % 8 == 0 ? (gridDim.x / 8 - 1 - blockIdx.x / 8) * 8 + blockIdx.x % 8 : gridDim.x - 1 - blockIdx.x;
-#else
-    const int blk = blockIdx.x;
-#endif
     extern __shared__ float2 mr[];                                  // [groups] mean, rstd
     __shared__ double sm[2 * TPB];
-    const int n = blk / p.B, bi = blk % p.B;
+    const int n = blockIdx.x / p.B, bi = blockIdx.x % p.B;
     const double cnt = (double)p.npix * p.cg;
     join_groups(p.part + (int64_t)n * p.S * p.groups * 2, p.S, p.groups, sm, [&](int g, double a, double b) {
         mr[g] = moments(a, b, cnt, p.eps);
@@ -388,10 +401,10 @@ __global__ __launch_bounds__(TPB) void gn_apply_kernel(GnParams p) {
             constexpr int N = decltype(nu)::value;
             Raw<TR, VEC> xv[N], rv[N];
 #pragma unroll
-            for (int u = 0; u < N; ++u) xv[u] = ldr<TR, VEC>(x + u * xs);
+            for (int u = 0; u < N; ++u) xv[u] = ldr_nt<TR, VEC>(x + u * xs);
             if (r) {
 #pragma unroll
-                for (int u = 0; u < N; ++u) rv[u] = ldr<TR, VEC>(r + u * rs);
+                for (int u = 0; u < N; ++u) rv[u] = ldr_nt<TR, VEC>(r + u * rs);
                 r += N * rs;
             }
 #pragma unroll
@@ -405,7 +418,7 @@ __global__ __launch_bounds__(TPB) void gn_apply_kernel(GnParams p) {
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) v[j] += q[j];
                 }
-                stv<TR, VEC>(o + u * os, v);
+                stv_nt<TR, VEC>(o + u * os, v);
             }
             x += N * xs; o += N * os;
         };
@@ -565,13 +578,7 @@ __global__ __launch_bounds__(TPB) void gn_bwd_apply_kernel(GnParams p) {
         join_params(p, (int)blockIdx.x - p.nb * p.B, p.nb * p.S, sm);
         return;
     }
-    const int nblk = p.nb * p.B;
-#ifdef GN_REV
-    const int blk = nblk % 8 == 0 ? (nblk / 8 - 1 - (int)blockIdx.x / 8) * 8 + (int)blockIdx.x % 8 : nblk - 1 - (int)blockIdx.x;
-#else
-    const int blk = blockIdx.x;
-#endif
-    const int n = blk / p.B, bi = blk % p.B;
+    const int n = blockIdx.x / p.B, bi = blockIdx.x % p.B;
     const double cnt = (double)p.npix * p.cg;
     join_groups(p.part + (int64_t)n * p.S * p.groups * 2, p.S, p.groups, sm,
                 [&](int g, double a, double b) { gm[g] = make_float2((float)(a / cnt), (float)(b / cnt)); });
@@ -598,7 +605,7 @@ __global__ __launch_bounds__(TPB) void gn_bwd_apply_kernel(GnParams p) {
             constexpr int N = decltype(nu)::value;
             Raw<TR, VEC> xv[N], dv[N];
 #pragma unroll
-            for (int u = 0; u < N; ++u) { xv[u] = ldr<TR, VEC>(x + u * xs); dv[u] = ldr<TR, VEC>(d + u * ds); }
+            for (int u = 0; u < N; ++u) { xv[u] = ldr_nt<TR, VEC>(x + u * xs); dv[u] = ldr_nt<TR, VEC>(d + u * ds); }
 #pragma unroll
             for (int u = 0; u < N; ++u) {
                 float v[VEC], dy[VEC], g[VEC];
@@ -606,7 +613,7 @@ __global__ __launch_bounds__(TPB) void gn_bwd_apply_kernel(GnParams p) {
                 unraw<TR, VEC>(dv[u], dy);
                 k.grad(p.act, alpha, v, dy, g);
                 k.dx(v, g, m0, m1, v);
-                stv<TR, VEC>(o + u * os, v);
+                stv_nt<TR, VEC>(o + u * os, v);
             }
             x += N * xs; d += N * ds; o += N * os;
         };
@@ -762,17 +769,11 @@ __global__ __launch_bounds__(TPB) void gn_join_kernel(GnParams p) {
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
-// Splits of an image in both passes: enough workgroups to fill the chip (2048 = 8 per CU), at least 32 KB of the tensor per
-// workgroup, and at most 8192 pairs (128 KB, in L2) for a workgroup of the second pass to join.
-#ifndef GN_WGB
-#define GN_WGB 512
-#endif
-#ifndef GN_WGBA
-#define GN_WGBA GN_WGB
-#endif
-#ifndef GN_WGA
-#define GN_WGA GN_WG
-#endif
+// Splits of an image in both passes: FWD_WGS or BWD_WGS workgroups in all, at least 32 KB of the tensor per workgroup, and at
+// most 8192 pairs (128 KB, in L2) for a workgroup of the second pass to join.  32 x 256^2 x 32 bf16 forward with 1024 / 2048 / 4096
+// workgroups: 90.8 / 88.5 / 90.5 us; 32 x 256^2 x 16 backward, whose sums per workgroup cost more, with 256 / 512 / 1024 / 2048: 75.2 /
+// 72.5 / 76.6 / 82.0 (all before the second pass went past the caches).
+constexpr int FWD_WGS = 2048, BWD_WGS = 512;
 int splits(int esz, int nb, int64_t npix, int c, int groups, int wgs) {
     const int64_t bytes = npix * c * esz;
     int64_t s = (wgs + nb - 1) / nb;
@@ -783,7 +784,7 @@ int splits(int esz, int nb, int64_t npix, int c, int groups, int wgs) {
 }
 
 // Small images: slabs of whole groups at least 64 bytes wide, held by 256 threads with at most `most` vectors each.
-// 16 x 16 x 256 bf16, one image: TODO
+// (one image of 16 x 16 x 256 bf16: 6.7 us of kernel against 4.5 + 7.5 in two passes.)
 struct Small { bool ok; int groups, slabs, nv; };
 Small small_of(int esz, int vec, int64_t npix, int c, int groups, int most) {
     const int cg = c / groups;
@@ -865,7 +866,7 @@ extern "C" {
 
 size_t mi_groupnorm_act_workspace_bytes(int dtype, int nb, int64_t npix, int c, int groups, int backward) {
     if (check_shape(__func__, dtype, nb, npix, c, groups)) return 0;
-    const size_t s = (size_t)nb * splits(dtype ? 2 : 4, nb, npix, c, groups, backward ? GN_WGB : GN_WG);
+    const size_t s = (size_t)nb * splits(dtype ? 2 : 4, nb, npix, c, groups, backward ? BWD_WGS : FWD_WGS);
     // a small image's backward pass: [nb][c][2] and at most [nb][groups]
     return (s * groups * 2 + (backward ? s * c * 2 + s : 0)) * sizeof(double);
 }
@@ -895,7 +896,7 @@ int mi_groupnorm_act_fwd(int dtype, int nb, int64_t npix, int c, int groups, con
         GN_SMALL(gn_small_fwd_kernel, nb * p.S, q.groups * 2 * sizeof(double));
         return 0;
     }
-    p.S = splits(esz, nb, npix, c, groups, GN_WG); p.B = splits(esz, nb, npix, c, groups, GN_WGA);
+    p.S = p.B = splits(esz, nb, npix, c, groups, FWD_WGS);
     GN_LAUNCH(gn_stats_kernel, nb * p.S, groups * 2 * sizeof(double));
     GN_LAUNCH(gn_apply_kernel, nb * p.B, groups * 2 * sizeof(float));
     return 0;
@@ -931,7 +932,7 @@ int mi_groupnorm_act_bwd(int dtype, int nb, int64_t npix, int c, int groups, con
         MI_HIP(hipGetLastError());
         return 0;
     }
-    p.S = splits(esz, nb, npix, c, groups, GN_WGB); p.B = splits(esz, nb, npix, c, groups, GN_WGBA);
+    p.S = p.B = splits(esz, nb, npix, c, groups, BWD_WGS);
     const size_t s = (size_t)nb * p.S;
     p.part = (double*)workspace;
     p.part_c = p.part + s * groups * 2;

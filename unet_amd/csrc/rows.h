@@ -14,6 +14,16 @@ __device__ __forceinline__ void st_any(char* p, const uint4& v) {
     uvec4 u = {v.x, v.y, v.z, v.w};
     *reinterpret_cast<uvec4*>(p) = u;
 }
+// the same past the caches
+template <class TR>
+__device__ __forceinline__ uint4 ld_any_nt(const char* p) {
+    const uvec4 u = __builtin_nontemporal_load(reinterpret_cast<const uvec4*>(p));
+    return make_uint4(u.x, u.y, u.z, u.w);
+}
+__device__ __forceinline__ void st_any_nt(char* p, const uint4& v) {
+    const uvec4 u = {v.x, v.y, v.z, v.w};
+    __builtin_nontemporal_store(u, reinterpret_cast<uvec4*>(p));
+}
 template <class TR>
 __device__ __forceinline__ float ld_one(const char* p, int64_t i) {
     if constexpr (TR::ESZ == 2) return bf16_to_f32(reinterpret_cast<const unsigned short*>(p)[i]);
