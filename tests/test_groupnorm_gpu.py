@@ -118,6 +118,13 @@ CASES = [  # N, spatial, C, groups, act, affine, residual, mean offset
     (2, (4, 4), 2050, 1025, "none", True, False, 0.0),
     (300, (2, 2), 16, 16, "silu", True, False, 0.0),
     (2, (80, 80), 16, 2, "silu", True, False, 1000.0),     # mean far from zero
+    (3, (61, 53), 33, 3, "silu", True, True, 0.0),         # odd channel counts, a number of pixels that is no multiple of 8 or 4
+    (1, (151, 149), 5, 5, "prelu", True, False, 0.0),
+    (2, (67, 71), 30, 10, "gelu", True, True, 2.0),
+    (1, (50, 51), 255, 5, "silu", True, False, 0.0),
+    (1, (41, 43), 257, 1, "relu", True, False, 0.0),
+    (2, (53, 37), 250, 125, "silu", False, False, 0.0),
+    (2, (103, 101), 12, 2, "none", True, False, 0.0),
 ]
 
 
@@ -204,6 +211,24 @@ def test_views_and_other_orders(dev, mode):
     assert torch.equal(y1, y2)
 
 
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+def test_large_slices_of_wider_tensors(dev, mode):
+    """The same numbers from a slice of the channels, read where it lies, as from a dense copy of it."""
+    for c, lo, width in ((30, 1, 40), (32, 8, 64), (7, 2, 9)):
+        case = (2, (73, 77), c, 1, "silu", True, False, 0.0)
+        x, dy, w, b, _, _ = make(case, mode, dev)
+        wide = torch.full((2, 73, 77, width), float("nan"), dtype=x.dtype, device=dev)
+        wide[..., lo:lo + c] = x
+        y, s = ops.groupnorm_act_fwd(wide[..., lo:lo + c], 1, w, b)
+        got = ops.groupnorm_act_bwd(dy, wide[..., lo:lo + c], s, 1, w, b)
+        ref = formula(x, 1, w, b, "silu", None, None, dy)
+        check_forward(y, s, ref, mode)
+        check_backward(got, ref, mode)
+        y, s = ops.groupnorm_act_fwd(x, 1, w, b)
+        check_forward(y, s, ref, mode)
+        check_backward(ops.groupnorm_act_bwd(dy, x, s, 1, w, b), ref, mode)
+
+
 def test_nan_and_infinity_stay_in_their_group(dev):
     x, dy, w, b, _, _ = make((2, (40, 40), 16, 4, "silu", True, False, 0.0), "fp32", dev)
     y0, s0 = ops.groupnorm_act_fwd(x, 4, w, b)
@@ -216,6 +241,16 @@ def test_nan_and_infinity_stay_in_their_group(dev):
     for act in ("none", "relu", "gelu"):
         y, _ = ops.groupnorm_act_fwd(bad, 4, w, b, act=act)
         assert torch.isnan(y[0, ..., :4]).all()
+    x, dy, w, b, _, _ = make((1, (81, 83), 15, 5, "silu", True, False, 0.0), "bf16", dev)
+    y0, s0 = ops.groupnorm_act_fwd(x, 5, w, b)
+    g0 = ops.groupnorm_act_bwd(dy, x, s0, 5, w, b)
+    bad = x.clone()
+    bad[0, 80, 82, 4] = float("nan")                       # the last pixel, group 1
+    y, s = ops.groupnorm_act_fwd(bad, 5, w, b)
+    g = ops.groupnorm_act_bwd(dy, bad, s, 5, w, b)
+    keep = [0, 1, 2] + list(range(6, 15))
+    assert torch.isnan(y[..., 3:6]).all() and torch.equal(y[..., keep], y0[..., keep])
+    assert torch.isnan(g[0][..., 3:6]).all() and torch.equal(g[0][..., keep], g0[0][..., keep]) and torch.equal(g[1][keep], g0[1][keep])
 
 
 def test_an_outlier_as_the_first_value_does_not_cost_the_variance(dev):
