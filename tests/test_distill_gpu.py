@@ -47,7 +47,8 @@ def check_top(x, k):
 
 TOP = [(1, 1, 1), (7, 2, 2), (300, 3, 2), (300, 16, 4), (65, 16, 16), (130, 21, 5), (33, 64, 64), (40, 133, 8), (9, 255, 255), (5, 256, 256),
        (17, 257, 17), (6, 512, 16), (6, 513, 40), (5, 1024, 100), (5, 1025, 16), (5, 1025, 200), (4, 2048, 16), (4, 2049, 3), (3, 5000, 256), (2, 50001, 32),
-       (1, 128000, 64), (1, 4097, 1), (600, 2100, 20), (520, 4200, 100), (513, 20000, 70), (513, 40000, 200), (3, 70000, 256), (2, 140000, 256), (2, 2049, 256), (300, 176, 17), (40, 700, 130)]
+       (1, 128000, 64), (1, 4097, 1), (600, 2100, 20), (520, 4200, 100), (513, 20000, 70), (513, 40000, 200), (3, 70000, 256), (2, 140000, 256), (2, 2049, 256), (300, 176, 17), (40, 700, 130), (5, 2100, 24), (5, 2100, 200), (5, 4200, 60),
+       (5, 9000, 42)]
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])
@@ -400,6 +401,34 @@ def test_captured_steps_replay(dev):
             want = step()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_more_than_2_31_logits(dev):
+    """Offsets beyond 32 bits: the last rows of 66000 x 32800 bf16 logits against calls on those rows alone."""
+    rows, v, k = 66000, 32800, 3
+    x = torch.empty(rows, v, dtype=torch.bfloat16, device=dev)
+    x.normal_()
+    g = torch.Generator().manual_seed(12)
+    t, i = lists(rows, v, k, g, dev)
+    i[-5:] = torch.tensor([v - 1, 0, 5], device=dev)
+    values, index = ops.top_logits(x, k)
+    last = slice(rows - 3, rows)
+    v1, i1 = ops.top_logits(x[last].clone(), k)
+    assert torch.equal(values[last], v1) and torch.equal(index[last], i1)
+    del values, index
+    fn = unet_amd.TopLogitDistillationLoss(2.0, "none")
+    x.requires_grad_(True)
+    out = fn(x, t, i)
+    (dz,) = torch.autograd.grad(out, x, torch.ones_like(out))
+    x1 = x[last].detach().clone().requires_grad_(True)
+    o1 = fn(x1, t[last], i[last])
+    (d1,) = torch.autograd.grad(o1, x1, torch.ones_like(o1))
+    assert torch.allclose(out[last], o1, rtol=1e-5) and torch.allclose(dz[last].float(), d1.float(), rtol=2.0 ** -7, atol=1e-9)
+    del dz, d1
+    total = unet_amd.TopLogitDistillationLoss(2.0, "sum")
+    (dz,) = torch.autograd.grad(total(x, t, i), x)
+    (d1,) = torch.autograd.grad(total(x1, t[last], i[last]), x1)
+    assert torch.allclose(dz[last].float(), d1.float(), rtol=2.0 ** -7, atol=1e-9)
 
 
 # ---- together ---------------------------------------------------------------------------------------------------------

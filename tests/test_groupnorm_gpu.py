@@ -261,6 +261,23 @@ def test_an_outlier_as_the_first_value_does_not_cost_the_variance(dev):
     assert abs(float(s[0, 0, 1]) / float(ref["rstd"]) - 1) < STAT
 
 
+def test_more_than_2_31_elements(dev):
+    """Offsets beyond 32 bits: an image whose last pixels lie behind 2^31 elements, and its gradient."""
+    npix, c = 67200000, 32
+    x = torch.empty(1, npix, c, dtype=torch.bfloat16, device=dev)
+    x.normal_()
+    y, s = ops.groupnorm_act_fwd(x, 4, act="none")
+    m = torch.stack([p.reshape(-1, 4, 8).float().double().mean((0, 2)) * p.shape[0] for p in x[0].split(4200000)]).sum(0) / npix
+    q = torch.stack([p.reshape(-1, 4, 8).float().double().square().mean((0, 2)) * p.shape[0] for p in x[0].split(4200000)]).sum(0) / npix
+    rstd = 1 / torch.sqrt(q - m * m + 1e-5)
+    assert (s[0, :, 0].double() - m).abs().max() < STAT and (s[0, :, 1].double() / rstd - 1).abs().max() < STAT
+    for a in (0, npix - 40):
+        want = (x[0, a:a + 40].double().reshape(-1, 4, 8) - m[:, None]) * rstd[:, None]
+        assert ((y[0, a:a + 40].double().reshape(want.shape) - want).abs() <= want.abs() * HALF_STEP["bf16"] + 4 * STAT).all()
+    dx, _, _, _ = ops.groupnorm_act_bwd(y, x, s, 4, act="none")     # y as its own gradient: dx = rstd (y - xh mean(y xh)) = 0
+    assert dx[0, -40:].float().abs().max() < 6 * 2.0 ** -8 * float(rstd.max()) * 1.1      # |xh| < 6, half a step of y
+
+
 def test_results_repeat_bit_for_bit_and_other_streams_wait(dev):
     case = (2, (200, 170), 32, 8, "prelu", True, False, 0.0)
     x, dy, w, b, alpha, _ = make(case, "bf16", dev)

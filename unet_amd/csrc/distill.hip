@@ -10,8 +10,8 @@
 // over the list, nothing that cancels.
 //
 // Bandwidth-bound: the forward pass cannot do without one read of z, the backward pass without one read and one write.
-//   short rows (up to ROW_REG bytes per lane group): L neighbouring lanes share a row and hold it in registers
-//   long rows : a workgroup per row, one pass with a running maximum and sum per thread
+//   short rows (up to 4 KB): L neighbouring lanes share a row and hold it in registers
+//   long rows : a wave or a workgroup per row, one pass with a running maximum and sum per thread
 //   long rows in training: the workgroup holds the row in registers and writes the gradient for gout = 1 in the same
 //                          launch (one read and one write in all); the backward pass recomputes it only for another gout
 #include <string.h>
@@ -736,7 +736,7 @@ int check_args(const char* who, int dtype, int64_t rows, int v, int64_t pitch, c
     const size_t esz = dtype ? 2 : 4;
     if ((uintptr_t)logits % esz || (uintptr_t)teacher % (t_dtype ? 2 : 4) || (uintptr_t)index % (i_dtype == 2 ? 8 : 4))
         return bad("address is not a multiple of the element size");
-    if (!(temperature > 0.0f) || !(temperature < INFINITY)) return bad("temperature must be positive and finite");
+    if (!(temperature >= 1e-6f && temperature <= 1e6f)) return bad("temperature must be in 1e-6 .. 1e6");
     if (!(weight - weight == 0.0f)) return bad("weight must be finite");
     if (reduction < 0 || reduction > 2) return bad("unknown reduction");
     return 0;
@@ -762,7 +762,9 @@ void fill(DistParams& p, const Plan& q, int dtype, int64_t rows, int v, int64_t 
     memset(&p, 0, sizeof(p));
     p.z = (const char*)logits; p.t = (const char*)teacher; p.idx = (const char*)index;
     p.rows = rows; p.v = v; p.k = k; p.zp = pitch * (dtype ? 2 : 4); p.t_bf16 = t_dtype; p.i64 = i_dtype == 2; p.red = reduction;
-    p.L = q.L; p.nparts = q.blocks; p.wl = weight * temperature * temperature; p.wg = weight * temperature; p.inv_t = 1.0f / temperature; p.c = (float)(1.4426950408889634 / (double)temperature);
+    p.L = q.L; p.nparts = q.blocks;
+    p.wl = weight * temperature * temperature; p.wg = weight * temperature;
+    p.inv_t = 1.0f / temperature; p.c = (float)(1.4426950408889634 / (double)temperature);
     p.sums = (double*)saved; p.part = p.sums + 2;
     p.counts = p.part + 2 * q.parts;
     const int64_t c = (rows + 63) / 64;
@@ -788,7 +790,7 @@ int mi_distill_loss_fwd(int dtype, int64_t rows, int v, int64_t pitch, const voi
                         void* saved, void* stream) {
     if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction)) return r;
     MI_CHECK(loss && saved, "null argument");
-    MI_CHECK((uintptr_t)saved % 8 == 0 && (uintptr_t)loss % 4 == 0, "saved or loss is not aligned");
+    MI_CHECK((uintptr_t)saved % 16 == 0 && (uintptr_t)loss % 4 == 0, "saved or loss is not aligned");
     const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);
     DistParams p;
     fill(p, q, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction, saved);
@@ -827,7 +829,7 @@ int mi_distill_loss_step(int dtype, int64_t rows, int v, int64_t pitch, const vo
                          void* saved, int64_t dpitch, void* dlogits, void* stream) {
     if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction)) return r;
     MI_CHECK(loss && saved && dlogits, "null argument");
-    MI_CHECK((uintptr_t)saved % 8 == 0 && (uintptr_t)loss % 4 == 0, "saved or loss is not aligned");
+    MI_CHECK((uintptr_t)saved % 16 == 0 && (uintptr_t)loss % 4 == 0, "saved or loss is not aligned");
     MI_CHECK(dpitch >= v, "pitch of the gradient must cover the classes");
     MI_CHECK((uintptr_t)dlogits % (dtype ? 2 : 4) == 0, "address is not a multiple of the element size");
     MI_CHECK(mi_distill_loss_step_ready(dtype, rows, v, k, reduction), "not for these sizes or this reduction (mi_distill_loss_step_ready)");
@@ -866,7 +868,7 @@ int mi_distill_loss_bwd(int dtype, int64_t rows, int v, int64_t pitch, const voi
                         const float* grad_out, const void* saved, int after_step, int64_t dpitch, void* dlogits, void* stream) {
     if (int r = check_args(__func__, dtype, rows, v, pitch, logits, k, teacher_dtype, teacher, index_dtype, index, temperature, weight, reduction)) return r;
     MI_CHECK(grad_out && saved && dlogits, "null argument");
-    MI_CHECK((uintptr_t)saved % 8 == 0 && (uintptr_t)grad_out % 4 == 0, "saved or grad_out is not aligned");
+    MI_CHECK((uintptr_t)saved % 16 == 0 && (uintptr_t)grad_out % 4 == 0, "saved or grad_out is not aligned");
     MI_CHECK(dpitch >= v, "pitch of the gradient must cover the classes");
     MI_CHECK((uintptr_t)dlogits % (dtype ? 2 : 4) == 0, "address is not a multiple of the element size");
     const Plan q = plan_of(dtype ? 2 : 4, rows, v, k);

@@ -10,8 +10,7 @@
 // Thread layout of every kernel: a pixel is C / VEC vectors of up to 16 bytes; a sweep of the workgroup covers `rows`
 // pixels x `cols` vectors, and a thread keeps its vector column for all its pixels, so that the constants of its
 // channels live in registers.  VEC is the widest vector that the channel count, the pitches and the addresses of all
-// tensors of the call allow (odd channel counts go element by element: neighbouring lanes still read neighbouring
-// addresses).
+// tensors of the call allow; dense tensors of odd channel counts go in runs of VEC pixels (see Runs).
 //
 // Sums: a thread adds fp32 differences from its own first value (at most CHUNK of them), so that a mean far from zero
 // does not cancel; from there on everything is fp64 plain sums, joined in a fixed order (no atomics).
@@ -888,7 +887,7 @@ int splits(int esz, int nb, int64_t npix, int c, int groups, int wgs) {
 // Small images: slabs of whole groups at least 64 bytes wide, held by 256 threads with at most `most` vectors each.
 // (one image of 16 x 16 x 256 bf16: 6.7 us of kernel against 4.5 + 7.5 in two passes.)
 struct Small { bool ok; int groups, slabs, nv; };
-Small small_of(int esz, int vec, int64_t npix, int c, int groups, int most) {
+Small small_of(int esz, int vec, int nb, int64_t npix, int c, int groups, int most) {
     const int cg = c / groups;
     Small q = {false, 1, 1, 1};
     if (npix > 65536) return q;
@@ -898,6 +897,7 @@ Small small_of(int esz, int vec, int64_t npix, int c, int groups, int most) {
     const int per = (int)((npix + TPB / cols - 1) / (TPB / cols));
     if (per > most) return q;
     q.slabs = (groups + q.groups - 1) / q.groups;
+    if ((int64_t)nb * q.slabs > 1 << 23) return q;                    // a launch has at most 2^32 threads
     while (q.nv < per) q.nv *= 2;
     q.ok = true;
     return q;
@@ -1009,7 +1009,7 @@ int mi_groupnorm_act_fwd(int dtype, int nb, int64_t npix, int c, int groups, con
     p.nb = nb; p.npix = npix; p.c = c; p.groups = groups; p.cg = c / groups; p.act = act; p.eps = eps;
     p.cr = c; p.rep = 1; p.count = (double)npix * p.cg;
     hipStream_t st = (hipStream_t)stream;
-    const Small q = small_of(esz, vec, npix, c, groups, 8);
+    const Small q = small_of(esz, vec, nb, npix, c, groups, 8);
     if (q.ok) {
         p.S = q.slabs; p.B = q.groups;
         GN_SMALL(gn_small_fwd_kernel, nb * p.S, q.groups * 2 * sizeof(double));
@@ -1044,7 +1044,7 @@ int mi_groupnorm_act_bwd(int dtype, int nb, int64_t npix, int c, int groups, con
     p.cr = c; p.rep = 1; p.count = (double)npix * p.cg;
     hipStream_t st = (hipStream_t)stream;
     const int joins = dweight || dbias || dalpha ? (c + JC - 1) / JC + (dalpha ? 1 : 0) : 0;
-    const Small q = small_of(esz, vec, npix, c, groups, 8);
+    const Small q = small_of(esz, vec, nb, npix, c, groups, 8);
     if (q.ok) {
         p.S = q.slabs; p.B = q.groups;
         p.part_c = (double*)workspace;

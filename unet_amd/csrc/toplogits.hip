@@ -455,11 +455,12 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         while (q.nv < NVMAX && q.nv * q.L < nvec) q.nv *= 2;
         per = TPB / q.L;
     } else {
-        // Few rows: 1024 threads each.  Else few enough threads that each has some vectors, as many rows as possible being on their
+        // Few rows: up to 1024 threads each, one vector at least (else groups without any would leave fewer than k maxima).  Else few
+        // enough threads that each has some vectors, as many rows as possible being on their
         // way: 30000 x 4000 bf16, 8 of them: 128 threads 83 us, 256 98, 512 166; 2048 x 50001, 32: 128 threads 78, 256 64, 512 63.
         // G maxima, at least 1.5 per entry: the classes gathered are then few (G log(G / (G - k)) of them on average: 44 for k = 32, 355 for 256)
         q.kind = LONG;
-        q.T = rows < 512 ? 1024 : nvec <= 1024 && k <= 85 ? 128 : nvec <= 4096 && k <= 170 ? 256 : 512;
+        q.T = rows < 512 ? (nvec >= 1024 ? 1024 : nvec >= 512 || k > 170 ? 512 : 256) : nvec <= 1024 && k <= 85 ? 128 : nvec <= 4096 && k <= 170 ? 256 : 512;
         q.G = 64;
         while (q.G < q.T && q.G < k + k / 2) q.G *= 2;
     }

@@ -191,8 +191,8 @@ class TopLogitDistillationLoss(nn.Module):
     def __init__(self, temperature=1.0, reduction="mean", weight=1.0):
         super().__init__()
         temperature, weight = float(temperature), float(weight)
-        if not 0.0 < temperature < float("inf"):
-            raise ValueError(f"temperature must be positive and finite, got {temperature}")
+        if not 1e-6 <= temperature <= 1e6:
+            raise ValueError(f"temperature must be in 1e-6 .. 1e6, got {temperature}")
         if not abs(weight) < float("inf"):
             raise ValueError(f"weight must be finite, got {weight}")
         if reduction not in _REDUCTION:
