@@ -216,7 +216,7 @@ _HERE = _Here()
 
 def on_device(device):
     """Context in which launches go to ``device``: a kernel goes to the process's current device, whatever the stream."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 LABEL_DTYPES = None

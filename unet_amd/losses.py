@@ -137,11 +137,32 @@ def _distill_call(logits, teacher, index, temperature, weight, red, train):
             index.data_ptr(), temperature, weight, red, loss.data_ptr(), saved.data_ptr())
     with _lib.on_device(dev):
         if train and in_one:
-            dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
+            dz = z.new_empty(z.shape)
             _lib.check(lib.mi_distill_loss_step(*args, v, dz.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_step")
             return loss, saved, dz
         _lib.check(lib.mi_distill_loss_fwd(*args, _lib.stream_of(dev)), "mi_distill_loss_fwd")
     return loss, saved, None
+
+
+def _distill_gradient(ctx, gout):
+    logits, teacher, index, saved = ctx.saved_tensors
+    temperature, weight, red = ctx.cfg
+    lib, dev = _lib.load(), logits.device
+    z, pitch = _pixels(logits, "input")
+    v, k = z.shape[-1], index.shape[-1]
+    dz, ctx.dz = ctx.dz, None        # given away by the first backward call
+    done = dz is not None
+    if not done:
+        dz = z.new_empty(z.shape)
+    g = gout if gout.dtype == torch.float32 and gout.is_contiguous() else gout.contiguous().float()
+    with _lib.on_device(dev):
+        _lib.check(lib.mi_distill_loss_bwd(_DT[z.dtype], index.numel() // k, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(),
+                                           _INDEX[index.dtype], index.data_ptr(), temperature, weight, red, g.data_ptr(), saved.data_ptr(),
+                                           1 if done else 0, v, dz.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_bwd")
+    return dz, None, None, None, None, None
+
+
+_distill_gradient_once = torch.autograd.function.once_differentiable(_distill_gradient)
 
 
 class _DistillFunction(torch.autograd.Function):
@@ -153,23 +174,9 @@ class _DistillFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gout):
-        logits, teacher, index, saved = ctx.saved_tensors
-        temperature, weight, red = ctx.cfg
-        lib, dev = _lib.load(), logits.device
-        z, pitch = _pixels(logits, "input")
-        v, k = z.shape[-1], index.shape[-1]
-        dz, ctx.dz = ctx.dz, None        # given away by the first backward call
-        done = dz is not None
-        if not done:
-            dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
-        g = gout if gout.dtype == torch.float32 and gout.is_contiguous() else gout.contiguous().float()
-        with _lib.on_device(dev):
-            _lib.check(lib.mi_distill_loss_bwd(_DT[z.dtype], index.numel() // k, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(),
-                                               _INDEX[index.dtype], index.data_ptr(), temperature, weight, red, g.data_ptr(), saved.data_ptr(),
-                                               1 if done else 0, v, dz.data_ptr(), _lib.stream_of(dev)), "mi_distill_loss_bwd")
-        return dz, None, None, None, None, None
+        # only a graph of the gradient itself (create_graph) needs the refusal of a second derivative
+        return _distill_gradient_once(ctx, gout) if torch.is_grad_enabled() else _distill_gradient(ctx, gout)
 
 
 class TopLogitDistillationLoss(nn.Module):
@@ -217,7 +224,8 @@ class TopLogitDistillationLoss(nn.Module):
             raise ValueError(f"the teacher's lists are on {t.device} and {i.device}, expected {x.device}")
         if x.dtype not in _DT:
             x = x.float()
-        t = t.detach()
+        if t.requires_grad:
+            t = t.detach()
         if t.dtype not in _DT:
             t = t.float()
         red = _REDUCTION[self.reduction]
