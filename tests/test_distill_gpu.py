@@ -63,6 +63,19 @@ def test_top_logits(dev, mode, case):
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("k", range(1, 10))
+def test_top_logits_of_every_pattern(dev, mode, k):
+    """All rows of 16 zeros and ones: a network of exchanges that orders these orders everything."""
+    n = torch.arange(1 << 16)
+    bits = ((n[:, None] >> torch.arange(16)) & 1).to(DT[mode]).to(dev)
+    check_top(bits, k)
+    g = torch.Generator().manual_seed(k)
+    for v in (9, 23, 70, 300, 1100):
+        x = torch.rand(400, v, generator=g).argsort(-1).to(DT[mode]).to(dev)            # bf16: ties above 256
+        check_top(x, k)
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
 @pytest.mark.parametrize("v,k", [(16, 4), (300, 16), (2100, 24), (9000, 5)])
 def test_top_logits_of_special_values(dev, mode, v, k):
     g = torch.Generator().manual_seed(v)

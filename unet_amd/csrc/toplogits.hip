@@ -5,7 +5,7 @@
 // value and stands for "none".
 //
 // Bandwidth-bound: the rows have to be read once.
-//   top_short: lists of a few entries; L neighbouring lanes hold a row in registers and take the largest out k times
+//   top_short: lists of a few entries; L neighbouring lanes hold a row in registers and take the largest out k times, or order by networks
 //   top_wave : a wave holds the row; the k-th largest key is found bit by bit, by counting the keys from there on, the k classes
 //              are gathered in LDS (equal keys by ascending class) and placed by the number of full keys above their own
 //   top_long : a workgroup streams the row and keeps the largest key of every thread's part.  At least k classes lie at or above
@@ -33,8 +33,7 @@ struct TopParams {
 
 __device__ __forceinline__ unsigned key_of(float f) {
     const unsigned b = __float_as_uint(f + 0.0f);                  // -0 -> +0
-    if (f != f) return 0xffffffffu;
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return f != f ? 0xffffffffu : b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
 typedef unsigned long long u64;
 __device__ __forceinline__ u64 full_key(unsigned key, int i) { return ((u64)key << 32) | (unsigned)~i; }
@@ -66,15 +65,48 @@ __device__ __forceinline__ void load_keys(const char* x, int v, int L, int l, un
     }
 }
 
+// Networks on words: a holds the larger one after swap_down.  sort_down: N = 4 or 8 words, largest first (merge exchanges of two sorted
+// halves); top_of_two: the N largest of two sorted lists, sorted, in a.
+__device__ __forceinline__ void swap_down(unsigned& a, unsigned& b) {
+    const unsigned hi = max(a, b), lo = min(a, b);
+    a = hi; b = lo;
+}
+__device__ __forceinline__ void sort4(unsigned* a) {
+    swap_down(a[0], a[1]); swap_down(a[2], a[3]);
+    swap_down(a[0], a[2]); swap_down(a[1], a[3]);
+    swap_down(a[1], a[2]);
+}
+__device__ __forceinline__ void sort8(unsigned* a) {
+    sort4(a); sort4(a + 4);
+    swap_down(a[0], a[4]); swap_down(a[1], a[5]); swap_down(a[2], a[6]); swap_down(a[3], a[7]);
+    swap_down(a[2], a[4]); swap_down(a[3], a[5]);
+    swap_down(a[1], a[2]); swap_down(a[3], a[4]); swap_down(a[5], a[6]);
+}
+template <int N>
+__device__ __forceinline__ void top_of_two(unsigned* a, const unsigned* b) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = max(a[i], b[N - 1 - i]);    // rises, then falls (or a rotation of that)
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!(i & o)) swap_down(a[i], a[i + o]);
+}
+
 // The classes found go through LDS (dynamic, [workgroup's rows][k]): the results of a wave's rows are one piece of the output and
 // leave it with neighbouring lanes at neighbouring addresses.
-// bf16: key and class fit one word, (key, 65535 - class), so that a maximum is one instruction.
-template <class TR, int NV>
+// bf16: key and class fit one word, (key, 65535 - class), so that a maximum is one instruction.  Lists of at most K = 4 or 8 come from
+// networks: 76 or 108 instructions for the 16 words of two vectors, where taking out costs 40 per entry.  K = 1: the maximum.  K = 0: taken out
+// one by one.  2097152 rows of 16 classes, bf16: 4 of them 31 us (3.8 TB/s; taken out 38), 1 of them 21.5 (23), 8 of them 40 (57); 50000 x 512,
+// 4 of them: 20 (25).  Bounded by instructions: 350 per row of 16 (630 taken out).
+template <class TR, int NV, int K>
 __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
-    extern __shared__ unsigned short found[];
-    const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    unsigned short* mine = found + (threadIdx.x / L) * p.k;
-    const unsigned short* waves = found + wave * (64 / L) * p.k;
+    // bf16: (key, class), the key's lower half being that of the value's sign; fp32: the class
+    extern __shared__ unsigned found[];
+    const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    unsigned* mine = found + (threadIdx.x / L) * p.k;
+    const unsigned* waves = found + wave * (64 / L) * p.k;
+    const float inv = 1.0f / (float)p.k;
     for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += (int64_t)gridDim.x * per) {
         const int64_t r = r0 + threadIdx.x / L;
         const char* x = p.x + (r < p.rows ? r : 0) * p.xp;
@@ -82,12 +114,43 @@ __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
         load_keys<TR, NV>(x, p.v, L, l, key);
         if constexpr (TR::ESZ == 2) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i) {
+                const int e0 = (i * L + l) * TR::VEC;
 #pragma unroll
-                for (int j = 0; j < TR::VEC; ++j) {
-                    const unsigned cls = 0xffffu - (unsigned)((i * L + l) * TR::VEC + j);
-                    key[i][j] = key[i][j] ? (key[i][j] & 0xffff0000u) | cls : 0u;
+                for (int j = 0; j < TR::VEC; ++j) key[i][j] = (key[i][j] & 0xffff0000u) | (0xffffu - (unsigned)(e0 + j));
+                if (e0 + TR::VEC > p.v) {
+#pragma unroll
+                    for (int j = 0; j < TR::VEC; ++j) key[i][j] = e0 + j < p.v ? key[i][j] : 0u;
                 }
+            }
+        }
+        if constexpr (K != 0) {
+            unsigned* top = key[0];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if constexpr (K == 1) {
+#pragma unroll
+                    for (int j = 1; j < TR::VEC; ++j) key[i][0] = max(key[i][0], key[i][j]);
+                } else if constexpr (K == 8) {
+                    sort8(key[i]);
+                } else {
+                    sort4(key[i]); sort4(key[i] + 4);
+                    top_of_two<K>(key[i], key[i] + 4);
+                }
+                if (i) top_of_two<K>(top, key[i]);
+            }
+            for (int o = L >> 1; o > 0; o >>= 1) {
+                unsigned other[K];
+#pragma unroll
+                for (int n = 0; n < K; ++n) other[n] = __shfl_xor(top[n], o, 64);
+                top_of_two<K>(top, other);
+            }
+            if (l == 0) {
+#pragma unroll
+                for (int n = 0; n < K; ++n)
+                    if (n < p.k) mine[n] = top[n] ^ 0xffffu;
+            }
+        } else if constexpr (TR::ESZ == 2) {
             for (int n = 0; n < p.k; ++n) {
                 unsigned best = 0;
 #pragma unroll
@@ -99,7 +162,7 @@ __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
                     for (int j = 0; j < TR::VEC; ++j) key[i][j] = key[i][j] == best ? 0u : key[i][j];
-                if (l == 0) mine[n] = (unsigned short)(0xffffu - (best & 0xffffu));
+                if (l == 0) mine[n] = best ^ 0xffffu;
             }
         } else {
             for (int n = 0; n < p.k; ++n) {
@@ -120,16 +183,32 @@ __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
 #pragma unroll
                     for (int j = 0; j < TR::VEC; ++j)
                         if ((i * L + l) * TR::VEC + j == at) key[i][j] = 0u;
-                if (l == 0) mine[n] = (unsigned short)at;
+                if (l == 0) mine[n] = (unsigned)at;
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         __builtin_amdgcn_wave_barrier();
-        const int64_t w0 = r0 + wave * (64 / L);                   // first row of the wave
+        // the wave's rows, from w0 on: their outputs are neighbours.  (o + 1/2) / k is at least 1/(2k) away from a whole number and
+        // off by less than 64 * 256 / k * 2^-22
+        typedef typename TR::elem E;
+        const int64_t w0 = r0 + wave * (64 / L);
         const int outs = (int)max((int64_t)0, min((int64_t)(64 / L), p.rows - w0)) * p.k;
+        const char* xw = p.x + w0 * p.xp;
+        E* val = reinterpret_cast<E*>(p.val) + w0 * p.k;
+        int* idx = p.idx + w0 * p.k;
         for (int o = lane; o < outs; o += 64) {
-            const int row = o / p.k;
-            emit<TR>(p, w0 + row, o - row * p.k, waves[o]);
+            const unsigned f = waves[o];
+            const int cls = (int)(f & 0xffffu);
+            auto value = [&] { return reinterpret_cast<const E*>(xw + (int)(((float)o + 0.5f) * inv) * p.xp)[cls]; };
+            if constexpr (TR::ESZ == 2) {
+                const unsigned key = f >> 16;
+                E v = (E)(key & 0x8000u ? key ^ 0x8000u : ~key);
+                if (key == 0x8000u || key == 0xffffu) v = value();         // the value itself: a NaN keeps its bits, -0 its sign
+                val[o] = v;
+            } else {
+                val[o] = value();
+            }
+            idx[o] = cls;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         __builtin_amdgcn_wave_barrier();
@@ -439,7 +518,7 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
     int64_t per = 1;
     if (nvec <= 64 * NVMAX) {
         while (q.L < 64 && nvec > q.L * NVMAX) q.L *= 2;
-        // instructions of a wave per row: k times 3 (bf16) or 6 (fp32) per held class and 10 per exchange between lanes, for
+        // instructions of a wave per row: k times 3 (bf16) or 6 (fp32) per held class and 10 per exchange between lanes (networks: 44 or 70 per vector, 50 or 110 per exchange), for
         // 64 / L rows at once, against 4 per bit and 12 per held class (k <= 32, by the lanes' maxima) or 3 per held class and bit, and the placing.
         // 50000 rows of 512 bf16 classes, 16 of them: 50 us by search alone, 29 with the lanes' maxima; 100000 x 133 fp32, 5: 38 taken out
         int n1 = 1, n2 = 1;
@@ -449,8 +528,9 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         int lg = 0;
         while ((1 << lg) < q.L) ++lg;
         q.by_lanes = k <= 32 && 2 * nvec >= 3 * k;                 // enough lanes hold something
-        const int64_t take = ((int64_t)k * ((esz == 2 ? 3 : 6) * e1 + 10 * lg + 8) + 8 * e1) * q.L / 64, search = q.by_lanes ? 8 * esz * 4 + 12 * e2 + 6 * k + 100 : 8 * esz * 3 * e2 + 100 + (int64_t)k * ((k + 63) / 64) * 4;
-        q.kind = take <= search && k <= 32 ? SHORT : WAVE;             // 32: 16 KB of LDS
+        const int nets = esz == 2 && k <= 8 ? k <= 4 ? n1 * 44 + lg * 50 : n1 * 70 + lg * 110 : 0;
+        const int64_t take = ((nets ? nets : (int64_t)k * ((esz == 2 ? 3 : 6) * e1 + 10 * lg + 8)) + 8 * e1) * q.L / 64, search = q.by_lanes ? 8 * esz * 4 + 12 * e2 + 6 * k + 100 : 8 * esz * 3 * e2 + 100 + (int64_t)k * ((k + 63) / 64) * 4;
+        q.kind = take <= search && k <= 32 ? SHORT : WAVE;             // 32: 32 KB of LDS
         if (q.kind == WAVE) q.L = 64;
         while (q.nv < NVMAX && q.nv * q.L < nvec) q.nv *= 2;
         per = TPB / q.L;
@@ -469,6 +549,13 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
     return q;
 }
 
+#define SHORT_NV(T, K)                                                                            \
+    do {                                                                                       \
+        const size_t lds = TPB / q.L * k * 4;                                                    \
+        if (q.nv == 1) top_short<T, 1, K><<<q.blocks, TPB, lds, st>>>(p);                        \
+        else if (q.nv == 2) top_short<T, 2, K><<<q.blocks, TPB, lds, st>>>(p);                   \
+        else top_short<T, 4, K><<<q.blocks, TPB, lds, st>>>(p);                                  \
+    } while (0)
 #define NV_LAUNCH(KERN, lds)                                                                      \
     do {                                                                                       \
         if (dtype == 1) {                                                                      \
@@ -499,7 +586,11 @@ extern "C" int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, cons
     p.rows = rows; p.xp = pitch * (int64_t)esz; p.v = v; p.k = k; p.L = q.L; p.G = q.G; p.by_lanes = q.by_lanes;
     hipStream_t st = (hipStream_t)stream;
     if (q.kind == SHORT) {
-        NV_LAUNCH(top_short, TPB / q.L * k * 2);
+        if (dtype == 0) SHORT_NV(F32, 0);
+        else if (k == 1) SHORT_NV(BF16, 1);
+        else if (k <= 4) SHORT_NV(BF16, 4);
+        else if (k <= 8) SHORT_NV(BF16, 8);
+        else SHORT_NV(BF16, 0);
     } else if (q.kind == WAVE) {
         NV_LAUNCH(top_wave, 0);
     } else if (q.T == 128) {
