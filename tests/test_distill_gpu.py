@@ -48,7 +48,8 @@ def check_top(x, k):
 TOP = [(1, 1, 1), (7, 2, 2), (300, 3, 2), (300, 16, 4), (65, 16, 16), (130, 21, 5), (33, 64, 64), (40, 133, 8), (9, 255, 255), (5, 256, 256),
        (17, 257, 17), (6, 512, 16), (6, 513, 40), (5, 1024, 100), (5, 1025, 16), (5, 1025, 200), (4, 2048, 16), (4, 2049, 3), (3, 5000, 256), (2, 50001, 32),
        (1, 128000, 64), (1, 4097, 1), (600, 2100, 20), (520, 4200, 100), (513, 20000, 70), (513, 40000, 200), (3, 70000, 256), (2, 140000, 256), (2, 2049, 256), (300, 176, 17), (40, 700, 130), (5, 2100, 24), (5, 2100, 200), (5, 4200, 60),
-       (5, 9000, 42)]
+       (5, 9000, 42), (9, 1025, 85), (600, 1025, 85), (9, 1030, 86), (7, 1999, 64), (12, 517, 33), (600, 1025, 1), (520, 10241, 9), (520, 20500, 171),
+       (520, 100001, 5)]
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])
@@ -104,6 +105,17 @@ def test_top_logits_of_views(dev, mode):
     check_top(wide[0, 0, :1].expand(7, 40), 5)
     v, i = ops.top_logits(wide[:0], 3)
     assert v.shape == (0, 5, 7, 3) and i.shape == (0, 5, 7, 3)
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+def test_top_logits_of_long_views(dev, mode):
+    """Rows that begin at any element, with the largest classes first and last."""
+    g = torch.Generator().manual_seed(3)
+    wide = torch.randn(5, 9007, generator=g)
+    for lo, hi in ((0, 9007), (1, 9007), (1, 9001), (2, 9007), (3, 1030), (1, 2050), (5, 8199)):
+        x = wide.clone()
+        x[:, lo], x[:, hi - 1] = 9.0, 9.0
+        check_top(x.to(DT[mode]).to(dev)[:, lo:hi], 20)
 
 
 def test_top_logits_refusals(dev):

@@ -13,6 +13,7 @@
 //              (from L2), the classes from there on are gathered in LDS and placed.  Rows with so many equal values that they do
 //              not fit get the exact k-th largest key, the classes above it and the first ones at it
 #include <string.h>
+#include <type_traits>
 
 #include "rows.h"
 #include "../../include/unet_mi355.h"
@@ -227,6 +228,19 @@ __device__ __forceinline__ int lanes_before(int v, int& all) {
     all = __shfl(s, 63, 64);
     return s - v;
 }
+// how many of n full keys in LDS lie above f: eight reads on their way at a time (30000 x 4000 bf16, 64 of them: 131 -> 100 us)
+__device__ __forceinline__ int above(const u64* list, int n, u64 f) {
+    int place = 0, c = 0;
+    for (; c + 8 <= n; c += 8) {
+        ulonglong2 y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) y[u] = *reinterpret_cast<const ulonglong2*>(list + c + 2 * u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) place += (y[u].x > f ? 1 : 0) + (y[u].y > f ? 1 : 0);
+    }
+    for (; c < n; ++c) place += list[c] > f ? 1 : 0;
+    return place;
+}
 // the k largest of n full keys in LDS to their places, by one wave
 template <class TR>
 __device__ __forceinline__ void place_all(const TopParams& p, int64_t r, int l, const u64* mine, int n) {
@@ -234,9 +248,7 @@ __device__ __forceinline__ void place_all(const TopParams& p, int64_t r, int l, 
     __builtin_amdgcn_wave_barrier();
     for (int a = l; a < n; a += 64) {
         const u64 f = mine[a];
-        int place = 0;
-#pragma unroll 4
-        for (int b = 0; b < n; ++b) place += mine[b] > f ? 1 : 0;
+        const int place = above(mine, n, f);
         if (place < p.k) emit<TR>(p, r, place, (int)~(unsigned)f);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
@@ -245,7 +257,7 @@ __device__ __forceinline__ void place_all(const TopParams& p, int64_t r, int l, 
 
 template <class TR, int NV>
 __global__ __launch_bounds__(TPB) void top_wave(TopParams p) {
-    __shared__ u64 list[TPB / 64][MAX_K];
+    __shared__ alignas(16) u64 list[TPB / 64][MAX_K];
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
     u64* mine = list[w];
     for (int64_t r = (int64_t)blockIdx.x * (TPB / 64) + w; r < p.rows; r += (int64_t)gridDim.x * (TPB / 64)) {
@@ -443,25 +455,45 @@ __device__ __noinline__ void gather_ties(const char* x, int v, int k, unsigned t
 template <class TR, int T>
 __global__ __launch_bounds__(T) void top_long(TopParams p) {
     constexpr int CAP = T <= 512 ? 4 * T : 2048;                   // classes gathered, 12 times the usual number
-    __shared__ u64 cand[CAP];
+    __shared__ alignas(16) u64 cand[CAP];
     __shared__ unsigned top[T], thr_s;
     __shared__ unsigned short hot[T];
     __shared__ int count_s, hot_s, sm[T / 64];
-    const int tid = threadIdx.x, nv = p.v / TR::VEC, per = (nv + T - 1) / T, et = nv * TR::VEC + tid;
+    const int tid = threadIdx.x;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const char* x = p.x + r * p.xp;
-        constexpr int UN = 8;                                      // vectors in flight per thread
+        // Vectors begin at a word: in between, a load takes longer (2048 rows of 50001 bf16 classes 58 us, of 50002 48).  The class in front
+        // and those behind the last vector, fewer than a vector's worth, belong to a thread each.
+        const int head = TR::ESZ == 2 ? (int)((uintptr_t)x >> 1) & 1 : 0, nv = (p.v - head) / TR::VEC, per = (nv + T - 1) / T;
+        const int et = head && tid == T - 1 ? 0 : head + nv * TR::VEC + tid;
+        const char* xv = x + head * TR::ESZ;
+        constexpr int UN = 8;                                      // vectors in flight per thread; few at the end cost most (8000 x 16000: 88 -> 71 us)
         BestOf<TR> b;
         int i = tid;
-        for (; i + (UN - 1) * T < nv; i += UN * T) {
-            uint4 raw[UN];
+        auto batch = [&](auto nu) {
+            constexpr int N = decltype(nu)::value;
+            uint4 raw[N];
 #pragma unroll
-            for (int u = 0; u < UN; ++u) raw[u] = ld_any<TR>(x + (int64_t)(i + u * T) * 16);
+            for (int u = 0; u < N; ++u) raw[u] = ld_any<TR>(xv + (int64_t)(i + u * T) * 16);
 #pragma unroll
-            for (int u = 0; u < UN; ++u) best_vec(b, raw[u]);
+            for (int u = 0; u < N; ++u) best_vec(b, raw[u]);
+            i += N * T;
+        };
+        while (i + (UN - 1) * T < nv) batch(std::integral_constant<int, UN>{});
+        if (i + 4 * T < nv) {                                      // 5 to 7 more: all at once, the last vector standing in for those behind the end
+            uint4 raw[UN - 1];
+#pragma unroll
+            for (int u = 0; u < UN - 1; ++u) raw[u] = ld_any<TR>(xv + (int64_t)min(i + u * T, nv - 1) * 16);
+#pragma unroll
+            for (int u = 0; u < UN - 1; ++u)
+                if (i + u * T < nv) best_vec(b, raw[u]);
+        } else if (i + 3 * T < nv) {
+            batch(std::integral_constant<int, 4>{});
+        } else {
+            if (i + T < nv) batch(std::integral_constant<int, 2>{});
+            if (i < nv) batch(std::integral_constant<int, 1>{});
         }
-        for (; i < nv; i += T) best_vec(b, ld_any<TR>(x + (int64_t)i * 16));
-        const unsigned tail = et < p.v ? key_of(ld_one<TR>(x, et)) : 0u;      // fewer than a vector's worth
+        const unsigned tail = et < p.v ? key_of(ld_one<TR>(x, et)) : 0u;
         const unsigned best = max(b.key(), tail);
         // G maxima of T / G neighbouring threads each
         unsigned group = best;
@@ -489,9 +521,9 @@ __global__ __launch_bounds__(T) void top_long(TopParams p) {
             const int at = (m % per) * T + hot[m / per];
             if (at < nv) {
                 float y[TR::VEC];
-                unpack_vec<TR>(ld_any<TR>(x + (int64_t)at * 16), y);
+                unpack_vec<TR>(ld_any<TR>(xv + (int64_t)at * 16), y);
 #pragma unroll
-                for (int j = 0; j < TR::VEC; ++j) add(key_of(y[j]), at * TR::VEC + j);
+                for (int j = 0; j < TR::VEC; ++j) add(key_of(y[j]), head + at * TR::VEC + j);
             }
         }
         __syncthreads();
@@ -502,8 +534,7 @@ __global__ __launch_bounds__(T) void top_long(TopParams p) {
         }
         for (int a = tid; a < n; a += T) {
             const u64 f = cand[a];
-            int place = 0;
-            for (int c = 0; c < n; ++c) place += cand[c] > f ? 1 : 0;
+            const int place = above(cand, n, f);
             if (place < p.k) emit<TR>(p, r, place, (int)~(unsigned)f);
         }
         __syncthreads();
@@ -516,7 +547,10 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
     Plan q = {SHORT, 1, 1, TPB, 0, 0, 0};
     const int vec = 16 / esz, nvec = (v + vec - 1) / vec;
     int64_t per = 1;
-    if (nvec <= 64 * NVMAX) {
+    // From 129 vectors on, lists that a wave would search out bit by bit (and all bf16 lists up to 85) go by workgroups of 128: 20000 rows of 2000
+    // bf16 classes, 64 of them: 90 -> 51 us, 8 of them 39 -> 35; of 1000 fp32 classes, 64: 65 -> 45, but 16: 28 -> 34.
+    const bool small_groups = nvec > 128 && nvec <= 64 * NVMAX && k <= 85 && (esz == 2 || k > 32);
+    if (nvec <= 64 * NVMAX && !small_groups) {
         while (q.L < 64 && nvec > q.L * NVMAX) q.L *= 2;
         // instructions of a wave per row: k times 3 (bf16) or 6 (fp32) per held class and 10 per exchange between lanes (networks: 44 or 70 per vector, 50 or 110 per exchange), for
         // 64 / L rows at once, against 4 per bit and 12 per held class (k <= 32, by the lanes' maxima) or 3 per held class and bit, and the placing.
@@ -535,12 +569,13 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         while (q.nv < NVMAX && q.nv * q.L < nvec) q.nv *= 2;
         per = TPB / q.L;
     } else {
-        // Few rows: up to 1024 threads each, one vector at least (else groups without any would leave fewer than k maxima).  Else few
-        // enough threads that each has some vectors, as many rows as possible being on their
-        // way: 30000 x 4000 bf16, 8 of them: 128 threads 83 us, 256 98, 512 166; 2048 x 50001, 32: 128 threads 78, 256 64, 512 63.
+        // Few rows: up to 1024 threads each, one vector at least (else groups without any would leave fewer than k maxima).  Else about
+        // eight vectors a thread, all on their way at once, as many rows as possible beside each other: us with 128 / 256 / 512 / 1024 threads
+        // 30000 x 4000 bf16, 8 of them: 63 / 93 / - / -, 15000 x 8000: 49 / 64 / 97 / -, 8000 x 16000, 32: 78 / 64 / 79 / 176,
+        // 4000 x 32000: 80 / 68 / 58 / 109, 2048 x 50001: 76 / 63 / 58 / 82, 1000 x 131072: 86 / 74 / 64 / 59.
         // G maxima, at least 1.5 per entry: the classes gathered are then few (G log(G / (G - k)) of them on average: 44 for k = 32, 355 for 256)
         q.kind = LONG;
-        q.T = rows < 512 ? (nvec >= 1024 ? 1024 : nvec >= 512 || k > 170 ? 512 : 256) : nvec <= 1024 && k <= 85 ? 128 : nvec <= 4096 && k <= 170 ? 256 : 512;
+        q.T = small_groups ? 128 : rows < 512 ? (nvec >= 1024 ? 1024 : nvec >= 512 || k > 170 ? 512 : 256) : nvec <= 1280 && k <= 85 ? 128 : nvec <= 2560 && k <= 170 ? 256 : nvec <= 12288 ? 512 : 1024;
         q.G = 64;
         while (q.G < q.T && q.G < k + k / 2) q.G *= 2;
     }
