@@ -227,6 +227,42 @@ def test_loss_and_gradient(dev, mode, case):
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,v", [(513, 2600), (513, 4700), (513, 5900), (513, 7001), (513, 9003), (513, 11111), (513, 13001), (513, 19501), (513, 23502),
+                                    (513, 28003), (513, 32775), (513, 39999), (513, 48001), (513, 56003), (514, 66001), (3, 45001), (3, 60007), (2, 90001), (2, 105003)])
+def test_step_at_every_number_of_vectors(dev, mode, rows, v):
+    """Few rows have a list: theirs is the loss, and the gradient of all others is exactly 0."""
+    g = torch.Generator().manual_seed(v)
+    gd = torch.Generator(device=dev).manual_seed(v)
+    z = (torch.randn(rows, v, generator=gd, device=dev) * 3).to(DT[mode]).requires_grad_(True)
+    some = sorted({0, 1, rows // 2, rows - 1})
+    t, i = lists(rows, v, 7, g, torch.device("cpu"), ragged=False)
+    i[:, 0], i[:, 1] = 0, v - 1                            # the first class and the last
+    keep = torch.zeros(rows, 1, dtype=torch.bool)
+    keep[some] = True
+    i = torch.where(keep, i, torch.full_like(i, -1))
+    t, i = t.to(dev), i.to(dev)
+    out = unet_amd.TopLogitDistillationLoss(1.5, "mean")(z, t, i)
+    (dz,) = torch.autograd.grad(out, z)
+    loss, tol, ref, tol_dz = definition(z[some], t[some], i[some], 1.5, "mean", torch.ones(()))
+    assert (out.detach().double().cpu() - loss).abs() <= tol
+    bound = tol_dz * 1.01 + HALF_STEP[mode] * ref.abs() + 1e-37
+    err = (dz[some].double().cpu() - ref).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+    assert int((dz != 0).any(-1).sum()) == len(some) and not dz.isnan().any()
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+def test_long_rows_at_any_offset(dev, mode):
+    g = torch.Generator().manual_seed(8)
+    wide = (torch.randn(6, 9001, generator=g) * 2).to(DT[mode]).to(dev)
+    for lo, hi in ((0, 9001), (1, 9001), (1, 3000), (2, 2101), (3, 8201), (33, 2090), (63, 8999)):
+        z = wide[:, lo:hi]
+        t, i = lists(6, hi - lo, 5, g, dev)
+        check_loss(z, t, i, 1.0, "mean", mode, one=True)
+        check_loss(z, t, i, 2.0, "none", mode)
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
 @pytest.mark.parametrize("v", [16, 300, 4000])
 def test_masks_infinities_and_repeats(dev, mode, v):
     g = torch.Generator().manual_seed(v)
