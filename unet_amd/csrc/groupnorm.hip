@@ -870,14 +870,17 @@ __global__ __launch_bounds__(TPB) void gn_join_kernel(GnParams p) {
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
-// Splits of an image in both passes: FWD_WGS or BWD_WGS workgroups in all, at least 32 KB of the tensor per workgroup, and at
-// most 8192 pairs (128 KB, in L2) for a workgroup of the second pass to join.  32 x 256^2 x 32 bf16 forward with 1024 / 2048 / 4096
-// workgroups: 90.8 / 88.5 / 90.5 us; 32 x 256^2 x 16 backward, whose sums per workgroup cost more, with 256 / 512 / 1024 / 2048: 75.2 /
-// 72.5 / 76.6 / 82.0 (all before the second pass went past the caches).
-constexpr int FWD_WGS = 2048, BWD_WGS = 512;
-int splits(int esz, int nb, int64_t npix, int c, int groups, int wgs) {
+// Splits of an image in both passes: about two workgroups per compute unit in all, at least 32 KB of the tensor per workgroup, and at
+// most 8192 pairs (128 KB, in L2) for a workgroup of the second pass to join.  Every workgroup pays for its sums: 32 x 256^2 x 32 bf16
+// forward with 256 / 512 / 1024 / 2048 workgroups 77 / 72 / 74 / 77 us, 4 x 117^2 x 256 with 512 / 852 / 1704 of them 21 / 24 / 36;
+// 32 x 256^2 x 16 backward with 256 / 512 / 1024: 81 / 64 / 70.  One split less where the last round over the units would be nearly
+// empty: 5 x 200^2 x 64 forward 23.2 -> 21.1, backward 38 -> 34; 60 x 80^2 x 32 22.4 -> 19.2, 36 -> 32.
+constexpr int WGS = 512, UNITS = 256;
+int splits(int esz, int nb, int64_t npix, int c, int groups) {
     const int64_t bytes = npix * c * esz;
-    int64_t s = (wgs + nb - 1) / nb;
+    int64_t s = (WGS + nb - 1) / nb;
+    auto load = [&](int64_t n) { return (n * nb + UNITS - 1) / UNITS; };       // n-ths of an image on the busiest unit
+    if (s > 1 && load(s - 1) * s < load(s) * (s - 1)) --s;
     s = s < bytes / 32768 ? s : bytes / 32768;
     s = s < 8192 / groups ? s : 8192 / groups;
     s = s < npix ? s : npix;
@@ -983,7 +986,7 @@ extern "C" {
 
 size_t mi_groupnorm_act_workspace_bytes(int dtype, int nb, int64_t npix, int c, int groups, int backward) {
     if (check_shape(__func__, dtype, nb, npix, c, groups)) return 0;
-    const size_t s = (size_t)nb * splits(dtype ? 2 : 4, nb, npix, c, groups, backward ? BWD_WGS : FWD_WGS);
+    const size_t s = (size_t)nb * splits(dtype ? 2 : 4, nb, npix, c, groups);
     // a small image's backward pass: [nb][c][2] and at most [nb][groups]
     return (s * groups * 2 + (backward ? s * c * 2 + s : 0)) * sizeof(double);
 }
@@ -1015,7 +1018,7 @@ int mi_groupnorm_act_fwd(int dtype, int nb, int64_t npix, int c, int groups, con
         GN_SMALL(gn_small_fwd_kernel, nb * p.S, q.groups * 2 * sizeof(double));
         return 0;
     }
-    p.S = p.B = splits(esz, nb, npix, c, groups, FWD_WGS);
+    p.S = p.B = splits(esz, nb, npix, c, groups);
     take_runs(p, esz, vec, dense);
     GN_LAUNCH(gn_stats_kernel, nb * p.S, groups * 2 * sizeof(double));
     GN_LAUNCH(gn_apply_kernel, nb * p.B, groups * 2 * sizeof(float));
@@ -1054,7 +1057,7 @@ int mi_groupnorm_act_bwd(int dtype, int nb, int64_t npix, int c, int groups, con
         MI_HIP(hipGetLastError());
         return 0;
     }
-    p.S = p.B = splits(esz, nb, npix, c, groups, BWD_WGS);
+    p.S = p.B = splits(esz, nb, npix, c, groups);
     take_runs(p, esz, vec, dense);
     const size_t s = (size_t)nb * p.S;
     p.part = (double*)workspace;
