@@ -53,6 +53,13 @@ __device__ __forceinline__ int list_i(const DistParams& p, int64_t at) {
     return i >= 0 && i < p.v ? (int)i : -1;
 }
 
+// lanes that look at one list in distill_count
+__host__ __device__ inline int count_lanes(int k) {
+    int L = 1;
+    while (L < 64 && L < k) L *= 2;
+    return L;
+}
+
 // running maximum, sum and weighted gap of a list; natural units (to base 2 a student's class masked with the type's lowest
 // value would pass the end of fp32)
 struct ListSum {
@@ -533,16 +540,27 @@ __global__ __launch_bounds__(T) void distill_long_fwd(DistParams p) {
     if (p.red) block_part<T>(p, loss, count);
 }
 
-// rows with a used slot, per workgroup
-__global__ __launch_bounds__(64) void distill_count(DistParams p) {
-    double n = 0.0;
-    for (int64_t r = (int64_t)blockIdx.x * 64 + threadIdx.x; r < p.rows; r += (int64_t)gridDim.x * 64) {
+// rows with a used slot, per workgroup: up to 64 neighbouring lanes look at a row's list (4096 lists of 32: 7.6 -> 3.5 us, against a thread each)
+__global__ __launch_bounds__(TPB) void distill_count(DistParams p) {
+    __shared__ int sm[TPB / 64];
+    const int L = count_lanes(p.k), l = threadIdx.x & (L - 1), lane = threadIdx.x & 63;
+    int n = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * (TPB / L); r0 < p.rows; r0 += (int64_t)gridDim.x * (TPB / L)) {
+        const int64_t r = r0 + threadIdx.x / L;
         bool some = false;
-        for (int j = 0; j < p.k && !some; ++j) some = (list_i(p, r * p.k + j) >= 0) & (list_t(p, r * p.k + j) != -INFINITY);
-        n += some ? 1.0 : 0.0;
+        if (r < p.rows)
+            for (int j = l; j < p.k; j += L) some |= (list_i(p, r * p.k + j) >= 0) & (list_t(p, r * p.k + j) != -INFINITY);
+        const unsigned long long ball = __ballot(some), mine = L == 64 ? ball : ball >> (lane & ~(L - 1)) & ((1ull << L) - 1);
+        n += l == 0 && mine != 0 ? 1 : 0;
     }
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-    if (threadIdx.x == 0) p.counts[blockIdx.x] = n;
+    if (lane == 0) sm[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double all = 0.0;
+        for (int w = 0; w < TPB / 64; ++w) all += sm[w];
+        p.counts[blockIdx.x] = all;
+    }
 }
 
 // Loss and gradient for gout = 1 of long rows: up to NV vectors of the row in every thread's registers.  The list and the
@@ -805,7 +823,7 @@ void fill(DistParams& p, const Plan& q, int dtype, int64_t rows, int v, int64_t 
     p.inv_t = 1.0f / temperature; p.c = (float)(1.4426950408889634 / (double)temperature);
     p.sums = (double*)saved; p.part = p.sums + 2;
     p.counts = p.part + 2 * q.parts;
-    const int64_t c = (rows + 63) / 64;
+    const int64_t per = TPB / count_lanes(k), c = (rows + per - 1) / per;
     p.ncounts = (int)(c < COUNTS ? c : COUNTS);
     p.stat = (float2*)(p.counts + (q.is_long ? COUNTS : 0));
 }
@@ -878,7 +896,7 @@ int mi_distill_loss_step(int dtype, int64_t rows, int v, int64_t pitch, const vo
     hipStream_t st = (hipStream_t)stream;
     p.nparts = q.step_blocks;
     if (reduction == 1) {
-        distill_count<<<p.ncounts, 64, 0, st>>>(p);
+        distill_count<<<p.ncounts, TPB, 0, st>>>(p);
         MI_HIP(hipGetLastError());
     }
     bool launched = false;
