@@ -217,6 +217,8 @@ __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
 }
 
 // ---- a wave per row -----------------------------------------------------------------------------------------------------
+// 20000 rows of 1000 fp32 classes, 16 of them: 28 us (2.9 TB/s); 50000 x 512 bf16, 16: 29 us (1.9 TB/s): bounded by instructions, the
+// search among the lanes' maxima and the gathering.
 // exclusive prefix sum over the lanes; all: the sum
 __device__ __forceinline__ int lanes_before(int v, int& all) {
     int s = v;
@@ -337,6 +339,8 @@ __global__ __launch_bounds__(TPB) void top_wave(TopParams p) {
 }
 
 // ---- a workgroup per row ------------------------------------------------------------------------------------------------
+// Bound by the read where the lists are short against the row: 2048 x 50001 bf16, 32 of them 48 us, 4.3 TB/s; 15000 x 8000 fp32, 8 of them
+// 86 us, 5.6 TB/s.  200 of 50001: 76 us, half of it for the threads' parts read again and the placing.
 // Largest key of 16-byte vectors without making the keys: the bits of a value, with the lower ones turned over if it is
 // negative, order as signed numbers, two bf16 at a time, except that NaN with a sign lies below -inf; the smallest such number
 // tells whether there is one.  2.5 (bf16) and 5 (fp32) instructions per class instead of 9.
@@ -417,7 +421,7 @@ __device__ __forceinline__ int block_count(int c, int* sm) {
 
 // Exactly the k classes of a row with too many classes at or above key t: the k-th largest key by halving, the classes above
 // it in any order, and as many at it as are missing, by ascending class, T classes at a time until there are enough.
-template <class TR, int T>
+template <class TR, int T, bool ODD>                               // one for every caller: a shared one costs all of them 26 registers
 __device__ __noinline__ void gather_ties(const char* x, int v, int k, unsigned t, u64* cand, int* count, int* sm) {
     unsigned hi = 0xffffffffu;                                     // k classes reach t
     bool first = true;                                             // with many equal values t mostly is the key already
@@ -452,7 +456,7 @@ __device__ __noinline__ void gather_ties(const char* x, int v, int k, unsigned t
     __syncthreads();
 }
 
-template <class TR, int T>
+template <class TR, int T, bool ODD>
 __global__ __launch_bounds__(T) void top_long(TopParams p) {
     constexpr int CAP = T <= 512 ? 4 * T : 2048;                   // classes gathered, 12 times the usual number
     __shared__ alignas(16) u64 cand[CAP];
@@ -463,8 +467,9 @@ __global__ __launch_bounds__(T) void top_long(TopParams p) {
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const char* x = p.x + r * p.xp;
         // Vectors begin at a word: in between, a load takes longer (2048 rows of 50001 bf16 classes 58 us, of 50002 48).  The class in front
-        // and those behind the last vector, fewer than a vector's worth, belong to a thread each.
-        const int head = TR::ESZ == 2 ? (int)((uintptr_t)x >> 1) & 1 : 0, nv = (p.v - head) / TR::VEC, per = (nv + T - 1) / T;
+        // and those behind the last vector, fewer than a vector's worth, belong to a thread each.  ODD: some rows begin between words (where none
+        // does, the head costs 4 %: 4000 x 32000, 32 of them 58 -> 61).
+        const int head = ODD ? (int)((uintptr_t)x >> 1) & 1 : 0, nv = (p.v - head) / TR::VEC, per = (nv + T - 1) / T;
         const int et = head && tid == T - 1 ? 0 : head + nv * TR::VEC + tid;
         const char* xv = x + head * TR::ESZ;
         constexpr int UN = 8;                                      // vectors in flight per thread; few at the end cost most (8000 x 16000: 88 -> 71 us)
@@ -529,7 +534,7 @@ __global__ __launch_bounds__(T) void top_long(TopParams p) {
         __syncthreads();
         int n = count_s;
         if (n > CAP) {
-            gather_ties<TR, T>(x, p.v, p.k, t, cand, &count_s, sm);
+            gather_ties<TR, T, ODD>(x, p.v, p.k, t, cand, &count_s, sm);
             n = p.k;
         }
         for (int a = tid; a < n; a += T) {
@@ -572,7 +577,7 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         // Few rows: up to 1024 threads each, one vector at least (else groups without any would leave fewer than k maxima).  Else about
         // eight vectors a thread, all on their way at once, as many rows as possible beside each other: us with 128 / 256 / 512 / 1024 threads
         // 30000 x 4000 bf16, 8 of them: 63 / 93 / - / -, 15000 x 8000: 49 / 64 / 97 / -, 8000 x 16000, 32: 78 / 64 / 79 / 176,
-        // 4000 x 32000: 80 / 68 / 58 / 109, 2048 x 50001: 76 / 63 / 58 / 82, 1000 x 131072: 86 / 74 / 64 / 59.
+        // 4000 x 32000: 80 / 68 / 58 / 109, 2048 x 50001: 76 / 63 / 58 / 82 (49 since its vectors begin at words), 1000 x 131072: 86 / 74 / 64 / 59.
         // G maxima, at least 1.5 per entry: the classes gathered are then few (G log(G / (G - k)) of them on average: 44 for k = 32, 355 for 256)
         q.kind = LONG;
         q.T = small_groups ? 128 : rows < 512 ? (nvec >= 1024 ? 1024 : nvec >= 512 || k > 170 ? 512 : 256) : nvec <= 1280 && k <= 85 ? 128 : nvec <= 2560 && k <= 170 ? 256 : nvec <= 12288 ? 512 : 1024;
@@ -590,6 +595,13 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         if (q.nv == 1) top_short<T, 1, K><<<q.blocks, TPB, lds, st>>>(p);                        \
         else if (q.nv == 2) top_short<T, 2, K><<<q.blocks, TPB, lds, st>>>(p);                   \
         else top_short<T, 4, K><<<q.blocks, TPB, lds, st>>>(p);                                  \
+    } while (0)
+#define LONG_T(TR, ODD)                                                                           \
+    do {                                                                                       \
+        if (q.T == 128) top_long<TR, 128, ODD><<<q.blocks, 128, 0, st>>>(p);                     \
+        else if (q.T == 256) top_long<TR, 256, ODD><<<q.blocks, 256, 0, st>>>(p);                \
+        else if (q.T == 512) top_long<TR, 512, ODD><<<q.blocks, 512, 0, st>>>(p);                \
+        else top_long<TR, 1024, ODD><<<q.blocks, 1024, 0, st>>>(p);                              \
     } while (0)
 #define NV_LAUNCH(KERN, lds)                                                                      \
     do {                                                                                       \
@@ -628,18 +640,11 @@ extern "C" int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, cons
         else SHORT_NV(BF16, 0);
     } else if (q.kind == WAVE) {
         NV_LAUNCH(top_wave, 0);
-    } else if (q.T == 128) {
-        if (dtype == 1) top_long<BF16, 128><<<q.blocks, 128, 0, st>>>(p);
-        else top_long<F32, 128><<<q.blocks, 128, 0, st>>>(p);
-    } else if (q.T == 256) {
-        if (dtype == 1) top_long<BF16, 256><<<q.blocks, 256, 0, st>>>(p);
-        else top_long<F32, 256><<<q.blocks, 256, 0, st>>>(p);
-    } else if (q.T == 512) {
-        if (dtype == 1) top_long<BF16, 512><<<q.blocks, 512, 0, st>>>(p);
-        else top_long<F32, 512><<<q.blocks, 512, 0, st>>>(p);
     } else {
-        if (dtype == 1) top_long<BF16, 1024><<<q.blocks, 1024, 0, st>>>(p);
-        else top_long<F32, 1024><<<q.blocks, 1024, 0, st>>>(p);
+        const bool odd = esz == 2 && (pitch % 2 != 0 || (uintptr_t)logits % 4 != 0);
+        if (dtype == 0) LONG_T(F32, false);
+        else if (odd) LONG_T(BF16, true);
+        else LONG_T(BF16, false);
     }
     MI_HIP(hipGetLastError());
     return 0;
