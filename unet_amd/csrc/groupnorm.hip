@@ -560,7 +560,7 @@ __device__ __forceinline__ void spread_channels(const GnParams& p, double* sm, c
 }
 
 // ---- backward, pass 1: per (image, split) the channel sums of g and g xh, the group sums of w g and w g xh ----------
-// Bound by the reads of x and dy: 32 x 256^2 x 16 bf16 (134 MB) 32 us, 4.2 TB/s; 96^3 x 16 fp32 (113 MB) 24 us, 4.8 TB/s.
+// Bound by the reads of x and dy: 32 x 256^2 x 16 bf16 (134 MB) 32 us, 4.2 TB/s; 4 x 48^3 x 32 fp32 (113 MB) 25 us, 4.5 TB/s.
 template <class TR, int VEC>
 __global__ __launch_bounds__(TPB) void gn_bwd_reduce_kernel(GnParams p) {
     __shared__ double sm[2 * VEC * TPB];
