@@ -125,6 +125,9 @@ CASES = [  # N, spatial, C, groups, act, affine, residual, mean offset
     (1, (41, 43), 257, 1, "relu", True, False, 0.0),
     (2, (53, 37), 250, 125, "silu", False, False, 0.0),
     (2, (103, 101), 12, 2, "none", True, False, 0.0),
+    (3, (395, 397), 36, 3, "silu", True, False, 0.0),      # tens of MB whose pixels are a multiple of 8 bytes
+    (1, (397, 401), 54, 6, "gelu", True, True, 0.0),
+    (2, (45, 43), 36, 4, "prelu", True, False, 0.0),
 ]
 
 

@@ -937,11 +937,13 @@ int view_of(const char* who, const char* name, const mi_tensor* t, int64_t npix,
     return 0;
 }
 
-// Dense tensors of at most 256 channels whose widest vector has 2 or 4 bytes go in runs: backward of 8 x 200^2 x 33 bf16 61 -> 33 us,
-// fp32 73 -> 43, forward 29 -> 22 and 36 -> 29.  8-byte vectors stay as they are (8 x 200^2 x 36 bf16: 20.7 us, 22.7 in runs).
-void take_runs(GnParams& p, int esz, int& vec, bool dense) {
+// Dense tensors of at most 256 channels whose widest vector is shorter than 16 bytes go in runs: backward of 8 x 200^2 x 33 bf16 61 -> 33 us,
+// fp32 73 -> 43, of 64 x 200^2 x 36 bf16 (8 bytes) 212 -> 172; forward 29 -> 22, 36 -> 29, 121 -> 111.  Forward with 8-byte vectors from 32 MB on:
+// smaller ones lose with the folding of the runs (8 x 200^2 x 36: 21.1 -> 23.2; 4 x 200^2 x 50 fp32, 32 MB: 25.5 -> 25.0).
+void take_runs(GnParams& p, int esz, int& vec, bool dense, bool backward) {
     const int full = 16 / esz;
-    if (vec * esz >= 8 || !dense || p.c > TPB || p.npix < full) return;
+    if (vec == full || !dense || p.c > TPB || p.npix < full) return;
+    if (vec * esz == 8 && !backward && (int64_t)p.nb * p.npix * p.c * esz < 1 << 25) return;
     vec = p.rep = full;
     p.c *= full;
     p.tail = (int)(p.npix % full) * p.cr;
@@ -1025,7 +1027,7 @@ int mi_groupnorm_act_fwd(int dtype, int nb, int64_t npix, int c, int groups, con
         return 0;
     }
     p.S = p.B = splits(esz, nb, npix, c, groups);
-    take_runs(p, esz, vec, dense);
+    take_runs(p, esz, vec, dense, false);
     GN_LAUNCH(gn_stats_kernel, nb * p.S, groups * 2 * sizeof(double));
     GN_LAUNCH(gn_apply_kernel, nb * p.B, groups * 2 * sizeof(float));
     return 0;
@@ -1064,7 +1066,7 @@ int mi_groupnorm_act_bwd(int dtype, int nb, int64_t npix, int c, int groups, con
         return 0;
     }
     p.S = p.B = splits(esz, nb, npix, c, groups);
-    take_runs(p, esz, vec, dense);
+    take_runs(p, esz, vec, dense, true);
     const size_t s = (size_t)nb * p.S;
     p.part = (double*)workspace;
     p.part_c = p.part + s * groups * 2;
