@@ -316,6 +316,20 @@ def test_masks_infinities_and_repeats(dev, mode, v):
     assert torch.isnan(unet_amd.TopLogitDistillationLoss(reduction="none")(z3, t, i)[7])
 
 
+@pytest.mark.parametrize("i_dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("t_dtype", [torch.float32, torch.bfloat16])
+def test_lists_at_any_address(dev, t_dtype, i_dtype):
+    """Full and ragged lists whose tensors begin at any element."""
+    g = torch.Generator().manual_seed(12)
+    for rows, v, k in ((130, 16, 4), (77, 40, 8), (65, 300, 32), (9, 600, 256)):
+        z = (torch.randn(rows, v, generator=g) * 2).to(dev)
+        t, i = lists(rows, v, k, g, dev, t_dtype, i_dtype)
+        for off in (1, 2, 3):
+            tt = torch.zeros(rows * k + off, dtype=t_dtype, device=dev)[off:].view(rows, k).copy_(t)
+            ii = torch.zeros(rows * k + off, dtype=i_dtype, device=dev)[off:].view(rows, k).copy_(i)
+            check_loss(z, tt, ii, 1.0, "mean", "fp32")
+
+
 def test_nothing_to_learn_from(dev):
     for shape, v in (((6,), 16), ((2, 3, 4), 16), ((3,), 5000)):
         z = torch.randn(*shape, v, device=dev, requires_grad=True)

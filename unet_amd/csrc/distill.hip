@@ -171,14 +171,39 @@ __device__ __forceinline__ void block_part(const DistParams& p, double loss, dou
 }
 
 // ---- short rows -----------------------------------------------------------------------------------------------------
-// 524288 rows of 16 bf16 classes, 4 slots: forward 17 us (33 MB), backward 16 us (50 MB); 50001 x 133 fp32, 5 slots: 16 us (29 MB) and
+// 524288 rows of 16 bf16 classes, 4 slots: forward 15 us (33 MB), backward 15 us (50 MB); 50001 x 133 fp32, 5 slots: 16 us (29 MB) and
 // 22 us (55 MB).  Such calls are bounded by the latency of a row or two per thread (0.3 of the wave cycles issue); 2097152 rows of 16:
-// forward 51 us, 2.6 TB/s.
-// SL slots of a row's list in the registers of a lane: slot j of the list is slot j / L of lane j % L.  `fetch` only requests them.
+// forward 43 us, 3.1 TB/s.
+// SL slots of a row's list in the registers of a lane: slot j of the list is slot j / L of lane j % L, or slot j % 4 of lane j / 4 where every lane
+// has four (one or two loads in place of four: 2097152 rows of 16 bf16 classes, forward 51 -> 43 us).  `fetch` only requests them.
+typedef unsigned word4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned half4 __attribute__((ext_vector_type(2), aligned(2)));
 template <int SL>
 struct Slots {
     unsigned lo[SL], hi[SL], t[SL];
     __device__ __forceinline__ void fetch(const DistParams& p, int64_t r, bool in, int L, int l) {
+        if constexpr (SL == 4)
+            if (p.k == 4 * L) {                                    // every lane has four slots: its own are neighbours
+                const int64_t at = in ? r * p.k + 4 * l : 4 * l;
+                if (p.i64) {
+                    const word4 a = *reinterpret_cast<const word4*>(p.idx + at * 8), b = *reinterpret_cast<const word4*>(p.idx + at * 8 + 16);
+                    lo[0] = a.x; hi[0] = a.y; lo[1] = a.z; hi[1] = a.w;
+                    lo[2] = b.x; hi[2] = b.y; lo[3] = b.z; hi[3] = b.w;
+                } else {
+                    const word4 a = *reinterpret_cast<const word4*>(p.idx + at * 4);
+                    lo[0] = a.x; lo[1] = a.y; lo[2] = a.z; lo[3] = a.w;
+                    hi[0] = hi[1] = hi[2] = hi[3] = 0u;
+                }
+                if (p.t_bf16) {
+                    const half4 a = *reinterpret_cast<const half4*>(p.t + at * 2);
+                    t[0] = a.x & 0xffffu; t[1] = a.x >> 16; t[2] = a.y & 0xffffu; t[3] = a.y >> 16;
+                } else {
+                    const word4 a = *reinterpret_cast<const word4*>(p.t + at * 4);
+                    t[0] = a.x; t[1] = a.y; t[2] = a.z; t[3] = a.w;
+                }
+                if (!in) hi[0] = hi[1] = hi[2] = hi[3] = 0xffffffffu;
+                return;
+            }
 #pragma unroll
         for (int n = 0; n < SL; ++n) {
             const int j = n * L + l;
