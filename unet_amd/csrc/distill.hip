@@ -171,8 +171,8 @@ __device__ __forceinline__ void block_part(const DistParams& p, double loss, dou
 }
 
 // ---- short rows -----------------------------------------------------------------------------------------------------
-// 524288 rows of 16 bf16 classes, 4 slots: forward 15 us (33 MB), backward 15 us (50 MB); 50001 x 133 fp32, 5 slots: 16 us (29 MB) and
-// 22 us (55 MB).  Such calls are bounded by the latency of a row or two per thread (0.3 of the wave cycles issue); 2097152 rows of 16:
+// 524288 rows of 16 bf16 classes, 4 slots: forward 15 us (33 MB), backward 15 us (50 MB); 50001 x 133 fp32, 5 slots: 13 us (29 MB) and
+// 17 us (55 MB).  Such calls are bounded by the latency of a row or two per thread (0.3 of the wave cycles issue); 2097152 rows of 16:
 // forward 43 us, 3.1 TB/s.
 // SL slots of a row's list in the registers of a lane: slot j of the list is slot j / L of lane j % L, or slot j % 4 of lane j / 4 where every lane
 // has four (one or two loads in place of four: 2097152 rows of 16 bf16 classes, forward 51 -> 43 us).  `fetch` only requests them.
@@ -597,7 +597,7 @@ __global__ __launch_bounds__(TPB) void distill_count(DistParams p) {
 // a vector's gradient is stored, the same vector of the next row is requested.  The exponentials are taken twice: kept, they
 // need twice the registers of the bf16 row, and fewer rows in flight cost more than the arithmetic (4096 x 32768 bf16 step: 160 us
 // kept, 138 taken twice, 190 with two passes over memory).  Logits and gradient pass the caches by: 137 -> 123 us (the gradient alone
-// 131).  Bound by the read and the write: 112 us of kernel, 4.8 TB/s.
+// 131).  Bound by the read and the write: 108 us of kernel, 5.0 TB/s.
 template <class TR, int T, int NV>
 __global__ __launch_bounds__(T, 4) void distill_long_step(DistParams p) {
     __shared__ float wm[T / 64], ws[T / 64], qw[MAX_K], qt[MAX_K], qz[MAX_K], scale_s;
@@ -775,7 +775,7 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
     memset(&q, 0, sizeof(q));
     const int vec = 16 / esz, nvec = (v + vec - 1) / vec;
     auto least = [&](int64_t per, int64_t cap) { const int64_t b = (rows + per - 1) / per; return (int)(b < cap ? b : cap); };
-    auto vectors = [&](int L) { int n = 1; while (n * L < nvec) n *= 2; return n; };
+    auto vectors = [&](int L) { return (nvec + L - 1) / L; };
     q.is_long = nvec > 64 * NVMAX;
     if (!q.is_long) {
         q.L = 1;
@@ -832,10 +832,12 @@ int check_args(const char* who, int dtype, int64_t rows, int v, int64_t pitch, c
         if (dtype == 1) {                                                                                      \
             if (nv == 1) KERN<BF16, 1 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                                 \
             else if (nv == 2) KERN<BF16, 2 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                            \
+            else if (nv == 3) KERN<BF16, 3 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                            \
             else KERN<BF16, 4 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                                         \
         } else {                                                                                               \
             if (nv == 1) KERN<F32, 1 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                                  \
             else if (nv == 2) KERN<F32, 2 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                             \
+            else if (nv == 3) KERN<F32, 3 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                             \
             else KERN<F32, 4 __VA_ARGS__><<<grid, TPB, lds, st>>>(p);                                          \
         }                                                                                                      \
         MI_HIP(hipGetLastError());                                                                             \

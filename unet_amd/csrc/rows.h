@@ -50,12 +50,33 @@ __device__ __forceinline__ uint4 down(uint4 w, int n) {
 // the compiler takes the value as new: what was computed from it before is not kept in registers
 __device__ __forceinline__ void hold(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
 
-// maximum / sum over the L neighbouring lanes that share a row (L a power of two)
+// v joined by f (commutative) over L (a power of two, the same for the whole wave) neighbouring lanes, all of which end with the result:
+// lanes at distance 1, then 2, halves and rows mirrored (a quad's lanes agree by then), rows and halves of the wave swapped.  Nothing
+// goes through LDS, where an exchange takes a hundred cycles (1000000 rows of 133 fp32 classes, distillation loss: 192 -> 150 us).
+template <int CTRL>
+__device__ __forceinline__ unsigned lane_move(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+template <class F>
+__device__ __forceinline__ unsigned lanes_join(unsigned v, int L, F f) {
+    if (L == 1) return v;
+    v = f(v, lane_move<0xB1>(v));                                  // quad: 1 0 3 2
+    if (L == 2) return v;
+    v = f(v, lane_move<0x4E>(v));                                  // quad: 2 3 0 1
+    if (L == 4) return v;
+    v = f(v, lane_move<0x141>(v));                                 // eight lanes mirrored
+    if (L == 8) return v;
+    v = f(v, lane_move<0x140>(v));                                 // sixteen lanes mirrored
+    if (L == 16) return v;
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(r[0], r[1]);
+    if (L == 32) return v;
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(h[0], h[1]);
+}
 __device__ __forceinline__ float lanes_max(float v, int L) {
-    for (int o = L >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    return __uint_as_float(lanes_join(__float_as_uint(v), L, [](unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
 }
 __device__ __forceinline__ float lanes_sum(float v, int L) {
-    for (int o = L >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    return __uint_as_float(lanes_join(__float_as_uint(v), L, [](unsigned a, unsigned b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
+__device__ __forceinline__ unsigned lanes_max(unsigned v, int L) { return lanes_join(v, L, [](unsigned a, unsigned b) { return max(a, b); }); }
+__device__ __forceinline__ unsigned lanes_min(unsigned v, int L) { return lanes_join(v, L, [](unsigned a, unsigned b) { return min(a, b); }); }

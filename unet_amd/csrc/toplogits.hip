@@ -158,7 +158,7 @@ __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
                     for (int j = 0; j < TR::VEC; ++j) best = max(best, key[i][j]);
-                for (int o = L >> 1; o > 0; o >>= 1) best = max(best, __shfl_xor(best, o, 64));
+                best = lanes_max(best, L);
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -174,11 +174,8 @@ __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
 #pragma unroll
                     for (int j = 0; j < TR::VEC; ++j)
                         if (key[i][j] > best) { best = key[i][j]; at = (i * L + l) * TR::VEC + j; }
-                for (int o = L >> 1; o > 0; o >>= 1) {
-                    const unsigned ob = __shfl_xor(best, o, 64);
-                    const int oa = __shfl_xor(at, o, 64);
-                    if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-                }
+                const unsigned all = lanes_max(best, L);
+                at = (int)lanes_min(best == all ? (unsigned)at : 0x7fffffffu, L);
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -501,8 +498,7 @@ __global__ __launch_bounds__(T) void top_long(TopParams p) {
         const unsigned tail = et < p.v ? key_of(ld_one<TR>(x, et)) : 0u;
         const unsigned best = max(b.key(), tail);
         // G maxima of T / G neighbouring threads each
-        unsigned group = best;
-        for (int o = T / p.G >> 1; o > 0; o >>= 1) group = max(group, __shfl_xor(group, o, 64));
+        const unsigned group = lanes_max(best, T / p.G);
         if (tid % (T / p.G) == 0) top[tid / (T / p.G)] = group;
         if (tid == 0) count_s = hot_s = 0;
         __syncthreads();
@@ -559,10 +555,8 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         while (q.L < 64 && nvec > q.L * NVMAX) q.L *= 2;
         // instructions of a wave per row: k times 3 (bf16) or 6 (fp32) per held class and 10 per exchange between lanes (networks: 44 or 70 per vector, 50 or 110 per exchange), for
         // 64 / L rows at once, against 4 per bit and 12 per held class (k <= 32, by the lanes' maxima) or 3 per held class and bit, and the placing.
-        // 50000 rows of 512 bf16 classes, 16 of them: 50 us by search alone, 29 with the lanes' maxima; 100000 x 133 fp32, 5: 38 taken out
-        int n1 = 1, n2 = 1;
-        while (n1 * q.L < nvec) n1 *= 2;
-        while (n2 * 64 < nvec) n2 *= 2;
+        // 50000 rows of 512 bf16 classes, 16 of them: 50 us by search alone, 29 with the lanes' maxima; 100000 x 133 fp32, 5: 28 taken out
+        const int n1 = (nvec + q.L - 1) / q.L, n2 = (nvec + 63) / 64;
         const int e1 = n1 * vec, e2 = n2 * vec;
         int lg = 0;
         while ((1 << lg) < q.L) ++lg;
@@ -571,7 +565,7 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         const int64_t take = ((nets ? nets : (int64_t)k * ((esz == 2 ? 3 : 6) * e1 + 10 * lg + 8)) + 8 * e1) * q.L / 64, search = q.by_lanes ? 8 * esz * 4 + 12 * e2 + 6 * k + 100 : 8 * esz * 3 * e2 + 100 + (int64_t)k * ((k + 63) / 64) * 4;
         q.kind = take <= search && k <= 32 ? SHORT : WAVE;             // 32: 32 KB of LDS
         if (q.kind == WAVE) q.L = 64;
-        while (q.nv < NVMAX && q.nv * q.L < nvec) q.nv *= 2;
+        q.nv = (nvec + q.L - 1) / q.L;
         per = TPB / q.L;
     } else {
         // Few rows: up to 1024 threads each, one vector at least (else groups without any would leave fewer than k maxima).  Else about
@@ -594,6 +588,7 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         const size_t lds = TPB / q.L * k * 4;                                                    \
         if (q.nv == 1) top_short<T, 1, K><<<q.blocks, TPB, lds, st>>>(p);                        \
         else if (q.nv == 2) top_short<T, 2, K><<<q.blocks, TPB, lds, st>>>(p);                   \
+        else if (q.nv == 3) top_short<T, 3, K><<<q.blocks, TPB, lds, st>>>(p);                   \
         else top_short<T, 4, K><<<q.blocks, TPB, lds, st>>>(p);                                  \
     } while (0)
 #define LONG_T(TR, ODD)                                                                           \
@@ -608,10 +603,12 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         if (dtype == 1) {                                                                      \
             if (q.nv == 1) KERN<BF16, 1><<<q.blocks, TPB, lds, st>>>(p);                         \
             else if (q.nv == 2) KERN<BF16, 2><<<q.blocks, TPB, lds, st>>>(p);                    \
+            else if (q.nv == 3) KERN<BF16, 3><<<q.blocks, TPB, lds, st>>>(p);                    \
             else KERN<BF16, 4><<<q.blocks, TPB, lds, st>>>(p);                                   \
         } else {                                                                               \
             if (q.nv == 1) KERN<F32, 1><<<q.blocks, TPB, lds, st>>>(p);                          \
             else if (q.nv == 2) KERN<F32, 2><<<q.blocks, TPB, lds, st>>>(p);                     \
+            else if (q.nv == 3) KERN<F32, 3><<<q.blocks, TPB, lds, st>>>(p);                     \
             else KERN<F32, 4><<<q.blocks, TPB, lds, st>>>(p);                                    \
         }                                                                                      \
     } while (0)
