@@ -113,6 +113,10 @@ struct Row {
                 for (int j = 0; j < TR::VEC; ++j) x[i][j] = e0 + j < v ? ld_one<TR>(z, e0 + j) : -INFINITY;
                 continue;
             }
+            if ((i + 1) * L * TR::VEC <= v) {                     // the same for all lanes: they all hold whole vectors
+                unpack_vec<TR>(raw[i], x[i]);
+                continue;
+            }
             uint4 w = raw[i];
             if (v % TR::VEC) {                                    // the same for all lanes
                 const int over = e0 + TR::VEC - v;                // > 0: the partial vector, its first class lies `over` up
@@ -319,7 +323,7 @@ __device__ __forceinline__ void store_row(char* dz, int v, int L, int l, F f) {
         const int e0 = (i * L + l) * TR::VEC;
         float __attribute__((aligned(16))) d[TR::VEC];
         f(i, e0, d);
-        if (e0 + TR::VEC <= v) {
+        if ((i + 1) * L * TR::VEC <= v || e0 + TR::VEC <= v) {
             st_any(dz + (int64_t)e0 * TR::ESZ, pack_vec<TR>(d));
         } else {
 #pragma unroll
