@@ -64,7 +64,7 @@ def test_top_logits(dev, mode, case):
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])
-@pytest.mark.parametrize("k", range(1, 10))
+@pytest.mark.parametrize("k", range(1, 17))
 def test_top_logits_of_every_pattern(dev, mode, k):
     """All rows of 16 zeros and ones: a network of exchanges that orders these orders everything."""
     n = torch.arange(1 << 16)
@@ -73,7 +73,24 @@ def test_top_logits_of_every_pattern(dev, mode, k):
     g = torch.Generator().manual_seed(k)
     for v in (9, 23, 70, 300, 1100):
         x = torch.rand(400, v, generator=g).argsort(-1).to(DT[mode]).to(dev)            # bf16: ties above 256
-        check_top(x, k)
+        check_top(x, min(k, v))
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("v", [17, 31, 32, 33, 64, 65, 100, 128, 129, 200, 255, 256])
+def test_top_logits_of_whole_rows(dev, mode, v):
+    """Lists up to the whole row: orders, reversed orders, steps at every class, ties and special values."""
+    g = torch.Generator().manual_seed(v)
+    up = torch.arange(v, dtype=torch.float32)
+    steps = (up[:, None] >= up[None, :]).float()
+    x = torch.cat([torch.rand(300, v, generator=g).argsort(-1).float() - 100, up[None], -up[None], steps, 1 - steps, torch.randn(100, v, generator=g),
+                   torch.randint(0, 3, (100, v), generator=g).float()])
+    x[0, v // 2], x[1, 3], x[2, ::2], x[3, 1::2] = math.nan, -math.nan, -math.inf, math.inf
+    x[4] = torch.where(torch.arange(v) % 2 == 0, torch.tensor(0.0), torch.tensor(-0.0))
+    x = x.to(DT[mode]).to(dev)
+    for k in sorted({5, 9, 12, 33, v // 2, v - 1, v}):
+        if k <= v:
+            check_top(x, k)
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])

@@ -5,7 +5,7 @@
 // value and stands for "none".
 //
 // Bandwidth-bound: the rows have to be read once.
-//   top_short: lists of a few entries; L neighbouring lanes hold a row in registers and take the largest out k times, or order by networks
+//   top_short: L neighbouring lanes hold a row in registers and take the largest out k times, or order it by networks
 //   top_wave : a wave holds the row; the k-th largest key is found bit by bit, by counting the keys from there on, the k classes
 //              are gathered in LDS (equal keys by ascending class) and placed by the number of full keys above their own
 //   top_long : a workgroup streams the row and keeps the largest key of every thread's part.  At least k classes lie at or above
@@ -23,6 +23,7 @@ namespace {
 constexpr int TPB = 256;
 constexpr int MAX_K = 256;
 constexpr int NVMAX = 4;
+constexpr int SORT = -1;
 
 struct TopParams {
     const char* x;
@@ -66,18 +67,31 @@ __device__ __forceinline__ void load_keys(const char* x, int v, int L, int l, un
     }
 }
 
+// fp32 keys with their classes as doubles in 1 .. 2, which order like their bits: 32 bits of key, 20 of class
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+__device__ __forceinline__ double smaller(double a, double b) { return __builtin_fmin(a, b); }
+__device__ __forceinline__ double key_word(unsigned key, int cls) {
+    return __hiloint2double((int)(0x3ff00000u | key >> 12), (int)(key << 20 | (0xfffffu - (unsigned)cls)));
+}
+
 // Networks on words: a holds the larger one after swap_down.  sort_down: N = 4 or 8 words, largest first (merge exchanges of two sorted
 // halves); top_of_two: the N largest of two sorted lists, sorted, in a.
 __device__ __forceinline__ void swap_down(unsigned& a, unsigned& b) {
     const unsigned hi = max(a, b), lo = min(a, b);
     a = hi; b = lo;
 }
-__device__ __forceinline__ void sort4(unsigned* a) {
+__device__ __forceinline__ void swap_down(double& a, double& b) {
+    const double hi = larger(a, b), lo = smaller(a, b);
+    a = hi; b = lo;
+}
+template <class W>
+__device__ __forceinline__ void sort4(W* a) {
     swap_down(a[0], a[1]); swap_down(a[2], a[3]);
     swap_down(a[0], a[2]); swap_down(a[1], a[3]);
     swap_down(a[1], a[2]);
 }
-__device__ __forceinline__ void sort8(unsigned* a) {
+template <class W>
+__device__ __forceinline__ void sort8(W* a) {
     sort4(a); sort4(a + 4);
     swap_down(a[0], a[4]); swap_down(a[1], a[5]); swap_down(a[2], a[6]); swap_down(a[3], a[7]);
     swap_down(a[2], a[4]); swap_down(a[3], a[5]);
@@ -92,6 +106,83 @@ __device__ __forceinline__ void top_of_two(unsigned* a, const unsigned* b) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (!(i & o)) swap_down(a[i], a[i + o]);
+}
+
+// Sorting over lanes: E = 4 or 8 words a lane, largest first, lane by lane.  Two sorted halves of N lanes each: the first exchange is with the
+// mirrored lane and word, the others with lanes at distance N / 2 .. 1, the last ones within the lane.  An exchange takes the larger one
+// in the lower lane and the smaller one in the upper; for 32-bit words that is the middle one of the two and of everything or nothing: two
+// instructions a word.  67496 rows of 99 classes, 35 of them: bf16 71 -> 17.5 us, fp32 68 -> 36 (found bit by bit before); 300000 x 64, 16:
+// 38 -> 27.5 and 57 -> 48 (taken out).
+__device__ __forceinline__ unsigned pick(unsigned a, unsigned b, bool upper) {
+    const unsigned lim = upper ? 0u : 0xffffffffu;
+    return max(min(a, b), min(max(a, b), lim));
+}
+__device__ __forceinline__ double pick(double a, double b, bool upper) { return (a > b) != upper ? a : b; }
+template <int X>
+__device__ __forceinline__ unsigned from_lane(unsigned v) {                        // lane ^ X
+    if constexpr (X == 1) return lane_move<0xB1>(v);
+    else if constexpr (X == 2) return lane_move<0x4E>(v);
+    else if constexpr (X == 3) return lane_move<0x1B>(v);
+    else if constexpr (X == 4) return lane_move<0x1B>(lane_move<0x141>(v));
+    else if constexpr (X == 7) return lane_move<0x141>(v);
+    else if constexpr (X == 8) return lane_move<0x128>(v);
+    else if constexpr (X == 15) return lane_move<0x140>(v);
+    else if constexpr (X == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? r[0] : r[1];
+    } else if constexpr (X == 31) {
+        return from_lane<16>(lane_move<0x140>(v));
+    } else {
+        static_assert(X == 63, "");
+        const unsigned m = from_lane<31>(v);
+        const auto r = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+        return threadIdx.x & 32 ? r[0] : r[1];
+    }
+}
+template <int X>
+__device__ __forceinline__ double from_lane(double v) {
+    return __hiloint2double((int)from_lane<X>((unsigned)__double2hiint(v)), (int)from_lane<X>((unsigned)__double2loint(v)));
+}
+template <int X, bool MIRROR, int E, class W>
+__device__ __forceinline__ void exchange(W* a) {
+    const bool upper = threadIdx.x & (MIRROR ? (X + 1) / 2 : X);
+    W b[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) b[e] = from_lane<X>(a[MIRROR ? E - 1 - e : e]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) a[e] = pick(a[e], b[e], upper);
+}
+// two sorted halves of N lanes -> one of 2 N
+template <int N, int E, class W>
+__device__ __forceinline__ void merge_lanes(W* a) {
+    exchange<2 * N - 1, true, E>(a);
+    if constexpr (N >= 32) exchange<16, false, E>(a);
+    if constexpr (N >= 16) exchange<8, false, E>(a);
+    if constexpr (N >= 8) exchange<4, false, E>(a);
+    if constexpr (N >= 4) exchange<2, false, E>(a);
+    if constexpr (N >= 2) exchange<1, false, E>(a);
+#pragma unroll
+    for (int o = E / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (!(i & o)) swap_down(a[i], a[i + o]);
+}
+template <int E, class W>
+__device__ __forceinline__ void sort_lanes(W* a, int L) {
+    if constexpr (E == 8) sort8(a);
+    else sort4(a);
+    if (L == 1) return;
+    merge_lanes<1, E>(a);
+    if (L == 2) return;
+    merge_lanes<2, E>(a);
+    if (L == 4) return;
+    merge_lanes<4, E>(a);
+    if (L == 8) return;
+    merge_lanes<8, E>(a);
+    if (L == 16) return;
+    merge_lanes<16, E>(a);
+    if constexpr (E == 4)
+        if (L == 64) merge_lanes<32, E>(a);
 }
 
 // The classes found go through LDS (dynamic, [workgroup's rows][k]): the results of a wave's rows are one piece of the output and
@@ -125,7 +216,22 @@ __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
                 }
             }
         }
-        if constexpr (K != 0) {
+        if constexpr (K == SORT) {
+            if constexpr (TR::ESZ == 2) {
+                sort_lanes<8>(key[0], L);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (l * 8 + e < p.k) mine[l * 8 + e] = key[0][e] ^ 0xffffu;
+            } else {
+                double w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = key_word(key[0][e], l * 4 + e);
+                sort_lanes<4>(w, L);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (l * 4 + e < p.k) mine[l * 4 + e] = 0xfffffu - ((unsigned)__double2loint(w[e]) & 0xfffffu);
+            }
+        } else if constexpr (K != 0) {
             unsigned* top = key[0];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -542,7 +648,7 @@ __global__ __launch_bounds__(T) void top_long(TopParams p) {
     }
 }
 
-enum { SHORT, WAVE, LONG };
+enum { SHORT, SORTED, WAVE, LONG };
 struct Plan { int kind, L, nv, T, G, blocks, by_lanes; };
 Plan plan_of(int esz, int64_t rows, int v, int k) {
     Plan q = {SHORT, 1, 1, TPB, 0, 0, 0};
@@ -564,6 +670,12 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         const int nets = esz == 2 && k <= 8 ? k <= 4 ? n1 * 44 + lg * 50 : n1 * 70 + lg * 110 : 0;
         const int64_t take = ((nets ? nets : (int64_t)k * ((esz == 2 ? 3 : 6) * e1 + 10 * lg + 8)) + 8 * e1) * q.L / 64, search = q.by_lanes ? 8 * esz * 4 + 12 * e2 + 6 * k + 100 : 8 * esz * 3 * e2 + 100 + (int64_t)k * ((k + 63) / 64) * 4;
         q.kind = take <= search && k <= 32 ? SHORT : WAVE;             // 32: 32 KB of LDS
+        if (k > (esz == 2 ? 8 : 4) && nvec <= (esz == 2 ? 32 : 64)) {
+            int s = 1, ls = 0;
+            while (s < nvec) s *= 2, ++ls;
+            const int sort = (200 + (esz == 2 ? 24 : 12) * ls + (esz == 2 ? 9 : 13) * ls * (ls + 1)) * s / 64;
+            if (sort < (q.kind == SHORT ? take : search)) { q.kind = SORTED; q.L = s; }
+        }
         if (q.kind == WAVE) q.L = 64;
         q.nv = (nvec + q.L - 1) / q.L;
         per = TPB / q.L;
@@ -629,7 +741,10 @@ extern "C" int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, cons
     p.x = (const char*)logits; p.val = (char*)values; p.idx = index;
     p.rows = rows; p.xp = pitch * (int64_t)esz; p.v = v; p.k = k; p.L = q.L; p.G = q.G; p.by_lanes = q.by_lanes;
     hipStream_t st = (hipStream_t)stream;
-    if (q.kind == SHORT) {
+    if (q.kind == SORTED) {
+        if (dtype == 1) top_short<BF16, 1, SORT><<<q.blocks, TPB, TPB / q.L * k * 4, st>>>(p);
+        else top_short<F32, 1, SORT><<<q.blocks, TPB, TPB / q.L * k * 4, st>>>(p);
+    } else if (q.kind == SHORT) {
         if (dtype == 0) SHORT_NV(F32, 0);
         else if (k == 1) SHORT_NV(BF16, 1);
         else if (k <= 4) SHORT_NV(BF16, 4);
