@@ -181,8 +181,8 @@ __device__ __forceinline__ void sort_lanes(W* a, int L) {
     merge_lanes<8, E>(a);
     if (L == 16) return;
     merge_lanes<16, E>(a);
-    if constexpr (E == 4)
-        if (L == 64) merge_lanes<32, E>(a);
+    if (L == 32) return;
+    merge_lanes<32, E>(a);
 }
 
 // The classes found go through LDS (dynamic, [workgroup's rows][k]): the results of a wave's rows are one piece of the output and
@@ -670,7 +670,7 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         const int nets = esz == 2 && k <= 8 ? k <= 4 ? n1 * 44 + lg * 50 : n1 * 70 + lg * 110 : 0;
         const int64_t take = ((nets ? nets : (int64_t)k * ((esz == 2 ? 3 : 6) * e1 + 10 * lg + 8)) + 8 * e1) * q.L / 64, search = q.by_lanes ? 8 * esz * 4 + 12 * e2 + 6 * k + 100 : 8 * esz * 3 * e2 + 100 + (int64_t)k * ((k + 63) / 64) * 4;
         q.kind = take <= search && k <= 32 ? SHORT : WAVE;             // 32: 32 KB of LDS
-        if (k > (esz == 2 ? 8 : 4) && nvec <= (esz == 2 ? 32 : 64)) {
+        if (k > (esz == 2 ? 8 : 4) && nvec <= 64) {
             int s = 1, ls = 0;
             while (s < nvec) s *= 2, ++ls;
             const int sort = (200 + (esz == 2 ? 24 : 12) * ls + (esz == 2 ? 9 : 13) * ls * (ls + 1)) * s / 64;
