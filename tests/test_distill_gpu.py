@@ -49,7 +49,7 @@ TOP = [(1, 1, 1), (7, 2, 2), (300, 3, 2), (300, 16, 4), (65, 16, 16), (130, 21, 
        (17, 257, 17), (6, 512, 16), (6, 513, 40), (5, 1024, 100), (5, 1025, 16), (5, 1025, 200), (4, 2048, 16), (4, 2049, 3), (3, 5000, 256), (2, 50001, 32),
        (1, 128000, 64), (1, 4097, 1), (600, 2100, 20), (520, 4200, 100), (513, 20000, 70), (513, 40000, 200), (3, 70000, 256), (2, 140000, 256), (2, 2049, 256), (300, 176, 17), (40, 700, 130), (5, 2100, 24), (5, 2100, 200), (5, 4200, 60),
        (5, 9000, 42), (9, 1025, 85), (600, 1025, 85), (9, 1030, 86), (7, 1999, 64), (12, 517, 33), (600, 1025, 1), (520, 10241, 9), (520, 20500, 171),
-       (520, 100001, 5), (300, 150, 9), (300, 23, 9), (70, 600, 33), (70, 1100, 33), (70, 1100, 20)]
+       (520, 100001, 5), (300, 150, 9), (300, 23, 9), (70, 600, 33), (70, 1100, 33), (70, 1100, 20), (66000, 130, 40)]
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])
@@ -227,7 +227,7 @@ LOSS = [(1, 1, 1), (5, 2, 1), (64, 3, 3), (300, 16, 4), (257, 21, 5), (70, 16, 2
         (17, 2048, 256), (9, 2049, 7), (9, 1023, 256), (5000, 7, 2), (3, 50001, 32), (1, 32001, 64), (4100, 2050, 3), (7, 8200, 12), (5, 16390, 9), (3, 33000, 4),
         (2, 70000, 8), (2, 131072, 5), (2, 131080, 5),
         (520, 9000, 4), (513, 34000, 3), (600, 29, 12), (2, 5, 1), (2050, 16, 1), (90, 2043, 2), (300, 1021, 17),
-        (40, 1100, 16), (40, 600, 20), (130, 140, 7), (130, 75, 40)]
+        (40, 1100, 16), (40, 600, 20), (130, 140, 7), (130, 75, 40), (40000, 140, 40), (140000, 68, 5), (530000, 5, 2)]
 
 
 @pytest.mark.parametrize("mode", ["fp32", "bf16"])

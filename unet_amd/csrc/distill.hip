@@ -398,7 +398,7 @@ __global__ __launch_bounds__(TPB) void distill_short_bwd_reg(DistParams p) {
 // floats of LDS per row of the kernel below: class weights (whole vectors), classes and weights of the slots; 16-byte rows
 __host__ __device__ __forceinline__ int lds_row(int vec, int v, int k) { return (v + vec - 1) / vec * vec + (2 * k + 3) / 4 * 4; }
 
-// any list: the slots' weights are put down at their classes in LDS
+// any list: the slots' weights are put down at their classes in LDS.  Logits and list are requested one row ahead: nothing else is read.
 template <class TR, int NV>
 __global__ __launch_bounds__(TPB) void distill_short_bwd(DistParams p) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -406,26 +406,57 @@ __global__ __launch_bounds__(TPB) void distill_short_bwd(DistParams p) {
     float* acc = lds + slot * lds_row(TR::VEC, p.v, p.k);
     int* qi = reinterpret_cast<int*>(acc + va);
     float* qw = reinterpret_cast<float*>(qi) + p.k;
-    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += (int64_t)gridDim.x * per) {
-        const int64_t r = r0 + slot;
+    const int64_t step = (int64_t)gridDim.x * per;
+    int64_t r = (int64_t)blockIdx.x * per + slot;
+    uint4 raw[NV];
+    Slots<4> next;
+    auto fetch = [&](int64_t row) {
+        const bool in = row < p.rows;
+        Row<TR, NV>::fetch(raw, p.z + (in ? row : 0) * p.zp, p.v, L, l);
+        next.fetch(p, row, in, L, l);
+    };
+    fetch(r);
+    const bool near = p.k == 4 * L;                               // which slot of the list a lane's n-th is
+    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += step, r += step) {
         const bool in = r < p.rows;
-        uint4 raw[NV];
-        const char* z = p.z + (in ? r : 0) * p.zp;
-        Row<TR, NV>::fetch(raw, z, p.v, L, l);
         for (int i = 4 * l; i < va; i += 4 * L) *reinterpret_cast<float4*>(acc + i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const bool some = list_weights(p, r, in, L, l, qi, qw, qw);
+        Row<TR, NV> x;
+        x.take(raw, p.z + (in ? r : 0) * p.zp, p.v, L, l);
+        float q[4], tm = -INFINITY, total = 0.0f;
+        int cls[4];
+        bool some = false;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            cls[n] = next.cls(p, n);
+            q[n] = next.teacher(p, n);
+            if (cls[n] >= 0) { tm = fmaxf(tm, q[n]); some = true; }
+        }
+        if (r0 + step < p.rows) fetch(r + step);
+        tm = lanes_max(tm, L);
+        some = (bool)lanes_max(some ? 1.0f : 0.0f, L);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            q[n] = cls[n] >= 0 ? __builtin_amdgcn_exp2f((q[n] - tm) * p.c) : 0.0f;
+            total += q[n];
+        }
+        const float qs = 1.0f / lanes_sum(total, L);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int j = near ? 4 * l + n : n * L + l;
+            q[n] *= qs;
+            if (j < p.k) { qi[j] = cls[n]; qw[j] = q[n]; }
+        }
         wave_sync();
         bool twice = false;                                       // a class that already has a weight
-        if (in && some)
-            for (int j = l; j < p.k; j += L)
-                if (qi[j] >= 0) twice |= atomicExch(acc + qi[j], qw[j]) != 0.0f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            if (cls[n] >= 0) twice |= atomicExch(acc + cls[n], q[n]) != 0.0f;
         if (lanes_max(twice ? 1.0f : 0.0f, L) != 0.0f) {
             wave_sync();
-            for (int j = l; j < p.k; j += L)
-                if (qi[j] >= 0) acc[qi[j]] = weight_of(qi, qw, p.k, qi[j]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                if (cls[n] >= 0) acc[cls[n]] = weight_of(qi, qw, p.k, cls[n]);
         }
-        Row<TR, NV> x;
-        x.take(raw, z, p.v, L, l);
         const float m = x.max_of(L), s = x.exp_of(m, p.c, L);
         wave_sync();
         if (in) {
@@ -759,13 +790,14 @@ __global__ __launch_bounds__(1024) void distill_final(DistParams p) {
 
 // ---- host side --------------------------------------------------------------------------------------------------------
 // Short rows: the fewest lanes whose registers (NVMAX vectors each) hold the row and, 4 slots each, its list.  The backward
-// pass compares every held class with every slot while that is cheap (k * held classes <= REG_WORK: 2 M rows of 16 bf16 classes, 4
-// slots 103 us a step, 151 through LDS; 50000 x 512, 16 slots 79 and 72), else it goes through LDS, with the rows of a workgroup
-// within 32 KB.
+// pass compares every held class with every slot while that is cheap, slots of other lanes costing their way here as well (not where a lane has few
+// rows: 50001 x 133 fp32, 5 slots 17 us, 20 through LDS); else it goes through LDS, with the rows of a workgroup within
+// 32 KB.  Steps by comparing and through LDS: 4000000 x 16 bf16, 4 slots (work 64) 173 and 186 us, 2000000 x 21, 4 (96) 143 and 151, 2000000 x 32, 8 (128) 192 and 193; 1000000 x 133 fp32, 5 (60, from many lanes) 526 and 466, 1000000 x 64 fp32, 5 (80) 216
+// and 190, 100000 x 1000 bf16, 2 (64) 182 and 167.
 // Long rows, forward: a wave per row up to 1024 vectors, 256 threads behind that, 1024 where rows alone do not fill the chip (5 x
 // 32001 fp32: 256 threads 13.1 us, 1024 7.8).  Step: the fewest threads of 64, 256, 512, 1024 that hold the row with at
 // most 16 vectors each (262144 bytes of row).
-constexpr int REG_WORK = 128;
+constexpr int REG_WORK = 120;
 struct Plan {
     bool is_long;
     int L, nv, sl;                   // short rows
@@ -787,9 +819,9 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
         q.nv = vectors(q.L);
         q.sl = k <= q.L ? 1 : 4;
         q.blocks = q.bwd_blocks = q.parts = least(TPB / q.L, 2048);
-        if (k * q.nv * vec > REG_WORK) {
+        if (k * (q.nv * vec + (q.L > 2 && rows > 4 * (int64_t)q.blocks * (TPB / q.L) ? 32 : 0)) > REG_WORK) {
             q.lds_L = 1;
-            while (q.lds_L < 64 && (nvec > q.lds_L * NVMAX || (TPB / q.lds_L) * lds_row(vec, v, k) * 4 > 32768)) q.lds_L *= 2;
+            while (q.lds_L < 64 && (nvec > q.lds_L * NVMAX || k > 4 * q.lds_L || (TPB / q.lds_L) * lds_row(vec, v, k) * 4 > 32768)) q.lds_L *= 2;
             q.lds_nv = vectors(q.lds_L);
             q.bwd_blocks = least(TPB / q.lds_L, 2048);
         }

@@ -74,8 +74,8 @@ __device__ __forceinline__ double key_word(unsigned key, int cls) {
     return __hiloint2double((int)(0x3ff00000u | key >> 12), (int)(key << 20 | (0xfffffu - (unsigned)cls)));
 }
 
-// Networks on words: a holds the larger one after swap_down.  sort_down: N = 4 or 8 words, largest first (merge exchanges of two sorted
-// halves); top_of_two: the N largest of two sorted lists, sorted, in a.
+// Networks on words: a holds the larger one after swap_down.  sort4, sort8: largest first (sort8 by merge exchanges of two sorted halves);
+// top_of_two: the N largest of two sorted lists, sorted, in a.
 __device__ __forceinline__ void swap_down(unsigned& a, unsigned& b) {
     const unsigned hi = max(a, b), lo = min(a, b);
     a = hi; b = lo;
@@ -190,7 +190,7 @@ __device__ __forceinline__ void sort_lanes(W* a, int L) {
 // bf16: key and class fit one word, (key, 65535 - class), so that a maximum is one instruction.  Lists of at most K = 4 or 8 come from
 // networks: 76 or 108 instructions for the 16 words of two vectors, where taking out costs 40 per entry.  K = 1: the maximum.  K = 0: taken out
 // one by one.  2097152 rows of 16 classes, bf16: 4 of them 31 us (3.8 TB/s; taken out 38), 1 of them 21.5 (23), 8 of them 40 (57); 50000 x 512,
-// 4 of them: 20 (25).  Bounded by instructions: 350 per row of 16 (630 taken out).
+// 4 of them: 20 (25).  Bounded by instructions: 380 per row of 16 (630 taken out).
 template <class TR, int NV, int K>
 __global__ __launch_bounds__(TPB) void top_short(TopParams p) {
     // bf16: (key, class), the key's lower half being that of the value's sign; fp32: the class
@@ -659,7 +659,8 @@ Plan plan_of(int esz, int64_t rows, int v, int k) {
     const bool small_groups = nvec > 128 && nvec <= 64 * NVMAX && k <= 85 && (esz == 2 || k > 32);
     if (nvec <= 64 * NVMAX && !small_groups) {
         while (q.L < 64 && nvec > q.L * NVMAX) q.L *= 2;
-        // instructions of a wave per row: k times 3 (bf16) or 6 (fp32) per held class and 10 per exchange between lanes (networks: 44 or 70 per vector, 50 or 110 per exchange), for
+        // instructions of a wave per row: k times 3 (bf16) or 6 (fp32) per held class and 10 per exchange between
+        // lanes (networks: 44 or 70 per vector, 50 or 110 per exchange; sorted: a fixed part, the merges within and between lanes), for
         // 64 / L rows at once, against 4 per bit and 12 per held class (k <= 32, by the lanes' maxima) or 3 per held class and bit, and the placing.
         // 50000 rows of 512 bf16 classes, 16 of them: 50 us by search alone, 29 with the lanes' maxima; 100000 x 133 fp32, 5: 28 taken out
         const int n1 = (nvec + q.L - 1) / q.L, n2 = (nvec + 63) / 64;
