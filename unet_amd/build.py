@@ -37,21 +37,36 @@ def _stale(target: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
+def _made_by(obj: Path) -> Path:
+    return obj.with_name(obj.name + ".cmd")
+
+
+def _other_command(obj: Path, command: str) -> bool:
+    """Whether the object was compiled by another command (other flags, another compiler) or by one that is not known."""
+    record = _made_by(obj)
+    return not record.exists() or record.read_text() != command
+
+
 def build(force: bool = False, verbose: bool = True) -> Path:
+    """Compiles what is out of date: a source or header changed, or the command that compiles it did.  ``force``: everything."""
     hipcc = _hipcc()
+    command = " ".join([hipcc] + FLAGS)
     LIBDIR.mkdir(exist_ok=True)
     OBJDIR.mkdir(exist_ok=True)
     headers = sorted(CSRC.glob("*.h")) + [HERE.parent / "include" / "unet_mi355.h"]
     jobs = []
     for src in SOURCES:
         obj = OBJDIR / (src + ".o")
-        if force or _stale(obj, [CSRC / src] + headers):
+        if force or _stale(obj, [CSRC / src] + headers) or _other_command(obj, command):
             jobs.append((src, obj))
 
     def compile_one(job):
         src, obj = job
         cmd = [hipcc] + FLAGS + ["-c", str(CSRC / src), "-o", str(obj)]
+        _made_by(obj).unlink(missing_ok=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode == 0:
+            _made_by(obj).write_text(command)
         return src, r.returncode, r.stdout + r.stderr
 
     if jobs:
