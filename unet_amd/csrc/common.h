@@ -169,6 +169,9 @@ __device__ __forceinline__ bool dropout_keep1(const DropKeys& k, unsigned idx) {
 // ---- host side ----------------------------------------------------------------
 #include <string>
 void mi_set_error(const std::string& s);
+// Zeros behind p, `bytes` a multiple of 8, by a kernel: a memset that a caller's stream capture records has left wrong values on
+// replays after the first.
+int launch_zero(void* p, size_t bytes, hipStream_t st);
 // mean / rstd of a one-channel image from its fp64 statistics slots ([nb][NSLOT][2])
 __device__ __forceinline__ void c1_moments(const double* stats, int img, int npix, float eps, float& mean, float& rstd) {
     double s1 = 0.0, s2 = 0.0;

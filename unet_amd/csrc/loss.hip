@@ -283,9 +283,18 @@ static bool loss_v4(const LossParams& p) {
     return p.npix % 4 == 0 && ((uintptr_t)p.logits & 15) == 0 && ((uintptr_t)p.target & (uintptr_t)(4 * tsz > 16 ? 15 : 4 * tsz - 1)) == 0;
 }
 
+static __global__ __launch_bounds__(256) void zero_kernel(unsigned long long* p, long long n) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = 0ull;
+}
+int launch_zero(void* p, size_t bytes, hipStream_t st) {
+    const long long n = (long long)(bytes / 8);
+    hipLaunchKernelGGL(zero_kernel, dim3(grid_for(n, 256, 1024)), dim3(256), 0, st, static_cast<unsigned long long*>(p), n);
+    return check_launch("zero");
+}
+
 // sums ([nb][4] doubles) is zeroed here, then filled; loss[0] is written; loss_accum (optional) is accumulated.
 int launch_loss_fwd(const LossParams& p, hipStream_t st) {
-    if (!p.sums_cleared) MI_HIP(hipMemsetAsync(p.sums, 0, (size_t)p.nb * 4 * sizeof(double), st));
+    if (!p.sums_cleared) { if (int r = launch_zero(p.sums, (size_t)p.nb * 4 * sizeof(double), st)) return r; }
     if (loss_v4(p)) hipLaunchKernelGGL(loss_reduce_kernel<4>, dim3(grid_for(p.npix, 2048, 128), p.nb), dim3(256), 0, st, p);
     else hipLaunchKernelGGL(loss_reduce_kernel<1>, dim3(grid_for(p.npix, 2048, 128), p.nb), dim3(256), 0, st, p);
     if (int r = check_launch("loss_reduce")) return r;
@@ -348,7 +357,7 @@ int launch_loss_bwd(const LossParams& p, hipStream_t st) {
 }
 
 int launch_dice_counts(const CountParams& p, hipStream_t st) {
-    MI_HIP(hipMemsetAsync(p.counts, 0, (size_t)p.nb * 4 * sizeof(unsigned long long), st));
+    if (int r = launch_zero(p.counts, (size_t)p.nb * 4 * sizeof(unsigned long long), st)) return r;
     hipLaunchKernelGGL(dice_counts_kernel, dim3(grid_for(p.npix, 2048, 128), p.nb), dim3(256), 0, st, p);
     return check_launch("dice_counts");
 }

@@ -231,7 +231,7 @@ int mi_instnorm_prelu_bwd(int dtype, int nb, int64_t npix, int c, const mi_tenso
     p.stats = stats; p.bstats = bstats; p.alpha = alpha; p.dalpha = dalpha;
     p.nb = nb; p.npix = (int)npix; p.c = c; p.eps = 1e-5f;
     fill_drop(p, dropout, seed, layer);
-    MI_HIP(hipMemsetAsync(bstats, 0, (size_t)nb * MI_NSLOT * c * 2 * sizeof(double), (hipStream_t)stream));
+    if (int r = launch_zero(bstats, (size_t)nb * MI_NSLOT * c * 2 * sizeof(double), (hipStream_t)stream)) return r;
     return launch_norm_bwd(dtype, p, (hipStream_t)stream);
 }
 
