@@ -71,7 +71,8 @@ int mi_unet_bucket_range(const mi_unet* u, int bucket, int64_t* offset, int64_t*
 double mi_unet_flops(const mi_unet* u, int backward);          /* 2*MAC of the convolutions of one call */
 int mi_unet_num_steps(const mi_unet* u, int backward);         /* kernel launches per call (host logic check) */
 
-/* logits[b,1,...] = UNet(x[b,1,...]); `training` != 0 enables dropout (seeded, stateless).  */
+/* A pass (forward, backward, training step) forks and joins a stream of its own and is refused on a stream under graph capture.
+ * logits[b,1,...] = UNet(x[b,1,...]); `training` != 0 enables dropout (seeded, stateless).  */
 int mi_unet_forward(mi_unet* u, const float* params, const float* x, float* logits, void* workspace,
                     int training, uint64_t seed, void* stream);
 /* grads (flat fp32, same layout as params) of the forward that last used `workspace`.

@@ -83,3 +83,33 @@ def test_instance_norm_backward_replays(dev):
     stats[:, 0] = torch.stack([x.sum(1), x.square().sum(1)], -1)
 
     replay(dev, [dy], lambda: ops.instnorm_prelu_bwd(dy, raw, stats, alpha)[:1])
+
+
+def test_passes_over_the_network_are_refused_under_capture(dev):
+    """Nothing of a refused step stays behind: the next eager step leaves the parameters where it leaves them without the attempt."""
+    x = torch.rand(2, 1, 32, 32, device=dev)
+    t = (torch.rand(2, 1, 32, 32, device=dev) > 0.6).float()
+
+    def make():
+        torch.manual_seed(11)
+        m = unet_amd.UNet(2, 1, 1, (16, 32), (2,), num_res_units=2, dropout=0.1, compute_dtype=torch.float32).to(dev).train()
+        return m, unet_amd.Trainer(m, unet_amd.DiceCELoss(sigmoid=True), unet_amd.AdamW(m.parameters(), lr=1e-3, model=m))
+
+    (m0, tr0), (m1, tr1) = make(), make()
+    for tr in (tr0, tr1):
+        tr.step(x, t)
+    torch.cuda.synchronize()
+    plan, flat = m1._plan_for(x, True), m1._ensure_flat(dev)
+    ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=dev)
+    y, g = torch.empty_like(x), torch.zeros_like(flat)
+    for attempt in (lambda: tr1.step(x, t), lambda: m1(x), lambda: plan.forward(flat, x, y, ws, True, 3), lambda: plan.backward(flat, x, y, g, ws, True, 3)):
+        scratch = torch.ones(8, device=dev)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            scratch.zero_()
+            with pytest.raises(RuntimeError, match="captured"):
+                attempt()
+    for m, tr in ((m0, tr0), (m1, tr1)):
+        tr.step(x, t)
+    torch.cuda.synchronize()
+    assert torch.equal(m0.flat_parameters(), m1.flat_parameters())

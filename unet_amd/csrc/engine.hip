@@ -1184,6 +1184,12 @@ int run_list(mi_unet& u, std::vector<Step>& list, int backward, int bucket, char
     // the slab reductions (joined at the end of the call), in the forward pass the weight packing (joined in
     // front of the first kernel that reads packed weights).  Timing runs stay on one stream.
     bool side = false;
+    // A pass forks and joins a second stream and clears statistics by memsets.  A process that replayed a captured training step ended
+    // with a segmentation fault inside the replay (once; other runs of the same test passed) and the cause is not known: a pass is not recorded.
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    bool capture_elsewhere = false;          // the default stream while another one is captured: no value waits then
+    if (hipStreamIsCapturing(st, &capture) != hipSuccess) { (void)hipGetLastError(); capture_elsewhere = true; capture = hipStreamCaptureStatusNone; }
+    MI_CHECK(capture == hipStreamCaptureStatusNone, "a pass over the network cannot be captured into a graph");
     if (!u.prof) {
         if (u.use_side < 0) {
             u.use_side = getenv("MI_NO_SIDE_STREAM") ? 0 : 1;
@@ -1234,13 +1240,7 @@ int run_list(mi_unet& u, std::vector<Step>& list, int backward, int bucket, char
             if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&can, hipDeviceAttributeCanUseStreamWaitValue, dev) != hipSuccess) { (void)hipGetLastError(); can = 0; }
             u.can_wait_value = can ? 1 : 0;
         }
-        bool capturing = false;       // a stream under graph capture takes no value waits: events there
-        {
-            hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-            if (hipStreamIsCapturing(st, &cs) != hipSuccess) { (void)hipGetLastError(); capturing = true; }
-            else capturing = cs != hipStreamCaptureStatusNone;
-        }
-        if (!off && !capturing && u.can_wait_value == 1) {
+        if (!off && !capture_elsewhere && u.can_wait_value == 1) {
             flag_base = reinterpret_cast<unsigned*>(bases[B_ARENA] + u.off_flags);
             if (u.flag_seq == 0) u.flag_seq = 0x9e3779b9u * (unsigned)(reinterpret_cast<uintptr_t>(&u) >> 4) | 1u;
             u.flag_seq += 0x61c88647u;

@@ -444,6 +444,8 @@ class UNet(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         self._check_input(x)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a pass over the network cannot be captured into a graph")
         _lib.load()
         xin = x.as_subclass(torch.Tensor) if type(x) is not torch.Tensor else x
         in_dtype = xin.dtype

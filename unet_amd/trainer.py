@@ -71,6 +71,8 @@ class Trainer:
         model._check_input(x)
         if not model.training:
             raise RuntimeError("Trainer.step needs model.train()")
+        if torch.cuda.is_current_stream_capturing():       # before the step count and the seed move on
+            raise RuntimeError("a training step cannot be captured into a graph")
         lib = _lib.load()
         x = x.contiguous()
         if x.dtype != torch.float32:
