@@ -1,0 +1,69 @@
+"""The distillation loss where its numbers are hard: NaN and infinities in the teacher's lists."""
+import math
+
+import pytest
+import torch
+
+import unet_amd
+from unet_amd import ops
+
+pytestmark = pytest.mark.gpu
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
+
+
+# ---- NaN and +inf in the teacher --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("v,k", [(2, 1), (16, 4), (16, 2), (40, 40), (133, 5), (64, 16), (1000, 60), (600, 200), (4000, 6), (4000, 100), (4000, 256), (140000, 8)])
+def test_nan_and_inf_of_the_teacher_reach_the_loss(dev, mode, v, k, t_dtype):
+    """softmax over a list with a NaN or a +inf is NaN in every slot: so are the row's loss and its gradient at the listed classes,
+    wherever in the list the value stands, and no other row's."""
+    g = torch.Generator().manual_seed(v + k)
+    bad = [(n, value) for n in sorted({0, k // 2, k - 1}) for value in (math.nan, math.inf)]
+    rows = 2 * len(bad) + 3
+    z = torch.randn(rows, v, generator=g).to(DT[mode]).to(dev)
+    t = torch.randn(rows, k, generator=g)
+    i = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(rows)])
+    if k > 2:
+        i[:, 1] = torch.where(torch.arange(rows) % 2 == 0, i[:, 1], torch.tensor(-1))        # an unused slot in every second row
+    where = []
+    for n, (slot, value) in enumerate(bad):
+        row = 2 * n + 1
+        t[row, slot] = value
+        if int(i[row, slot]) >= 0:
+            where.append(row)
+    t[rows - 1] = math.nan                                 # and a list of nothing else
+    where.append(rows - 1)
+    spoilt = torch.zeros(rows, dtype=torch.bool)
+    spoilt[where] = True
+    t, i = t.to(t_dtype).to(dev), i.to(dev)
+    z.requires_grad_(True)
+    each = unet_amd.TopLogitDistillationLoss(2.0, "none")
+    with torch.no_grad():
+        assert torch.equal(torch.isnan(each(z, t, i)).cpu(), spoilt)
+    out = each(z, t, i)
+    assert torch.equal(torch.isnan(out).cpu(), spoilt) and torch.isfinite(out[~spoilt.to(dev)]).all()
+    (dz,) = torch.autograd.grad(out, z, torch.ones_like(out))
+    listed = torch.zeros(rows, v + 1, dtype=torch.bool, device=dev).scatter_(1, torch.where(i < 0, v, i), True)[:, :v]
+    assert torch.equal(torch.isnan(dz), listed & spoilt.to(dev)[:, None])
+    for reduction in ("mean", "sum"):
+        fn = unet_amd.TopLogitDistillationLoss(2.0, reduction)
+        out = fn(z, t, i)
+        assert torch.isnan(out)
+        (dz,) = torch.autograd.grad(out, z)
+        assert torch.equal(torch.isnan(dz), listed & spoilt.to(dev)[:, None])
+        keep = torch.where(spoilt.to(dev)[:, None], torch.full_like(i, -1), i)               # the rows left out
+        assert torch.isfinite(fn(z, t, keep))
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("v,k", [(16, 4), (300, 16), (5000, 8)])
+def test_a_teacher_pixel_of_nan_reaches_the_loss_through_its_top_logits(dev, mode, v, k):
+    g = torch.Generator().manual_seed(v)
+    teacher = torch.randn(6, v, generator=g).to(DT[mode]).to(dev)
+    z = torch.randn(6, v, generator=g).to(DT[mode]).to(dev)
+    teacher[2, v // 3] = math.nan
+    t, i = ops.top_logits(teacher, k)
+    assert torch.isnan(t[2, 0])
+    out = unet_amd.TopLogitDistillationLoss(2.0, "none")(z, t, i)
+    assert torch.isnan(out).tolist() == [False, False, True, False, False, False]

@@ -75,7 +75,7 @@ struct ListSum {
     }
     __device__ __forceinline__ void rescale(float to, float inv_t) {
         const float d = (m - to) * inv_t, f = __builtin_amdgcn_exp2f(d * LOG2E);
-        if (f == 0.0f) { s = 0.0f; a = 0.0f; }                    // also the first slot: m = -inf
+        if (f == 0.0f) { s *= f; a = s; }                         // also the first slot: m = -inf; a NaN in s stays, an infinite a does not
         else { a = f * fmaf(d, s, a); s *= f; }
         m = to;
     }
