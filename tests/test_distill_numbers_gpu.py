@@ -1,8 +1,9 @@
-"""The distillation loss where its numbers are hard: NaN and infinities in the teacher's lists."""
+"""The distillation loss where it is easily wrong without a word: NaN and infinities in the teacher's lists, tangents."""
 import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import unet_amd
 from unet_amd import ops
@@ -67,3 +68,19 @@ def test_a_teacher_pixel_of_nan_reaches_the_loss_through_its_top_logits(dev, mod
     assert torch.isnan(t[2, 0])
     out = unet_amd.TopLogitDistillationLoss(2.0, "none")(z, t, i)
     assert torch.isnan(out).tolist() == [False, False, True, False, False, False]
+
+
+@pytest.mark.parametrize("rows,v", [(5, 16), (5, 5000)])
+def test_forward_mode_tangents_are_refused(dev, rows, v):
+    """A tangent that the loss cannot carry on must not vanish without a word."""
+    z = torch.randn(rows, v, device=dev)
+    t, i = torch.randn(rows, 3, device=dev), torch.zeros(rows, 3, dtype=torch.int32, device=dev)
+    fn = unet_amd.TopLogitDistillationLoss()
+    with forward_ad.dual_level():
+        plain = fn(z, t, i)                                # no tangent: nothing to refuse
+        dual = forward_ad.make_dual(z, torch.ones_like(z))
+        with pytest.raises(RuntimeError):
+            fn(dual, t, i)
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            fn(dual, t, i)
+    assert torch.equal(plain, fn(z, t, i))

@@ -9,6 +9,7 @@ import functools
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _DT, _pixels
@@ -233,6 +234,8 @@ class TopLogitDistillationLoss(nn.Module):
             total = x.float().sum(-1)                              # nothing to learn from: zeros that know the input
             return total if red == 0 else total.sum()
         t, i = t.contiguous(), i.contiguous()
-        if x.requires_grad and torch.is_grad_enabled():
+        # a tangent of forward-mode differentiation is refused by autograd; without a level there is none (asking takes 1 us)
+        tangent = forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
+        if tangent or x.requires_grad and torch.is_grad_enabled():
             return _DistillFunction.apply(x, t, i, self.temperature, self.weight, red)
         return _distill_call(x, t, i, self.temperature, self.weight, red, False)[0]
