@@ -1,5 +1,7 @@
-"""The distillation loss where it is easily wrong without a word: NaN and infinities in the teacher's lists, tangents."""
+"""The distillation loss where it is easily wrong without a word: NaN and infinities in the teacher's lists, tangents, and what is kept
+between forward and backward."""
 import math
+import threading
 
 import pytest
 import torch
@@ -84,3 +86,71 @@ def test_forward_mode_tangents_are_refused(dev, rows, v):
         with torch.no_grad(), pytest.raises(RuntimeError):
             fn(dual, t, i)
     assert torch.equal(plain, fn(z, t, i))
+
+
+# ---- the gradient that the forward call of long rows leaves behind -----------------------------------------------------
+# Written by the forward call or computed again, a gradient scale (p - q) is off by (V / 256 + 64 + 8 |x|) u of scale p, at a listed class also by
+# (2 k + 32 + 8 |y|) u of scale q, u = 2^-24 (sums, exponents, weights); with V <= 9000, k = 5 and |x|, |y| <= 8: 163 u and 106 u.  Twice that between two.
+def close(a, b, scale):
+    return ((a - b).abs() <= 2 * 163 * 2.0 ** -24 * b.abs() + 2 * (163 + 106) * 2.0 ** -24 * scale).all()
+
+
+def test_saved_tensor_hooks_see_all_that_a_training_step_keeps(dev):
+    rows, v = 300, 9000
+    g = torch.Generator().manual_seed(1)
+    z = torch.randn(rows, v, generator=g).to(dev).requires_grad_(True)
+    t, i = torch.randn(rows, 5, generator=g).to(dev), torch.randint(0, v, (rows, 5), generator=g).to(dev)
+    fn = unet_amd.TopLogitDistillationLoss(2.0)
+    (want,) = torch.autograd.grad(fn(z, t, i), z)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(dev)
+    with torch.autograd.graph.save_on_cpu():
+        out = fn(z, t, i)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated(dev) - before < z.numel()              # bytes: a quarter of the gradient
+    (dz,) = torch.autograd.grad(out, z, retain_graph=True)
+    (again,) = torch.autograd.grad(out, z, torch.full((), 3.0, device=dev))
+    assert torch.equal(dz, want)
+    assert close(again, 3.0 * want, 3.0 * 2.0 / rows)
+
+
+def test_threads_share_a_retained_graph(dev):
+    """Every backward call gets a tensor of its own, also when several threads run them at once and change what they get."""
+    rows, v = 64, 5000
+    g = torch.Generator().manual_seed(2)
+    z = torch.randn(rows, v, generator=g).to(dev).requires_grad_(True)
+    t, i = torch.randn(rows, 5, generator=g).to(dev), torch.randint(0, v, (rows, 5), generator=g).to(dev)
+    fn = unet_amd.TopLogitDistillationLoss(2.0)
+    for _ in range(10):
+        out = fn(z, t, i)
+        got, start = [], threading.Barrier(4)
+
+        def run():
+            start.wait()
+            (dz,) = torch.autograd.grad(out, z, retain_graph=True)
+            got.append(dz)
+
+        threads = [threading.Thread(target=run) for _ in range(4)]
+        for th in threads:
+            th.start()
+        for th in threads:
+            th.join()
+        torch.cuda.synchronize()
+        assert len(got) == 4 and len({d.data_ptr() for d in got}) == 4
+        assert all(close(d, got[0], 2.0 / rows) for d in got)
+    (first,) = torch.autograd.grad(out, z, retain_graph=True)
+    kept = first.clone()
+    first.zero_()                                          # the caller's own
+    (second,) = torch.autograd.grad(out, z)
+    assert torch.equal(second, kept)
+
+
+def test_gradients_accumulate_over_a_retained_graph(dev):
+    z = torch.randn(40, 5000, device=dev, requires_grad=True)
+    t, i = torch.randn(40, 5, device=dev), torch.randint(0, 5000, (40, 5), device=dev)
+    out = unet_amd.TopLogitDistillationLoss(2.0)(z, t, i)
+    out.backward(retain_graph=True)
+    once = z.grad.clone()
+    out.backward(retain_graph=True)
+    out.backward()
+    assert close(z.grad, 3.0 * once, 3.0 * 2.0 / 40)

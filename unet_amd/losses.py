@@ -146,15 +146,16 @@ def _distill_call(logits, teacher, index, temperature, weight, red, train):
 
 
 def _distill_gradient(ctx, gout):
-    logits, teacher, index, saved = ctx.saved_tensors
+    logits, teacher, index, saved, dz = ctx.saved_tensors
     temperature, weight, red = ctx.cfg
     lib, dev = _lib.load(), logits.device
     z, pitch = _pixels(logits, "input")
     v, k = z.shape[-1], index.shape[-1]
-    dz, ctx.dz = ctx.dz, None        # given away by the first backward call
-    done = dz is not None
-    if not done:
-        dz = z.new_empty(z.shape)
+    try:                                     # the first backward call gives it away (one of several threads: a list pops once)
+        done = ctx.first.pop()
+    except IndexError:
+        done = False
+    dz = dz.data if done else z.new_empty(z.shape)       # the receiver may change it in place: not the saved tensor itself
     g = gout if gout.dtype == torch.float32 and gout.is_contiguous() else gout.contiguous().float()
     with _lib.on_device(dev):
         _lib.check(lib.mi_distill_loss_bwd(_DT[z.dtype], index.numel() // k, v, pitch, z.data_ptr(), k, _DT[teacher.dtype], teacher.data_ptr(),
@@ -169,8 +170,9 @@ _distill_gradient_once = torch.autograd.function.once_differentiable(_distill_gr
 class _DistillFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher, index, temperature, weight, red):
-        loss, saved, ctx.dz = _distill_call(logits, teacher, index, temperature, weight, red, True)
-        ctx.save_for_backward(logits, teacher, index, saved)
+        loss, saved, dz = _distill_call(logits, teacher, index, temperature, weight, red, True)
+        ctx.save_for_backward(logits, teacher, index, saved, dz)
+        ctx.first = [True] if dz is not None else []
         ctx.cfg = (temperature, weight, red)
         return loss
 
