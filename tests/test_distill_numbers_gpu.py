@@ -1,8 +1,9 @@
-"""The distillation loss where it is easily wrong without a word: NaN and infinities in the teacher's lists, tangents, and what is kept
-between forward and backward."""
+"""The distillation loss where it is easily wrong without a word: NaN and infinities in the teacher's lists, tangents, what is kept
+between forward and backward, temperatures at which its terms cancel."""
 import math
 import threading
 
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -154,3 +155,107 @@ def test_gradients_accumulate_over_a_retained_graph(dev):
     out.backward(retain_graph=True)
     out.backward()
     assert close(z.grad, 3.0 * once, 3.0 * 2.0 / 40)
+
+
+# ---- temperatures -----------------------------------------------------------------------------------------------------
+# The definition in numpy's long double (2^-64: T^2 times the 64-bit one's own error passes the loss at T = 1e6), and a row's tolerance, u = 2^-24.
+# x_j = log q_j - log p_j.  Short rows add q_j phi(x_j), phi(x) = x - 1 + exp(-x), and R = 1 - sum p_j.  An x is off by dx = (3 |a| + 3 |b| + 3 |a - b|) u / T
+# + 2 |x| u (a, b: gaps of t and z to their maxima; differences, 1 / T, products) and, all alike, by d = (V / 64 + k + 16 + 2 ln V + mean |a| / T) u (sums, two
+# logarithms), which enters as R d and d^2 / 2.  A weight q is off by eq = (k + 8 + 4 |a| / T) u relatively, a probability by ep = (V / 64 + 12 + 4 |b| / T) u.
+# For |x| < 1/2 (up to dx) phi is a series: q (|x| dx + phi (eq + 16 u)); beyond, q dx + (q (|x| + 1) + p) (eq + ep + 16 u).
+# R: fp64 sums above T = 4, R (16 + 4 max |b| / T) u; below, sums of fp32 are off by at most 32 u (and so is what they set to zero).
+# Long rows: T^2 u (V / 256 + 2 k + 64 + 8 (1 + M)^2), M the largest |a| or |b| over T of a listed class.
+U = 2.0 ** -24
+
+
+def rows_in_long_double(z, t, i, temperature, short):
+    L = np.longdouble
+    T = L(np.float32(temperature))
+    z, t, i = z.float().cpu().numpy().astype(L), t.float().cpu().numpy().astype(L), i.cpu().numpy()
+    loss, tol = [], []
+    v, k = z.shape[1], t.shape[1]
+    for zr, tr, ir in zip(z, t, i):
+        used = (ir >= 0) & (ir < v) & (tr > -np.inf)
+        tr, ir = tr[used], ir[used]
+        b, a = zr - zr.max(), tr - tr.max()
+        with np.errstate(all="ignore"):
+            lp, lq = b / T - np.log(np.exp(b / T).sum()), a / T - np.log(np.exp(a / T).sum())
+            p, q, bl = np.exp(lp), np.exp(lq), b[ir]
+            x = np.where(q > 0, lq - lp[ir], 0)
+            pj = p[ir]
+            loss.append(T * T * np.where(q > 0, q * x, 0).sum())
+            A, B = np.abs(a) / T, np.where(np.isfinite(bl), np.abs(bl), 0) / T
+            if not short:
+                M = max(np.where(q > 1e-30, np.maximum(A, B), 0).max(), 0)
+                tol.append(T * T * U * (v / 256 + 2 * k + 64 + 8 * (1 + M) ** 2))
+                continue
+            dx = (3 * A + 3 * B + 3 * np.where(np.isfinite(bl), np.abs(a - bl), 0) / T) * U + 2 * np.abs(x) * U
+            d = (v / 64 + k + 16 + 2 * np.log(L(v)) + (q * A).sum()) * U
+            eq, ep = (k + 8 + 4 * A) * U, (v / 64 + 12 + 4 * B) * U
+            phi = x - 1 + np.exp(-x)
+            near = q * (np.abs(x) * dx + dx * dx + np.abs(phi) * (eq + 16 * U))
+            far = q * dx + (q * (np.abs(x) + 1) + pj) * (eq + ep + 16 * U)
+            e = np.where(np.abs(x) < 0.5 - dx, near, np.where(np.abs(x) > 0.5 + dx, far, np.maximum(near, far))).sum()
+            R = abs(1 - pj.sum())
+            most = np.where(p > 0, np.abs(np.where(p > 0, b, 0)), 0).max() / T
+            e += R * d + (R * (16 + 4 * most) * U if temperature > 4 else 32 * U) + (64 * U * d if temperature > 4 else d * d)
+            tol.append(T * T * e + 8 * U * abs(loss[-1]))
+    return np.array(loss, dtype=np.float64), np.array(tol, dtype=np.float64)
+
+
+def check_rows(z, t, i, temperature, short):
+    want, tol = rows_in_long_double(z, t, i, temperature, short)
+    got = unet_amd.TopLogitDistillationLoss(temperature, "none")(z, t, i).double().cpu().numpy()
+    err = np.abs(got - want)
+    assert (err <= tol + 1e-37).all(), (temperature, float((err / (tol + 1e-37)).max()), float(got[(err / (tol + 1e-37)).argmax()]), float(want[(err / (tol + 1e-37)).argmax()]))
+    return got, want, tol
+
+
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 4.0, 4.5, 20.0, 100.0, 1e3, 1e4, 1e6])
+@pytest.mark.parametrize("v,k", [(1, 1), (2, 2), (5, 2), (16, 16), (16, 4), (40, 40), (133, 100), (256, 256), (300, 256), (600, 20), (1000, 200)])
+def test_short_rows_keep_their_digits_at_any_temperature(dev, v, k, temperature):
+    g = torch.Generator().manual_seed(v + k)
+    for spread in (2.0, 20.0):
+        z = torch.randn(24, v, generator=g) * spread
+        i = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(24)])
+        t = z.gather(1, i) + 0.5 * torch.randn(24, k, generator=g)
+        t[::6] = z.gather(1, i)[::6]                       # a student that agrees
+        for zt in (torch.float32, torch.bfloat16):
+            got, want, tol = check_rows(z.to(zt).to(dev), t.to(dev), i.to(dev), temperature, True)
+            assert (got >= -tol).all()                     # no class twice: a divergence
+
+
+@pytest.mark.parametrize("temperature", [1.0, 20.0, 1e3])
+@pytest.mark.parametrize("v,k", [(16, 16), (64, 64), (900, 10)])
+def test_what_a_short_list_cancels(dev, v, k, temperature):
+    """The figure in words: the loss of lists that hold all the mass, 0.02 to 0.3 here, is good to 2^-14 of itself."""
+    g = torch.Generator().manual_seed(v)
+    i = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(64)])
+    z = torch.randn(64, v, generator=g)
+    z = torch.full_like(z, -math.inf).scatter_(1, i, z.gather(1, i))                       # classes that are not listed are masked
+    t = z.gather(1, i) + 0.5 * torch.randn(64, k, generator=g)
+    got, want, tol = check_rows(z.to(dev), t.to(dev), i.to(dev), temperature, True)
+    big = want > 0.02
+    assert big.sum() > 32 and (np.abs(got - want)[big] <= 2.0 ** -14 * want[big]).all()
+
+
+@pytest.mark.parametrize("temperature", [0.5, 2.0, 50.0])
+@pytest.mark.parametrize("v,k", [(16, 20), (3, 200), (400, 64)])
+def test_short_lists_with_repeats_and_unused_slots(dev, v, k, temperature):
+    g = torch.Generator().manual_seed(v)
+    z = torch.randn(30, v, generator=g) * 3
+    i = torch.randint(-1, v + 1, (30, k), generator=g)
+    i[:, 0] = 0
+    t = torch.randn(30, k, generator=g) * 3
+    check_rows(z.to(dev), t.to(dev), i.to(dev), temperature, True)
+
+
+@pytest.mark.parametrize("temperature", [0.5, 20.0, 1e3])
+@pytest.mark.parametrize("v,k", [(3000, 5), (5000, 256), (40000, 40)])
+def test_long_rows_at_high_temperatures(dev, v, k, temperature):
+    g = torch.Generator().manual_seed(v)
+    z = torch.randn(7, v, generator=g) * 3
+    i = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(7)])
+    t = z.gather(1, i) + 0.5 * torch.randn(7, k, generator=g)
+    for zt in (torch.float32, torch.bfloat16):
+        check_rows(z.to(zt).to(dev), t.to(dev), i.to(dev), temperature, False)

@@ -5,9 +5,15 @@
 //   row loss = w T^2 sum_j q_j (log q_j - log p_{i_j}) ;  dz_v = w T gout (p_v - sum_{j: i_j = v} q_j)
 //   mean: over the rows with a used slot; the other rows give a loss and a gradient of exactly 0, whatever z holds there.
 //
-// With zm = max z, tm = max t, e_j = exp((t_j - tm) / T): the row loss is w T^2 (A / St - log St + log Sz) where
-// A = sum e_j ((t_j - tm) - (z_{i_j} - zm)) / T, St = sum e_j and Sz = sum exp((z - zm) / T): one pass over the row, one
-// over the list, nothing that cancels.
+// With zm = max z, tm = max t, St = sum_j exp((t_j - tm) / T), Sz = sum exp((z - zm) / T) and x_j = log q_j - log p_{i_j}:
+//   long rows : w T^2 (A / St - log St + log Sz), A = sum_j exp((t_j - tm) / T) ((t_j - tm) - (z_{i_j} - zm)) / T.  One pass over the list; off by
+//               a few 2^-24 T^2, which the loss of a list of at most 256 of so many classes exceeds
+//   short rows: a list may hold all classes, and those terms then cancel down to 1 / T^2 of their size (16 of 16 classes: 2e-5 of the loss at
+//               T = 1, 4 % at 100).  There sum_j q_j (x_j - 1 + exp(-x_j)) + R, R = 1 - sum_j p_{i_j}, of which no part is negative where no class
+//               repeats.  An error d that all x_j share (that of log St - log Sz) comes in as d^2 / 2.  R is what is left of Sz without the listed classes:
+//               up to T = WIDE_T fp32 sums, which are off by 32 u at most (u = 2^-24), T^2 32 u = 2^-15 of weight in the loss; what lies below that is set
+//               to 0.  Above, Sz and the listed part are added in fp64, where the same fp32 exponentials leave exactly nothing behind, and d is taken
+//               out again: h = sum_j q_j expm1(-x_j) + R = -d, which - h^2 / 2 removes (d^2 / 2 alone: 5e-4 of the loss of 16 of 16 classes at T = 1e6)
 //
 // Bandwidth-bound: the forward pass cannot do without one read of z, the backward pass without one read and one write.
 //   short rows (up to 4 KB): L neighbouring lanes share a row and hold it in registers
@@ -27,13 +33,15 @@ constexpr int MAX_K = 256;
 constexpr int NVMAX = 4;              // 16-byte vectors of a row that a lane holds
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LN2 = 0.69314718055994531;
+// The loss of short rows adds in fp64 above this temperature: 500000 x 256 bf16 63 -> 69 us, 100000 x 2000 bf16 104 -> 123, 2097152 x 16 bf16 42.5 -> 44.
+constexpr float WIDE_T = 4.0f;
 
 struct DistParams {
     const char *z, *t, *idx;
     char* dz;
     int64_t rows, zp, dzp;            // pitches in bytes
     int v, k, t_bf16, i64, red, L;    // red: 0 none, 1 mean, 2 sum
-    float c, inv_t, wl, wg;           // log2(e) / T, 1 / T, weight * T^2 (loss), weight * T (gradient)
+    float temp, c, inv_t, wl, wg;     // T, log2(e) / T, 1 / T, weight * T^2 (loss), weight * T (gradient)
     float* loss;                      // [rows] (none) or [1]
     float2* stat;                     // long rows: {max z, Sz}
     double* sums;                     // {sum of the rows' losses, rows with a used slot}
@@ -152,7 +160,28 @@ struct Row {
             }
         return lanes_sum(s, L);
     }
+    // the sum of exp((x - m) / T) in fp64
+    __device__ __forceinline__ double exp_sum(float m, float c, int L) const {
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < TR::VEC; ++j) s += (double)__builtin_amdgcn_exp2f((x[i][j] - m) * c);
+        return lanes_sum(s, L);
+    }
 };
+
+// x - 1 + exp(-x) for |x| < 1/2: its series, cut where the next term is less than 2^-24 of the sum
+__device__ __forceinline__ float small_part(float x) {
+    float s = 1.0f / 40320.0f;
+    s = fmaf(s, x, -1.0f / 5040.0f);
+    s = fmaf(s, x, 1.0f / 720.0f);
+    s = fmaf(s, x, -1.0f / 120.0f);
+    s = fmaf(s, x, 1.0f / 24.0f);
+    s = fmaf(s, x, -1.0f / 6.0f);
+    s = fmaf(s, x, 0.5f);
+    return s * x * x;
+}
 
 // {a, b} added over a workgroup of T threads in a fixed order; thread 0 has the sums
 template <int T>
@@ -235,7 +264,7 @@ struct Slots {
 };
 
 // the logits and the list are requested one row ahead
-template <class TR, int NV, int SL>
+template <class TR, int NV, int SL, bool WIDE>
 __global__ __launch_bounds__(TPB) void distill_short_fwd(DistParams p) {
     const int L = p.L, l = threadIdx.x & (L - 1), per = TPB / L;
     double loss = 0.0, count = 0.0;
@@ -254,21 +283,71 @@ __global__ __launch_bounds__(TPB) void distill_short_fwd(DistParams p) {
         const char* z = p.z + (in ? r : 0) * p.zp;
         Row<TR, NV> x;
         x.take(raw, z, p.v, L, l);
-        const Slots<SL> now = next;
-        float zi[SL];
+        float t[SL], zi[SL];                                      // -inf: not used
 #pragma unroll
-        for (int n = 0; n < SL; ++n) zi[n] = now.cls(p, n) >= 0 ? ld_one<TR>(z, now.cls(p, n)) : 0.0f;
+        for (int n = 0; n < SL; ++n) {
+            const int cls = next.cls(p, n);
+            t[n] = cls >= 0 ? next.teacher(p, n) : -INFINITY;
+            zi[n] = cls >= 0 ? ld_one<TR>(z, cls) : 0.0f;
+        }
         if (r0 + step < p.rows) fetch(r + step);
-        const float m = x.max_of(L), s = x.exp_of(m, p.c, L);
-        ListSum q;
+        const float m = x.max_of(L);
+        float s = 0.0f;
+        double wide = 0.0;
+        if constexpr (WIDE) { wide = x.exp_sum(m, p.c, L); s = (float)wide; }
+        else s = x.exp_of(m, p.c, L);
+        float tm = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < SL; ++n)
-            if (now.cls(p, n) >= 0) q.add(now.teacher(p, n), (zi[n] - m) * p.inv_t, p.inv_t);
-        q.join(L, p.inv_t);
+        for (int n = 0; n < SL; ++n) tm = fmaxf(tm, t[n]);
+        tm = lanes_max(tm, L);
+        float et[SL], ez[SL], gap[SL], st = 0.0f;
+        std::conditional_t<WIDE, double, float> listed = 0.0f;
+#pragma unroll
+        for (int n = 0; n < SL; ++n) {
+            et[n] = ez[n] = gap[n] = 0.0f;
+            if (n && n * L >= p.k) continue;                      // no lane has such a slot
+            const bool used = t[n] != -INFINITY;
+            const float a = t[n] - tm, b = zi[n] - m;
+            et[n] = used ? __builtin_amdgcn_exp2f(a * p.c) : 0.0f;
+            ez[n] = used ? __builtin_amdgcn_exp2f(b * p.c) : 0.0f;
+            gap[n] = used ? a - b : 0.0f;
+            st += et[n]; listed += ez[n];
+        }
+        st = lanes_sum(st, L);                                    // 0: no slot is used
+        listed = lanes_sum(listed, L);
+        const float inv_z = __builtin_amdgcn_rcpf(s), inv_q = __builtin_amdgcn_rcpf(st);      // good to one unit; s and st are 1 at least
+        float rest;
+        if constexpr (WIDE) {
+            rest = (float)(wide - listed) * inv_z;
+        } else {
+            rest = (s - listed) * inv_z;
+            if (fabsf(rest) < 0x1p-19f) rest = 0.0f;              // 32 steps of fp32: such sums cannot tell it from nothing
+        }
+        const float shift = (__builtin_amdgcn_logf(st) - __builtin_amdgcn_logf(s)) * (float)LN2;
+        // far: q x T, in natural units (over T a class masked with the type's lowest value could pass the end of fp32)
+        float part = 0.0f, small = 0.0f, far = 0.0f;
+#pragma unroll
+        for (int n = 0; n < SL; ++n) {
+            if (n && n * L >= p.k) continue;
+            const float q = et[n] * inv_q, d = fmaf(gap[n], p.inv_t, -shift);
+            const bool near = fabsf(d) < 0.5f;
+            part += near ? q * small_part(d) : fmaf(ez[n], inv_z, -q);
+            far += near || q == 0.0f ? 0.0f : q * fmaf(-p.temp, shift, gap[n]);
+            if constexpr (WIDE) small += near ? q * d : 0.0f;
+        }
+        float row;
+        if constexpr (WIDE) {
+            part = lanes_sum(part, L) + rest;
+            const float h = part - lanes_sum(small, L);
+            row = fmaf(p.wl, fmaf(-0.5f * h, h, part), p.wg * lanes_sum(far, L));
+        } else {
+            row = fmaf(p.wl, rest, lanes_sum(fmaf(p.wl, part, p.wg * far), L));
+        }
         if (l == 0 && in) {
-            const float row = q.some ? q.loss(s, p.wl) : 0.0f;
+            const bool some = st != 0.0f;
+            if (!some) row = 0.0f;
             if (p.red == 0) p.loss[r] = row;
-            if (q.some) { loss += row; count += 1.0; }
+            if (some) { loss += row; count += 1.0; }
         }
     }
     if (p.red) block_part<TPB>(p, loss, count);
@@ -886,7 +965,7 @@ void fill(DistParams& p, const Plan& q, int dtype, int64_t rows, int v, int64_t 
     p.z = (const char*)logits; p.t = (const char*)teacher; p.idx = (const char*)index;
     p.rows = rows; p.v = v; p.k = k; p.zp = pitch * (dtype ? 2 : 4); p.t_bf16 = t_dtype; p.i64 = i_dtype == 2; p.red = reduction;
     p.L = q.L; p.nparts = q.blocks;
-    p.wl = weight * temperature * temperature; p.wg = weight * temperature;
+    p.temp = temperature; p.wl = weight * temperature * temperature; p.wg = weight * temperature;
     p.inv_t = 1.0f / temperature; p.c = (float)(1.4426950408889634 / (double)temperature);
     p.sums = (double*)saved; p.part = p.sums + 2;
     p.counts = p.part + 2 * q.parts;
@@ -931,8 +1010,13 @@ int mi_distill_loss_fwd(int dtype, int64_t rows, int v, int64_t pitch, const voi
         }
         MI_HIP(hipGetLastError());
     } else {
-        if (q.sl == 1) SHORT_NV(distill_short_fwd, q.nv, q.blocks, 0, COMMA 1);
-        else SHORT_NV(distill_short_fwd, q.nv, q.blocks, 0, COMMA 4);
+        if (temperature > WIDE_T) {
+            if (q.sl == 1) SHORT_NV(distill_short_fwd, q.nv, q.blocks, 0, COMMA 1 COMMA true);
+            else SHORT_NV(distill_short_fwd, q.nv, q.blocks, 0, COMMA 4 COMMA true);
+        } else {
+            if (q.sl == 1) SHORT_NV(distill_short_fwd, q.nv, q.blocks, 0, COMMA 1 COMMA false);
+            else SHORT_NV(distill_short_fwd, q.nv, q.blocks, 0, COMMA 4 COMMA false);
+        }
     }
     if (reduction) {
         distill_final<<<1, 1024, 0, st>>>(p);

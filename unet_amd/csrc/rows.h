@@ -80,3 +80,26 @@ __device__ __forceinline__ float lanes_sum(float v, int L) {
 }
 __device__ __forceinline__ unsigned lanes_max(unsigned v, int L) { return lanes_join(v, L, [](unsigned a, unsigned b) { return max(a, b); }); }
 __device__ __forceinline__ unsigned lanes_min(unsigned v, int L) { return lanes_join(v, L, [](unsigned a, unsigned b) { return min(a, b); }); }
+// the same for a double, half by half
+template <int CTRL>
+__device__ __forceinline__ double lane_move(double v) {
+    return __hiloint2double((int)lane_move<CTRL>((unsigned)__double2hiint(v)), (int)lane_move<CTRL>((unsigned)__double2loint(v)));
+}
+__device__ __forceinline__ double lanes_sum(double v, int L) {
+    if (L == 1) return v;
+    v += lane_move<0xB1>(v);
+    if (L == 2) return v;
+    v += lane_move<0x4E>(v);
+    if (L == 4) return v;
+    v += lane_move<0x141>(v);
+    if (L == 8) return v;
+    v += lane_move<0x140>(v);
+    if (L == 16) return v;
+    const unsigned hi = (unsigned)__double2hiint(v), lo = (unsigned)__double2loint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(hi, hi, false, false), b = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    v = __hiloint2double((int)a[0], (int)b[0]) + __hiloint2double((int)a[1], (int)b[1]);
+    if (L == 32) return v;
+    const unsigned hi2 = (unsigned)__double2hiint(v), lo2 = (unsigned)__double2loint(v);
+    const auto c = __builtin_amdgcn_permlane32_swap(hi2, hi2, false, false), d = __builtin_amdgcn_permlane32_swap(lo2, lo2, false, false);
+    return __hiloint2double((int)c[0], (int)d[0]) + __hiloint2double((int)c[1], (int)d[1]);
+}
