@@ -259,3 +259,26 @@ def test_long_rows_at_high_temperatures(dev, v, k, temperature):
     t = z.gather(1, i) + 0.5 * torch.randn(7, k, generator=g)
     for zt in (torch.float32, torch.bfloat16):
         check_rows(z.to(zt).to(dev), t.to(dev), i.to(dev), temperature, False)
+
+
+@pytest.mark.parametrize("temperature", [0.01, 0.5, 1.0])
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("v,k", [(16, 4), (300, 70), (5000, 4), (5000, 100)])
+def test_listed_classes_masked_with_the_lowest_value(dev, mode, v, k, temperature):
+    """Temperatures below 1 make the gap to such a class larger than fp32 holds; the loss, T times q times the gap, is not."""
+    g = torch.Generator().manual_seed(v + k)
+    z = torch.randn(6, v, generator=g) * 2
+    i = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(6)])
+    t = torch.randn(6, k, generator=g) * temperature
+    for row, slot in ((0, 0), (1, k // 2), (2, k - 1)):
+        z[row, i[row, slot]] = torch.finfo(DT[mode]).min
+    z = z.to(DT[mode]).to(dev)
+    for reduction in ("none", "sum"):
+        fn = unet_amd.TopLogitDistillationLoss(temperature, reduction)
+        leaf = z.clone().requires_grad_(True)
+        out = fn(leaf, t.to(dev), i.to(dev))
+        assert torch.isfinite(out).all()
+        (dz,) = torch.autograd.grad(out.sum(), leaf)
+        assert torch.isfinite(dz).all()
+    got, want, tol = check_rows(z, t.to(dev), i.to(dev), temperature, v <= 1024)
+    assert (want[:3] > 1e33).all()

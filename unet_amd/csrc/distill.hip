@@ -31,7 +31,6 @@ namespace {
 constexpr int TPB = 256;
 constexpr int MAX_K = 256;
 constexpr int NVMAX = 4;              // 16-byte vectors of a row that a lane holds
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LN2 = 0.69314718055994531;
 // The loss of short rows adds in fp64 above this temperature: 500000 x 256 bf16 63 -> 69 us, 100000 x 2000 bf16 104 -> 123, 2097152 x 16 bf16 42.5 -> 44.
 constexpr float WIDE_T = 4.0f;
@@ -68,35 +67,35 @@ __host__ __device__ inline int count_lanes(int k) {
     return L;
 }
 
-// running maximum, sum and weighted gap of a list; natural units (to base 2 a student's class masked with the type's lowest
-// value would pass the end of fp32)
+// running maximum, sum and weighted gap of a list; gaps in natural units, not over T (T below 1 would take that of a student's class masked with the
+// type's lowest value past the end of fp32)
 struct ListSum {
     float m = -INFINITY, s = 0.0f, a = 0.0f;
     bool some = false;
-    // gap_z = (z - zm) / T
-    __device__ __forceinline__ void add(float t, float gap_z, float inv_t) {
+    // gap_z = z - zm
+    __device__ __forceinline__ void add(float t, float gap_z, float c) {
         if (t == -INFINITY) return;
         some = true;
-        if (t > m) rescale(t, inv_t);
-        const float x = (t - m) * inv_t, e = __builtin_amdgcn_exp2f(x * LOG2E);
-        if (e != 0.0f) { s += e; a = fmaf(e, x - gap_z, a); }
+        if (t > m) rescale(t, c);
+        const float gap = t - m, e = __builtin_amdgcn_exp2f(gap * c);
+        if (e != 0.0f) { s += e; a = fmaf(e, gap - gap_z, a); }
     }
-    __device__ __forceinline__ void rescale(float to, float inv_t) {
-        const float d = (m - to) * inv_t, f = __builtin_amdgcn_exp2f(d * LOG2E);
+    __device__ __forceinline__ void rescale(float to, float c) {
+        const float gap = m - to, f = __builtin_amdgcn_exp2f(gap * c);
         if (f == 0.0f) { s *= f; a = s; }                         // also the first slot: m = -inf; a NaN in s stays, an infinite a does not
-        else { a = f * fmaf(d, s, a); s *= f; }
+        else { a = f * fmaf(gap, s, a); s *= f; }
         m = to;
     }
     // join the lists of L neighbouring lanes: every lane ends with the whole list
-    __device__ __forceinline__ void join(int L, float inv_t) {
+    __device__ __forceinline__ void join(int L, float c) {
         const float to = lanes_max(m, L);
         some = (bool)lanes_max(some ? 1.0f : 0.0f, L);
-        if (some && m != to) rescale(to, inv_t);
+        if (some && m != to) rescale(to, c);
         a = lanes_sum(a, L);
         s = lanes_sum(s, L);
     }
-    __device__ __forceinline__ float loss(float sz, float scale) const {
-        return scale * (a / s + (__builtin_amdgcn_logf(sz) - __builtin_amdgcn_logf(s)) * (float)LN2);
+    __device__ __forceinline__ float loss(float sz, const DistParams& p) const {
+        return fmaf(p.wg, a / s, p.wl * ((__builtin_amdgcn_logf(sz) - __builtin_amdgcn_logf(s)) * (float)LN2));
     }
 };
 
@@ -614,11 +613,11 @@ template <class TR>
 __device__ __forceinline__ void row_loss(const DistParams& p, int64_t r, const char* z, float2 st, ListSum& q, double& loss, double& count) {
     for (int j = 64 + (threadIdx.x & 63); j < p.k; j += 64) {
         const int i = list_i(p, r * p.k + j);
-        if (i >= 0) q.add(list_t(p, r * p.k + j), (ld_one<TR>(z, i) - st.x) * p.inv_t, p.inv_t);
+        if (i >= 0) q.add(list_t(p, r * p.k + j), ld_one<TR>(z, i) - st.x, p.c);
     }
-    q.join(64, p.inv_t);
+    q.join(64, p.c);
     if ((threadIdx.x & 63) == 0) {
-        const float row = q.some ? q.loss(st.y, p.wl) : 0.0f;
+        const float row = q.some ? q.loss(st.y, p) : 0.0f;
         p.stat[r] = st;
         if (p.red == 0) p.loss[r] = row;
         if (q.some) { loss += row; count += 1.0; }
@@ -676,7 +675,7 @@ __global__ __launch_bounds__(T) void distill_long_fwd(DistParams p) {
         if (tid < 64) {
             const float2 st = join_waves<T>(wm, ws, p.c);
             ListSum l;
-            if (li >= 0) l.add(lt, (lz - st.x) * p.inv_t, p.inv_t);
+            if (li >= 0) l.add(lt, lz - st.x, p.c);
             row_loss<TR>(p, r, z, st, l, loss, count);
         }
     }
@@ -792,11 +791,11 @@ __global__ __launch_bounds__(T, 4) void distill_long_step(DistParams p) {
         if (tid < 64) {
             ListSum ls;
             for (int j = tid; j < p.k; j += 64)
-                if (qi[j] >= 0) ls.add(qt[j], (qz[j] - st.x) * p.inv_t, p.inv_t);
-            ls.join(64, p.inv_t);
+                if (qi[j] >= 0) ls.add(qt[j], qz[j] - st.x, p.c);
+            ls.join(64, p.c);
             if (tid == 0) {
                 p.stat[r] = st;
-                if (ls.some) { loss += ls.loss(st.y, p.wl); count += 1.0; }
+                if (ls.some) { loss += ls.loss(st.y, p); count += 1.0; }
             }
         }
         __syncthreads();                                          // the classes of the list are written over
