@@ -333,7 +333,7 @@ int mi_top_logits(int dtype, int64_t rows, int v, int64_t pitch, const void* log
 /* Row loss weight * T^2 * KL(q || p): q = softmax(teacher / T) over the used slots of the row's list, p = softmax(logits / T) over all v
  * classes.  A slot is unused when its index lies outside [0, v) or its teacher logit is -inf; a class may be listed
  * more than once (its weights add).  Rows without a used slot have loss 0 and gradient 0, whatever their logits are.
- * temperature in 1e-6 .. 1e6.  teacher [rows][k] (teacher_dtype 0 fp32 | 1 bf16), index [rows][k] (index_dtype 2 int64 | 3 int32), 1 <= k <= 256.
+ * temperature in 1e-6 .. 1e6, weight * temperature^2 within fp32.  teacher [rows][k] (teacher_dtype 0 fp32 | 1 bf16), index [rows][k] (index_dtype 2 int64 | 3 int32), 1 <= k <= 256.
  * reduction: 0 none (loss [rows]), 1 mean over the rows with a used slot (0 if there are none), 2 sum (loss [1]).
  * `saved` (mi_distill_loss_saved_bytes, 16-byte aligned; 0: bad sizes) is written by the forward call and read by the backward call of the same
  * arguments.  grad_out: [rows] or [1], on the device; dlogits [rows][dpitch], type of the logits, v classes written.

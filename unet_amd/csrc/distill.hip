@@ -937,6 +937,7 @@ int check_args(const char* who, int dtype, int64_t rows, int v, int64_t pitch, c
         return bad("address is not a multiple of the element size");
     if (!(temperature >= 1e-6f && temperature <= 1e6f)) return bad("temperature must be in 1e-6 .. 1e6");
     if (!(weight - weight == 0.0f)) return bad("weight must be finite");
+    if (!(fabsf(weight * temperature * temperature) < INFINITY)) return bad("weight * temperature^2 must be within fp32");
     if (reduction < 0 || reduction > 2) return bad("unknown reduction");
     return 0;
 }

@@ -209,6 +209,8 @@ class TopLogitDistillationLoss(nn.Module):
             raise ValueError(f"temperature must be in 1e-6 .. 1e6, got {temperature}")
         if not abs(weight) < float("inf"):
             raise ValueError(f"weight must be finite, got {weight}")
+        if not abs(weight) * max(1.0, temperature, temperature * temperature) <= 3.4e38:
+            raise ValueError(f"weight * temperature**2 must be within fp32, got {weight} and {temperature}")
         if reduction not in _REDUCTION:
             raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
         self.temperature, self.reduction, self.weight = temperature, reduction, weight
