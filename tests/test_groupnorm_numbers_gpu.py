@@ -1,0 +1,58 @@
+"""Group norm where its numbers are hard.
+
+Statistics are sums in fp64 of values that fp64 holds exactly (squares too), so mean and 1 / sqrt(variance + eps) are their definitions rounded to
+fp32: off by u = 2^-24 of the mean, and of rstd by u plus what E[x^2] - mean^2 loses: additions of some hundred values a thread, each off by at most 2^-53 of a partial sum and in either direction, 2^-50
+(1 + mean^2 / variance).  y = (x - mean) rstd w + b then adds the
+difference's and two products' roundings and that of the mean over the deviation: 4 u |xh w| + u |mean| rstd |w| + u |y|."""
+import math
+
+import pytest
+import torch
+
+from unet_amd import ops
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def check_forward(x, groups, w, b, stored=0.0):
+    n, c = x.shape[0], x.shape[-1]
+    y, stats = ops.groupnorm_act_fwd(x, groups, w, b, act="none")
+    xd = x.double().cpu().reshape(n, -1, groups, c // groups)
+    mean = xd.mean((1, 3), keepdim=True)
+    var = (xd - mean).square().mean((1, 3), keepdim=True)
+    rstd = 1 / torch.sqrt(var + float(torch.tensor(1e-5, dtype=torch.float32)))
+    lost = 2.0 ** -50 * (1 + mean ** 2 / (var + 1e-5))
+    s = stats.double().cpu()
+    assert ((s[..., 0] - mean[:, 0, :, 0]).abs() <= 1.01 * U * mean[:, 0, :, 0].abs() + 1e-37).all()
+    rel = (s[..., 1] / rstd[:, 0, :, 0] - 1).abs()
+    assert (rel <= 1.01 * U + lost[:, 0, :, 0]).all(), float(rel.max() / U)
+    xh = (xd - mean) * rstd
+    wd, bd = w.double().cpu().reshape(groups, -1), b.double().cpu().reshape(groups, -1)
+    want = xh * wd + bd
+    tol = (4 * U + lost) * (xh * wd).abs() + 1.01 * U * mean.abs() * rstd * wd.abs() + (U + stored) * want.abs() + 1e-37
+    err = (y.double().cpu().reshape(want.shape) - want).abs()
+    assert (err <= 1.01 * tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("n,sp,c,groups", [(2, (256, 256), 32, 8), (1, (64, 64, 64), 16, 4), (1, (200, 210), 30, 5), (3, (16, 16), 256, 32), (2, (5, 7), 8, 2), (1, (300, 300), 8, 8)])
+@pytest.mark.parametrize("level", [0.0, 100.0])
+def test_a_pixel_unlike_all_others(dev, n, sp, c, groups, level):
+    """A bright pixel on an even background, at the first place of what a thread adds up or anywhere else: the variance is its doing alone."""
+    g = torch.Generator().manual_seed(c)
+    x = torch.full((n, math.prod(sp), c), level)
+    w, b = (1 + 0.2 * torch.randn(c, generator=g)).to(dev), (0.2 * torch.randn(c, generator=g)).to(dev)
+    for at in (0, 1, math.prod(sp) // 2, math.prod(sp) - 1):
+        y = x.clone()
+        y[:, at] += 0.5 + 2.5 * torch.rand(n, c, generator=g)
+        check_forward(y.reshape(n, *sp, c).to(dev), groups, w, b)
+
+
+@pytest.mark.parametrize("n,sp,c,groups", [(2, (256, 256), 32, 8), (1, (130, 170), 30, 5), (2, (12, 20), 64, 8), (1, (700, 700), 4, 1)])
+@pytest.mark.parametrize("mean,std", [(0.0, 1.0), (50.0, 1.0), (1000.0, 0.25), (3.0, 1e-2)])
+def test_statistics_are_their_definitions_rounded(dev, n, sp, c, groups, mean, std):
+    g = torch.Generator().manual_seed(c + int(mean))
+    x = (torch.randn(n, *sp, c, generator=g) * std + mean).to(dev)
+    w, b = (1 + 0.2 * torch.randn(c, generator=g)).to(dev), (0.2 * torch.randn(c, generator=g)).to(dev)
+    check_forward(x, groups, w, b)
+    check_forward(x.bfloat16(), groups, w, b, stored=2.0 ** -8)

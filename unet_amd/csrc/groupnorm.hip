@@ -12,8 +12,8 @@
 // channels live in registers.  VEC is the widest vector that the channel count, the pitches and the addresses of all
 // tensors of the call allow; dense tensors of odd channel counts go in runs of VEC pixels (see Runs).
 //
-// Sums: a thread adds fp32 differences from its own first value (at most CHUNK of them), so that a mean far from zero
-// does not cancel; from there on everything is fp64 plain sums, joined in a fixed order (no atomics).
+// Sums: the statistics are fp64 from the first addition on; the backward pass adds up to CHUNK fp32 gradients in a thread and goes on in fp64.  All
+// are joined in a fixed order (no atomics).
 #include <string.h>
 #include <type_traits>
 
@@ -351,10 +351,15 @@ __device__ __forceinline__ float2 moments(double a, double b, double cnt, double
     return make_float2((float)m, (float)(1.0 / sqrt(var + eps)));
 }
 
-// sum and sum of squares of cnt values k + d, from sums of d and d^2
-__device__ __forceinline__ void about_zero(double cnt, double k, double s1, double s2, double& d1, double& d2) {
-    d1 += cnt * k + s1;
-    d2 += cnt * k * k + 2.0 * k * s1 + s2;
+// sums of values and squares: fp64 holds both exactly.  (fp32 sums about a first value of the thread's own lost 2e-3 of the variance where that value was the
+// one bright pixel of an even image.)
+template <int VEC>
+__device__ __forceinline__ void add_moments(const float* v, double* d1, double* d2) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const double x = v[j];
+        d1[j] += x; d2[j] = fma(x, x, d2[j]);
+    }
 }
 
 // ---- forward, pass 1: sum and sum of squares per (image, split, group) -------------------------------------------
@@ -378,43 +383,28 @@ __global__ __launch_bounds__(TPB) void gn_stats_kernel(GnParams p) {
         double d1[VEC], d2[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) d1[j] = d2[j] = 0.0;
+        auto take = [&](const Raw<TR, VEC>& r) {
+            float v[VEC];
+            unraw<TR, VEC>(r, v);
+            add_moments<VEC>(v, d1, d2);
+        };
         int64_t left = l.row < l.rows && p0 + l.row < p1 ? (p1 - p0 - l.row + l.rows - 1) / l.rows : 0;
-        while (left > 0) {
-            const int cnt = (int)min((int64_t)CHUNK, left);
-            float k[VEC], s1[VEC], s2[VEC];
-            unraw<TR, VEC>(ldr<TR, VEC>(xc), k);
+        for (; left >= U; left -= U) {
+            Raw<TR, VEC> r[U];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s1[j] = s2[j] = 0.0f;
-            auto take = [&](const Raw<TR, VEC>& r) {
-                float v[VEC];
-                unraw<TR, VEC>(r, v);
+            for (int u = 0; u < U; ++u) r[u] = ldr<TR, VEC>(xc + u * step);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float d = v[j] - k[j];
-                    s1[j] += d; s2[j] = fmaf(d, d, s2[j]);
-                }
-            };
-            int i = 0;
-            for (; i + U <= cnt; i += U) {
-                Raw<TR, VEC> r[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) r[u] = ldr<TR, VEC>(xc + u * step);
-#pragma unroll
-                for (int u = 0; u < U; ++u) take(r[u]);
-                xc += U * step;
-            }
-            for (; i < cnt; ++i) { take(ldr<TR, VEC>(xc)); xc += step; }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) about_zero(cnt, k[j], s1[j], s2[j], d1[j], d2[j]);
-            left -= cnt;
+            for (int u = 0; u < U; ++u) take(r[u]);
+            xc += U * step;
         }
+        for (; left > 0; --left) { take(ldr<TR, VEC>(xc)); xc += step; }
         if (s == p.S - 1 && l.row == 0) {                           // behind the last run
             const int have = p.tail - l.col * VEC;
             float v[VEC];
             if (have > 0) ld_some<TR, VEC>(x + p.npix * p.x.pitch + l.col * (VEC * TR::ESZ), have, v);
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if (j < have) about_zero(1.0, v[j], 0.0, 0.0, d1[j], d2[j]);
+                if (j < have) { d1[j] += v[j]; d2[j] = fma((double)v[j], (double)v[j], d2[j]); }
         }
         add_groups<VEC>(p, sm, gs, d1, d2, l, col0 * VEC);
     }
@@ -755,24 +745,16 @@ __global__ __launch_bounds__(TPB) void gn_small_fwd_kernel(GnParams p) {
     for (int u = 0; u < NV; ++u)
         if (u < cnt) xv[u] = ldr<TR, VEC>(x + u * (l.rows * p.x.pitch));
     for (int g = tid; g < 2 * b.ng; g += TPB) gs[g] = 0.0;
-    float k[VEC], s1[VEC], s2[VEC];
+    double d1[VEC], d2[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) k[j] = s1[j] = s2[j] = 0.0f;
-    if (cnt) unraw<TR, VEC>(xv[0], k);
+    for (int j = 0; j < VEC; ++j) d1[j] = d2[j] = 0.0;
 #pragma unroll
-    for (int u = 1; u < NV; ++u)
+    for (int u = 0; u < NV; ++u)
         if (u < cnt) {
             float v[VEC];
             unraw<TR, VEC>(xv[u], v);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float d = v[j] - k[j];
-                s1[j] += d; s2[j] = fmaf(d, d, s2[j]);
-            }
+            add_moments<VEC>(v, d1, d2);
         }
-    double d1[VEC], d2[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) { d1[j] = d2[j] = 0.0; about_zero(cnt, k[j], s1[j], s2[j], d1[j], d2[j]); }
     add_groups<VEC>(p, sm, gs - 2 * b.g0, d1, d2, l, b.c0);
     float2* mr = reinterpret_cast<float2*>(sm);
     for (int g = tid; g < b.ng; g += TPB) {
