@@ -56,3 +56,19 @@ def test_statistics_are_their_definitions_rounded(dev, n, sp, c, groups, mean, s
     w, b = (1 + 0.2 * torch.randn(c, generator=g)).to(dev), (0.2 * torch.randn(c, generator=g)).to(dev)
     check_forward(x, groups, w, b)
     check_forward(x.bfloat16(), groups, w, b, stored=2.0 ** -8)
+
+
+def test_gelu_is_good_relatively_in_its_tail(dev):
+    """weight = 0: the activation sees the biases, exactly.  Phi(-|u|) is off by the fit, 4.8e-7, the exponential's 2^-23 and three roundings of its
+    exponent, 1.5 u^2 2^-24; the product with u adds 2^-24, and 1 - Phi another."""
+    u = torch.cat([torch.linspace(-12.5, 8.0, 4000), torch.tensor([0.0, -1e-30, 1e-30, -1e-3, 1e-3]), torch.linspace(-0.5, 0.5, 91)])
+    c = u.numel()
+    x = torch.randn(1, 3, 3, c, generator=torch.Generator().manual_seed(1)).to(dev)
+    y, _ = ops.groupnorm_act_fwd(x, 1, torch.zeros(c, device=dev), u.to(dev), act="gelu")
+    ud = u.double()
+    want = 0.5 * ud * torch.erfc(-ud * 0.5 ** 0.5)
+    rel = (y.double().cpu()[0].reshape(9, c) / want - 1).abs()
+    rel = torch.where(want == 0, torch.zeros_like(rel), rel)
+    bound = 4.8e-7 + (2 + 1.5 * ud ** 2 + 2) * U
+    assert (rel <= bound).all(), float((rel / bound).max())
+    assert not y[..., u.to(dev) == 0].any()
