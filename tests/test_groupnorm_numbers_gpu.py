@@ -72,3 +72,40 @@ def test_gelu_is_good_relatively_in_its_tail(dev):
     bound = 4.8e-7 + (2 + 1.5 * ud ** 2 + 2) * U
     assert (rel <= bound).all(), float((rel / bound).max())
     assert not y[..., u.to(dev) == 0].any()
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+def test_gradient_beyond_2_31_elements(dev, mode):
+    """One image whose upstream gradient is 0 except at its last pixels, 2^31 elements behind the first: the sums, and the gradient at both
+    ends, follow from those pixels alone.  Means of few values over all: u of each product."""
+    c, groups, last = 32, 4, 1000
+    npix = (1 << 31) // c + 5000
+    dt = torch.float32 if mode == "fp32" else torch.bfloat16
+    x = torch.empty(1, npix, 1, c, dtype=dt, device=dev).normal_(generator=torch.Generator(device=dev).manual_seed(1))
+    dy = torch.zeros(1, npix, 1, c, dtype=dt, device=dev)
+    g = torch.Generator().manual_seed(2)
+    dy[0, -last:, 0] = torch.randn(last, c, generator=g).to(dt).to(dev) * 1e3
+    w, b = (1 + 0.2 * torch.randn(c, generator=g)).to(dev), (0.2 * torch.randn(c, generator=g)).to(dev)
+    stats = torch.stack([0.01 * torch.randn(1, groups, generator=g), 1 + 0.1 * torch.rand(1, groups, generator=g)], -1).to(dev)
+    dx, dw, db, _ = ops.groupnorm_act_bwd(dy, x, stats, groups, w, b, act="relu")
+    mean, rstd = (stats[0, :, k].double().cpu().repeat_interleave(c // groups) for k in (0, 1))
+    wd, bd = w.double().cpu(), b.double().cpu()
+
+    def parts(rows):
+        xh = (x[0, rows, 0].double().cpu() - mean) * rstd
+        return xh, dy[0, rows, 0].double().cpu() * (xh * wd + bd > 0)
+
+    xh, gr = parts(slice(npix - last, npix))
+    for got, want, size in ((db, gr.sum(0), gr.abs().sum(0)), (dw, (gr * xh).sum(0), (gr * xh).abs().sum(0))):
+        assert ((got.double().cpu() - want).abs() <= 260 * U * size).all()                 # up to 256 values of a thread in fp32
+    count = npix * (c // groups)
+    m0 = ((gr * wd).sum(0).reshape(groups, -1).sum(1) / count).repeat_interleave(c // groups)
+    m1 = ((gr * wd * xh).sum(0).reshape(groups, -1).sum(1) / count).repeat_interleave(c // groups)
+    size = ((gr * wd).abs() * (1 + xh.abs())).sum() / count
+    assert float(size) > 1e-4
+    for rows in (slice(0, 50), slice(npix - last, npix)):
+        xh, gr = parts(rows)
+        want = rstd * (wd * gr - m0 - xh * m1)
+        tol = rstd * (8 * U * (wd * gr).abs() + 300 * U * size * (1 + xh.abs())) + (2.0 ** -8 if mode == "bf16" else U) * want.abs()
+        err = (dx[0, rows, 0].double().cpu() - want).abs()
+        assert (err <= 1.01 * tol).all(), float((err / tol).max())
