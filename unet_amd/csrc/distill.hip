@@ -134,11 +134,6 @@ struct Row {
             for (int j = 0; j < TR::VEC; ++j) x[i][j] = e0 + j < v ? x[i][j] : -INFINITY;
         }
     }
-    __device__ __forceinline__ void load(const char* z, int v, int L, int l) {
-        uint4 raw[NV];
-        fetch(raw, z, v, L, l);
-        take(raw, z, v, L, l);
-    }
     __device__ __forceinline__ float max_of(int L) const {
         float m = -INFINITY;
 #pragma unroll
