@@ -865,7 +865,7 @@ __global__ __launch_bounds__(1024) void distill_final(DistParams p) {
 // Short rows: the fewest lanes whose registers (NVMAX vectors each) hold the row and, 4 slots each, its list.  The backward
 // pass compares every held class with every slot while that is cheap, slots of other lanes costing their way here as well (not where a lane has few
 // rows: 50001 x 133 fp32, 5 slots 17 us, 20 through LDS); else it goes through LDS, with the rows of a workgroup within
-// 32 KB.  Steps by comparing and through LDS: 4000000 x 16 bf16, 4 slots (work 64) 173 and 186 us, 2000000 x 21, 4 (96) 143 and 151, 2000000 x 32, 8 (128) 192 and 193; 1000000 x 133 fp32, 5 (60, from many lanes) 526 and 466, 1000000 x 64 fp32, 5 (80) 216
+// 32 KB, or as few as 64 lanes each leave (four: 40 KB at 2048 bf16 classes and 256 slots).  Steps by comparing and through LDS: 4000000 x 16 bf16, 4 slots (work 64) 173 and 186 us, 2000000 x 21, 4 (96) 143 and 151, 2000000 x 32, 8 (128) 192 and 193; 1000000 x 133 fp32, 5 (60, from many lanes) 526 and 466, 1000000 x 64 fp32, 5 (80) 216
 // and 190, 100000 x 1000 bf16, 2 (64) 182 and 167.
 // Long rows, forward: a wave per row up to 1024 vectors, 256 threads behind that, 1024 where rows alone do not fill the chip (5 x
 // 32001 fp32: 256 threads 13.1 us, 1024 7.8).  Step: the fewest threads of 64, 256, 512, 1024 that hold the row with at

@@ -193,8 +193,8 @@ class TopLogitDistillationLoss(nn.Module):
     fills up short lists and leaves out pixels.  The weights of a class listed twice add.  ``reduction``: "mean" over the pixels with a used slot (0 if
     there are none), "sum", or "none" (one loss per pixel, 0 where no slot is used).  The gradient flows to ``input`` alone.
 
-    The loss of a pixel is good to a few 2^-24 of its parts, none of which is negative, also where the list holds all that the student's
-    distribution does (up to temperature 4: and to 2^-15 ``weight``; beyond 2048 bf16 or 1024 fp32 classes: and to ``(64 + classes / 256 + 2 k) 2^-24 weight
+    The loss of a pixel is good to a few 2^-24 of its parts, none of which is negative where no class repeats, also where the list holds all that
+    the student's distribution does (up to temperature 4: and to 2^-15 ``weight``; beyond 2048 bf16 or 1024 fp32 classes: and to ``(64 + classes / 256 + 2 k) 2^-24 weight
     temperature**2``).  The gradient is good to about 2^-20 of the two probabilities that it is the difference of.
 
     With more classes than 64 lanes hold (2048 bf16, 1024 fp32) the forward call of a training step writes the gradient along, for

@@ -2,7 +2,8 @@
 gradient / weight gradient, instance-norm + PReLU, group norm + activation and the top logits of a teacher.  Used by the operator parity tests and by
 callers that want to assemble other networks from the same kernels.
 
-Tensors are ``[N, (D,) H, W, C]`` contiguous, dtype ``torch.bfloat16`` or ``torch.float32``.
+Tensors are ``[N, (D,) H, W, C]`` contiguous, dtype ``torch.bfloat16`` or ``torch.float32``.  These are the kernels' calls, without autograd: results do
+not require a gradient, and the caller of a forward operator calls the backward one.
 """
 from __future__ import annotations
 
