@@ -282,3 +282,16 @@ def test_listed_classes_masked_with_the_lowest_value(dev, mode, v, k, temperatur
         assert torch.isfinite(dz).all()
     got, want, tol = check_rows(z, t.to(dev), i.to(dev), temperature, v <= 1024)
     assert (want[:3] > 1e33).all()
+
+
+def test_checkpointed_step_gives_the_gradient_of_the_plain_one(dev):
+    from torch.utils.checkpoint import checkpoint
+
+    g = torch.Generator().manual_seed(3)
+    fn = unet_amd.TopLogitDistillationLoss(2.0)
+    for v in (40, 5000):
+        x = torch.randn(30, v, generator=g).to(dev).requires_grad_(True)
+        t, i = torch.randn(30, 5, generator=g).to(dev), torch.randint(0, v, (30, 5), generator=g).to(dev)
+        (want,) = torch.autograd.grad(fn(x * 1.5, t, i), x)
+        (got,) = torch.autograd.grad(checkpoint(lambda a: fn(a * 1.5, t, i), x, use_reentrant=False), x)
+        assert torch.equal(got, want)
